@@ -13,6 +13,10 @@ int64_t acc_dbg_take_small_allreduce();
 int64_t acc_dbg_take_comm_pack();
 int64_t acc_dbg_take_moe_route();
 int64_t acc_dbg_take_cast();
+int64_t acc_dbg_take_layer_norm();
+int64_t acc_dbg_take_rope();
+int64_t acc_dbg_take_token_logprobs();
+int64_t acc_dbg_take_route_experts();
 bool debug_selftest(torch::Tensor out, int64_t overshoot);
 
 // (check id << 32 | source line) of the first failed device check since the last call, 0 if none; clears it.
@@ -20,7 +24,8 @@ static int64_t debug_status() {
   int64_t first = 0;
   for (auto fn : {acc_dbg_take_flash_attn, acc_dbg_take_fp8, acc_dbg_take_fp8_asm, acc_dbg_take_grouped_gemm, acc_dbg_take_norm_act,
                   acc_dbg_take_xent_optim, acc_dbg_take_small_allreduce, acc_dbg_take_comm_pack,
-                  acc_dbg_take_moe_route, acc_dbg_take_cast}) {
+                  acc_dbg_take_moe_route, acc_dbg_take_cast, acc_dbg_take_layer_norm, acc_dbg_take_rope,
+                  acc_dbg_take_token_logprobs, acc_dbg_take_route_experts}) {
     const int64_t w = fn();
     if (first == 0) first = w;
   }
@@ -40,6 +45,27 @@ void rope_inplace(torch::Tensor qkv, torch::Tensor cos, torch::Tensor sin, c10::
                   int64_t n_rot_heads, int64_t n_heads_total, int64_t head_dim, double sign);
 torch::Tensor rope_out(torch::Tensor src, torch::Tensor cos, torch::Tensor sin, c10::optional<torch::Tensor> pos,
                        int64_t n_rot_heads, int64_t n_heads_total, int64_t head_dim, double sign);
+// layer_norm.hip
+std::vector<torch::Tensor> layer_norm_fwd(torch::Tensor x, c10::optional<torch::Tensor> residual, c10::optional<torch::Tensor> w,
+                                          c10::optional<torch::Tensor> b, double eps, bool stats);
+std::vector<torch::Tensor> layer_norm_bwd(torch::Tensor dy, torch::Tensor s, c10::optional<torch::Tensor> w, torch::Tensor mean,
+                                          torch::Tensor rstd, c10::optional<torch::Tensor> dres, bool want_dw, bool want_db,
+                                          bool wide_params);
+// rope.hip
+torch::Tensor rope_any(torch::Tensor src, torch::Tensor cos, torch::Tensor sin, c10::optional<torch::Tensor> pos, int64_t n_rot,
+                       bool interleaved, double sign);
+// token_logprobs.hip
+std::vector<torch::Tensor> token_logprobs_fwd(torch::Tensor logits, torch::Tensor tokens, int64_t K, double inv_t, int64_t ignore,
+                                              bool want_stats);
+torch::Tensor token_logprobs_bwd(torch::Tensor logits, torch::Tensor tokens, torch::Tensor stats,
+                                 c10::optional<torch::Tensor> top_id, c10::optional<torch::Tensor> g_lp,
+                                 c10::optional<torch::Tensor> g_ent, c10::optional<torch::Tensor> g_top, double inv_t,
+                                 int64_t ignore);
+// route_experts.hip
+std::vector<torch::Tensor> route_experts_fwd(torch::Tensor logits, int64_t k, bool softmax, c10::optional<torch::Tensor> bias,
+                                             int64_t groups, int64_t top_groups, bool renorm, double scale);
+torch::Tensor route_experts_bwd(torch::Tensor logits, torch::Tensor weights, torch::Tensor experts, torch::Tensor dw, bool softmax,
+                                bool renorm, double scale);
 // xent_optim.hip
 std::vector<torch::Tensor> xent_fwd(torch::Tensor logits, torch::Tensor labels, int64_t ignore_index);
 void xent_bwd(torch::Tensor logits, torch::Tensor labels, torch::Tensor lse, torch::Tensor scale, torch::Tensor out,
@@ -134,6 +160,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("swiglu_bwd", &swiglu_bwd, pybind11::arg("gu"), pybind11::arg("dh"), pybind11::arg("amax") = pybind11::none());
   m.def("rope_inplace", &rope_inplace);
   m.def("rope_out", &rope_out);
+  m.def("layer_norm_fwd", &layer_norm_fwd);
+  m.def("layer_norm_bwd", &layer_norm_bwd);
+  m.def("rope_any", &rope_any);
+  m.def("token_logprobs_fwd", &token_logprobs_fwd);
+  m.def("token_logprobs_bwd", &token_logprobs_bwd);
+  m.def("route_experts_fwd", &route_experts_fwd);
+  m.def("route_experts_bwd", &route_experts_bwd);
   m.def("xent_fwd", &xent_fwd);
   m.def("xent_bwd", &xent_bwd);
   m.def("adam_multi_tensor", &adam_multi_tensor);

@@ -1,0 +1,400 @@
+// Layer norm, forward and backward, with the residual add fused in (bf16 / fp16 / fp32, statistics in fp32):
+//   s = round(x + residual),  y = (s - mean) * rstd * w + b,  rstd = 1 / sqrt(var + eps)
+//   g = dy * w,  dx = rstd * (g - mean(g) - h * mean(g * h)) (+ dres),  h = (s - mean) * rstd
+//   dw = sum over rows of dy * h,  db = sum over rows of dy
+// Both are bound by memory. The row stays in registers between its sums and its output, so x is read once; the variance
+// is the mean of squared distances from the mean, not a difference of two large sums. The threads of a row are chosen by
+// its width alone: one wave (no barrier) up to 256 16-byte chunks, then 256, 512 or 1024 threads.
+#include <hip/hip_runtime.h>
+#include <torch/extension.h>
+#include <ATen/hip/HIPContext.h>
+#include <algorithm>
+#include <type_traits>
+
+#include "row_ops.h"
+
+using namespace acc;
+
+namespace {
+
+constexpr int kMaxChunks = 4096;  // 16-byte chunks in a row: 32768 elements of 16 bits, 16384 of 32
+
+template <typename T, typename W, int TPR, int VPT>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_fwd_kernel(
+    const T* __restrict__ x, long x_stride, const T* __restrict__ res, long res_stride, const W* __restrict__ w,
+    const W* __restrict__ b, T* __restrict__ y, T* __restrict__ sum_out, float* __restrict__ mean_out,
+    float* __restrict__ rstd_out, long rows, int H, float eps) {
+  constexpr int VEC = 16 / sizeof(T), NT = TPR < 256 ? 256 : TPR, ROWS = NT / TPR;
+  __shared__ float slots[2][16];
+  const int li = threadIdx.x % TPR, nfull = H / VEC, tail = H % VEC;
+  const float width = (float)H;
+  // the trip count is uniform over each row's threads: one wave, or the whole block where barriers are used
+  for (long row = (long)blockIdx.x * ROWS + threadIdx.x / TPR; row < rows; row += (long)gridDim.x * ROWS) {
+    const T* xr = x + row * x_stride;
+    const T* rr = res == nullptr ? nullptr : res + row * res_stride;
+    float v[VPT][VEC];
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = li + i * TPR;
+      const int n = c < nfull ? VEC : (c == nfull ? tail : 0);
+      Pack<T, VEC> a = n == VEC ? load_any<T, VEC>(xr + c * VEC) : load_part<T, VEC>(xr + c * VEC, n);
+      if (rr != nullptr) {
+        const Pack<T, VEC> r = n == VEC ? load_any<T, VEC>(rr + c * VEC) : load_part<T, VEC>(rr + c * VEC, n);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) a.v[j] = from_f<T>(to_f<T>(a.v[j]) + to_f<T>(r.v[j]));
+        // what is normalised is what the residual stream stores
+        if (n == VEC) store_any<T, VEC>(sum_out + row * H + c * VEC, a);
+        else store_part<T, VEC>(sum_out + row * H + c * VEC, a, n);
+      }
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        v[i][j] = to_f<T>(a.v[j]);
+        sum += v[i][j];
+      }
+    }
+    const float mean = row_reduce<OpSum, TPR>(sum, slots[0]) / width;
+    float sq = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = li + i * TPR;
+      const int n = c < nfull ? VEC : (c == nfull ? tail : 0);
+      if (n == VEC) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          v[i][j] -= mean;
+          sq = fmaf(v[i][j], v[i][j], sq);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          v[i][j] = j < n ? v[i][j] - mean : 0.f;
+          sq = fmaf(v[i][j], v[i][j], sq);
+        }
+      }
+    }
+    const float rstd = 1.f / sqrtf(row_reduce<OpSum, TPR>(sq, slots[1]) / width + eps);
+    if (mean_out != nullptr && li == 0) {
+      mean_out[row] = mean;
+      rstd_out[row] = rstd;
+    }
+    T* yr = y + row * H;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = li + i * TPR;
+      const int n = c < nfull ? VEC : (c == nfull ? tail : 0);
+      if (n == 0) continue;
+      Pack<T, VEC> o;
+      Pack<W, VEC> ww, bb;
+      if (n == VEC) {
+        if (w != nullptr) ww = load_wide<W, VEC>(w + c * VEC);
+        if (b != nullptr) bb = load_wide<W, VEC>(b + c * VEC);
+      } else {
+        if (w != nullptr) ww = load_part<W, VEC>(w + c * VEC, n);
+        if (b != nullptr) bb = load_part<W, VEC>(b + c * VEC, n);
+      }
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        float f = v[i][j] * rstd;
+        if (w != nullptr) f *= to_f<W>(ww.v[j]);
+        if (b != nullptr) f += to_f<W>(bb.v[j]);
+        o.v[j] = from_f<T>(f);
+      }
+      if (n == VEC) store_any<T, VEC>(yr + c * VEC, o);
+      else store_part<T, VEC>(yr + c * VEC, o, n);
+    }
+  }
+}
+
+// One pass over the rows: dx, and each block's share of the column sums of dw and db in registers. The blocks' shares
+// (fp32, [blocks, 2, chunks * VEC]) are added up in a fixed order by layer_norm_colsum_kernel, so results repeat.
+template <typename T, typename W, int TPR, int VPT>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_bwd_kernel(
+    const T* __restrict__ dy, long dy_stride, const T* __restrict__ s, long s_stride, const W* __restrict__ w,
+    const float* __restrict__ mean, const float* __restrict__ rstd, const T* __restrict__ dres, long dres_stride,
+    T* __restrict__ dx, float* __restrict__ part, long rows, int H) {
+  constexpr int VEC = 16 / sizeof(T), NT = TPR < 256 ? 256 : TPR, ROWS = NT / TPR;
+  __shared__ float slots[2][2][16];
+  extern __shared__ float combine[];  // ROWS > 1: [2, chunks * VEC]
+  const int li = threadIdx.x % TPR, nfull = H / VEC, tail = H % VEC, chunks = (H + VEC - 1) / VEC;
+  const float width = (float)H;
+  float dw[VPT][VEC], db[VPT][VEC];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i)
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) dw[i][j] = db[i][j] = 0.f;
+  int parity = 0;
+  for (long row = (long)blockIdx.x * ROWS + threadIdx.x / TPR; row < rows; row += (long)gridDim.x * ROWS, parity ^= 1) {
+    const float mu = mean[row], r = rstd[row];
+    Pack<T, VEC> a[VPT], d[VPT];
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = li + i * TPR;
+      const int n = c < nfull ? VEC : (c == nfull ? tail : 0);
+      const T* ap = s + row * s_stride + c * VEC;
+      const T* dp = dy + row * dy_stride + c * VEC;
+      a[i] = n == VEC ? load_any<T, VEC>(ap) : load_part<T, VEC>(ap, n);
+      d[i] = n == VEC ? load_any<T, VEC>(dp) : load_part<T, VEC>(dp, n);  // zero past the row: adds nothing below
+    }
+    float s1 = 0.f, s2 = 0.f;
+    float g[VPT][VEC];
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = li + i * TPR;
+      const int n = c < nfull ? VEC : (c == nfull ? tail : 0);
+      Pack<W, VEC> ww;
+      if (w != nullptr) ww = n == VEC ? load_wide<W, VEC>(w + c * VEC) : load_part<W, VEC>(w + c * VEC, n);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const float dd = to_f<T>(d[i].v[j]), h = (to_f<T>(a[i].v[j]) - mu) * r;
+        g[i][j] = w != nullptr ? dd * to_f<W>(ww.v[j]) : dd;
+        dw[i][j] = fmaf(dd, h, dw[i][j]);
+        db[i][j] += dd;
+        s1 += g[i][j];
+        s2 = fmaf(g[i][j], h, s2);
+      }
+    }
+    s1 = wave_reduce<OpSum>(s1);
+    s2 = wave_reduce<OpSum>(s2);
+    if constexpr (TPR > 64) {  // both sums behind one barrier; the other parity's slots serve the next row
+      if ((threadIdx.x & 63) == 0) {
+        slots[parity][0][threadIdx.x >> 6] = s1;
+        slots[parity][1][threadIdx.x >> 6] = s2;
+      }
+      __syncthreads();
+      s1 = s2 = 0.f;
+#pragma unroll
+      for (int k = 0; k < TPR / 64; ++k) {
+        s1 += slots[parity][0][k];
+        s2 += slots[parity][1][k];
+      }
+    }
+    s1 /= width;
+    s2 /= width;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = li + i * TPR;
+      const int n = c < nfull ? VEC : (c == nfull ? tail : 0);
+      if (n == 0) continue;
+      Pack<T, VEC> q, o;
+      if (dres != nullptr) {
+        const T* qp = dres + row * dres_stride + c * VEC;
+        q = n == VEC ? load_any<T, VEC>(qp) : load_part<T, VEC>(qp, n);
+      }
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const float h = (to_f<T>(a[i].v[j]) - mu) * r;
+        float f = r * (g[i][j] - s1 - h * s2);
+        if (dres != nullptr) f += to_f<T>(q.v[j]);
+        o.v[j] = from_f<T>(f);
+      }
+      if (n == VEC) store_any<T, VEC>(dx + row * H + c * VEC, o);
+      else store_part<T, VEC>(dx + row * H + c * VEC, o, n);
+    }
+  }
+  if (part == nullptr) return;
+  const long pitch = (long)chunks * VEC;
+  float* out = part + (long)blockIdx.x * 2 * pitch;
+  if constexpr (ROWS > 1) {  // the block's waves add into shared memory one after another: a fixed order
+    for (int k = 0; k < ROWS; ++k) {
+      if ((int)threadIdx.x / TPR == k) {
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+          const int c = li + i * TPR;
+          if (c < chunks) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+              const int at = c * VEC + j;
+              combine[at] = k == 0 ? dw[i][j] : combine[at] + dw[i][j];
+              combine[pitch + at] = k == 0 ? db[i][j] : combine[pitch + at] + db[i][j];
+            }
+          }
+        }
+      }
+      __syncthreads();
+    }
+    for (long at = threadIdx.x; at < 2 * pitch; at += NT) out[at] = combine[at];
+  } else {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = li + i * TPR;
+      if (c < chunks) {
+#pragma unroll
+        for (int j = 0; j < VEC; j += 4) {
+          *reinterpret_cast<float4*>(out + c * VEC + j) = make_float4(dw[i][j], dw[i][j + 1], dw[i][j + 2], dw[i][j + 3]);
+          *reinterpret_cast<float4*>(out + pitch + c * VEC + j) =
+              make_float4(db[i][j], db[i][j + 1], db[i][j + 2], db[i][j + 3]);
+        }
+      }
+    }
+  }
+}
+
+// Column sums of the blocks' shares: 32 columns x 32 row groups per block, eight loads in flight per thread.
+template <typename W>
+__global__ __launch_bounds__(1024) void layer_norm_colsum_kernel(const float* __restrict__ part, W* __restrict__ dw,
+                                                                 W* __restrict__ db, int blocks, int H, long pitch) {
+  __shared__ float red[32][33];
+  const int c = threadIdx.x & 31, rg = threadIdx.x >> 5;
+  const long col = (long)blockIdx.x * 32 + c;
+  const float* src = part + blockIdx.y * pitch + col;
+  float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (col < H) {
+    int p = rg;
+    for (; p + 7 * 32 < blocks; p += 8 * 32)
+#pragma unroll
+      for (int u = 0; u < 8; ++u) acc[u] += src[(long)(p + 32 * u) * 2 * pitch];
+    for (; p < blocks; p += 32) acc[0] += src[(long)p * 2 * pitch];
+  }
+  red[rg][c] = ((acc[0] + acc[1]) + (acc[2] + acc[3])) + ((acc[4] + acc[5]) + (acc[6] + acc[7]));
+  __syncthreads();
+  if (rg == 0 && col < H) {
+    float t = 0.f;
+#pragma unroll
+    for (int k = 0; k < 32; ++k) t += red[k][c];
+    W* out = blockIdx.y == 0 ? dw : db;
+    if (out != nullptr) out[col] = from_f<W>(t);
+  }
+}
+
+void check_rows(const torch::Tensor& t, const char* name, const torch::Tensor& like) {
+  TORCH_CHECK(t.dim() == 2 && t.sizes() == like.sizes() && t.scalar_type() == like.scalar_type() && t.device() == like.device() &&
+                  (t.stride(1) == 1 || t.size(1) == 1 || t.numel() == 0),
+              "layer_norm: ", name, " must be a 2-D tensor of x's shape, type and device with contiguous rows");
+}
+
+void check_param(const c10::optional<torch::Tensor>& p, const char* name, const torch::Tensor& x) {
+  if (!p.has_value()) return;
+  TORCH_CHECK(p->dim() == 1 && p->size(0) == x.size(1) && p->is_contiguous() && p->device() == x.device() &&
+                  (p->scalar_type() == x.scalar_type() || p->scalar_type() == at::kFloat),
+              "layer_norm: ", name, " must be a contiguous [hidden] tensor in x's type or fp32, on x's device");
+}
+
+template <typename T>
+const T* ptr(const c10::optional<torch::Tensor>& t) { return t.has_value() ? reinterpret_cast<const T*>(t->data_ptr()) : nullptr; }
+template <typename T>
+T* out_ptr(const torch::Tensor& t) { return t.defined() ? reinterpret_cast<T*>(t.data_ptr()) : nullptr; }
+long row_stride(const c10::optional<torch::Tensor>& t) { return t.has_value() ? t->stride(0) : 0; }
+
+// Calls go(threads of a row, chunks of each) for a row of `chunks` 16-byte chunks.
+template <int N> using Const = std::integral_constant<int, N>;
+template <typename F>
+void by_width(long chunks, F go) {
+  if (chunks <= 64) go(Const<64>{}, Const<1>{});
+  else if (chunks <= 128) go(Const<64>{}, Const<2>{});
+  else if (chunks <= 256) go(Const<64>{}, Const<4>{});
+  else if (chunks <= 512) go(Const<256>{}, Const<2>{});
+  else if (chunks <= 1024) go(Const<256>{}, Const<4>{});
+  else if (chunks <= 2048) go(Const<512>{}, Const<4>{});
+  else go(Const<1024>{}, Const<4>{});
+}
+
+template <typename T, typename W>
+void launch_fwd(const torch::Tensor& x, const c10::optional<torch::Tensor>& res, const c10::optional<torch::Tensor>& w,
+                const c10::optional<torch::Tensor>& b, const torch::Tensor& y, const torch::Tensor& sum,
+                const torch::Tensor& mean, const torch::Tensor& rstd, float eps, hipStream_t stream) {
+  const long rows = x.size(0), H = x.size(1);
+  by_width((H * (long)sizeof(T) + 15) / 16, [&](auto tpr, auto vpt) {
+    constexpr int TPR = decltype(tpr)::value, VPT = decltype(vpt)::value, NT = TPR < 256 ? 256 : TPR, per = NT / TPR;
+    const long want = (rows + per - 1) / per, most = 2048L * 256 / NT;
+    hipLaunchKernelGGL((layer_norm_fwd_kernel<T, W, TPR, VPT>), dim3((unsigned)std::min(want, most)), dim3(NT), 0, stream,
+                       reinterpret_cast<const T*>(x.data_ptr()), x.stride(0), ptr<T>(res), row_stride(res), ptr<W>(w), ptr<W>(b),
+                       out_ptr<T>(y), out_ptr<T>(sum), out_ptr<float>(mean), out_ptr<float>(rstd), rows, (int)H, eps);
+  });
+}
+
+template <typename T, typename W>
+void launch_bwd(const torch::Tensor& dy, const torch::Tensor& s, const c10::optional<torch::Tensor>& w, const torch::Tensor& mean,
+                const torch::Tensor& rstd, const c10::optional<torch::Tensor>& dres, const torch::Tensor& dx,
+                const torch::Tensor& dw, const torch::Tensor& db, hipStream_t stream) {
+  constexpr int VEC = 16 / sizeof(T);
+  const long rows = s.size(0), H = s.size(1), chunks = (H + VEC - 1) / VEC, pitch = chunks * VEC;
+  const bool sums = dw.defined() || db.defined();
+  torch::Tensor part;
+  long blocks = 0;
+  by_width(chunks, [&](auto tpr, auto vpt) {
+    constexpr int TPR = decltype(tpr)::value, VPT = decltype(vpt)::value, NT = TPR < 256 ? 256 : TPR, per = NT / TPR;
+    blocks = std::min((rows + per - 1) / per, 512L * 256 / NT);
+    if (sums) part = torch::empty({blocks, 2, pitch}, s.options().dtype(at::kFloat));
+    hipLaunchKernelGGL((layer_norm_bwd_kernel<T, W, TPR, VPT>), dim3((unsigned)blocks), dim3(NT),
+                       per > 1 && sums ? 2 * pitch * sizeof(float) : 0, stream, reinterpret_cast<const T*>(dy.data_ptr()),
+                       dy.stride(0), reinterpret_cast<const T*>(s.data_ptr()), s.stride(0), ptr<W>(w), mean.data_ptr<float>(),
+                       rstd.data_ptr<float>(), ptr<T>(dres), row_stride(dres), out_ptr<T>(dx), out_ptr<float>(part), rows, (int)H);
+  });
+  if (sums)
+    hipLaunchKernelGGL((layer_norm_colsum_kernel<W>), dim3((unsigned)((H + 31) / 32), 2), dim3(1024), 0, stream,
+                       part.data_ptr<float>(), out_ptr<W>(dw), out_ptr<W>(db), (int)blocks, (int)H, pitch);
+}
+
+}  // namespace
+
+ACC_DEBUG_TAKE_FN(acc_dbg_take_layer_norm)
+
+// y [, s] [, mean, rstd (`stats`)] for x [rows, hidden].
+std::vector<torch::Tensor> layer_norm_fwd(torch::Tensor x, c10::optional<torch::Tensor> residual, c10::optional<torch::Tensor> w,
+                                          c10::optional<torch::Tensor> b, double eps, bool stats) {
+  TORCH_CHECK(x.is_cuda() && x.dim() == 2, "layer_norm: x must be a 2-D HIP tensor");
+  check_rows(x, "x", x);
+  if (residual.has_value()) check_rows(*residual, "residual", x);
+  check_param(w, "weight", x);
+  check_param(b, "bias", x);
+  TORCH_CHECK(!w.has_value() || !b.has_value() || w->scalar_type() == b->scalar_type(), "layer_norm: weight and bias of one type");
+  const long rows = x.size(0);
+  const int H = (int)x.size(1);
+  const long chunks = (x.size(1) * x.element_size() + 15) / 16;
+  TORCH_CHECK(x.size(1) >= 1 && chunks <= kMaxChunks, "layer_norm: 1 to ", kMaxChunks * 16 / x.element_size(), " columns expected");
+  const c10::DeviceGuard guard(x.device());
+  auto y = torch::empty({rows, H}, x.options());
+  torch::Tensor sum, mean, rstd;
+  if (residual.has_value()) sum = torch::empty({rows, H}, x.options());
+  if (stats) {
+    mean = torch::empty({rows}, x.options().dtype(torch::kFloat32));
+    rstd = torch::empty({rows}, x.options().dtype(torch::kFloat32));
+  }
+  if (rows == 0) return {y, sum, mean, rstd};
+  auto stream = at::hip::getCurrentHIPStream();
+  const bool wide = (w.has_value() ? w->scalar_type() : b.has_value() ? b->scalar_type() : x.scalar_type()) == at::kFloat;
+  ACC_FOR_FLOAT_TYPES(x.scalar_type(), "layer_norm", {
+    if (wide) launch_fwd<scalar, float>(x, residual, w, b, y, sum, mean, rstd, (float)eps, stream);
+    else launch_fwd<scalar, scalar>(x, residual, w, b, y, sum, mean, rstd, (float)eps, stream);
+  });
+  return {y, sum, mean, rstd};
+}
+
+// dx [, dw] [, db] as `want_dw` / `want_db` ask for them, in fp32 (`wide_params`) or the input's type. `w`, where given, has
+// that type too.
+std::vector<torch::Tensor> layer_norm_bwd(torch::Tensor dy, torch::Tensor s, c10::optional<torch::Tensor> w, torch::Tensor mean,
+                                          torch::Tensor rstd, c10::optional<torch::Tensor> dres, bool want_dw, bool want_db,
+                                          bool wide_params) {
+  TORCH_CHECK(s.is_cuda() && s.dim() == 2, "layer_norm: the normalised input must be a 2-D HIP tensor");
+  check_rows(s, "input", s);
+  check_rows(dy, "dy", s);
+  if (dres.has_value()) check_rows(*dres, "dres", s);
+  check_param(w, "weight", s);
+  TORCH_CHECK(!w.has_value() || (w->scalar_type() == at::kFloat) == (wide_params || s.scalar_type() == at::kFloat),
+              "layer_norm: the weight's type and wide_params differ");
+  const long rows = s.size(0);
+  for (const auto& t : {mean, rstd})
+    TORCH_CHECK(t.scalar_type() == at::kFloat && t.is_contiguous() && t.numel() == rows && t.device() == s.device(),
+                "layer_norm: mean and rstd must be fp32 [rows]");
+  const int H = (int)s.size(1);
+  const long chunks = (s.size(1) * s.element_size() + 15) / 16;
+  TORCH_CHECK(s.size(1) >= 1 && chunks <= kMaxChunks, "layer_norm: 1 to ", kMaxChunks * 16 / s.element_size(), " columns expected");
+  const c10::DeviceGuard guard(s.device());
+  auto dx = torch::empty({rows, H}, s.options());
+  const auto popt = s.options().dtype(wide_params ? at::kFloat : s.scalar_type());
+  torch::Tensor dw, db;
+  if (rows == 0) {
+    if (want_dw) dw = torch::zeros({H}, popt);
+    if (want_db) db = torch::zeros({H}, popt);
+    return {dx, dw, db};
+  }
+  if (want_dw) dw = torch::empty({H}, popt);
+  if (want_db) db = torch::empty({H}, popt);
+  auto stream = at::hip::getCurrentHIPStream();
+  ACC_FOR_FLOAT_TYPES(s.scalar_type(), "layer_norm", {
+    if (wide_params) launch_bwd<scalar, float>(dy, s, w, mean, rstd, dres, dx, dw, db, stream);
+    else launch_bwd<scalar, scalar>(dy, s, w, mean, rstd, dres, dx, dw, db, stream);
+  });
+  return {dx, dw, db};
+}

@@ -1,0 +1,393 @@
+// Log-probabilities of given tokens, the entropy of their distributions and the k best alternatives, over logits [rows, V]
+// (bf16 / fp16 / fp32, all sums in fp32), and the gradient of all three. With z = logits / temperature and one pass that
+// keeps the running maximum m, S = sum e^(x - m) and U = sum (x - m) e^(x - m) of each row:
+//   log p_i = (x_i - m) / T - log S,   H = log S - U / (S T)
+//   dlogits_i = (1/T) [ -p_i (G + dH (log p_i + H)) + sum of the gradients of the outputs that name i ],
+//   G = the sum of the row's log-probability gradients.
+// Bound by memory: the forward reads the logits once, the backward reads them once and writes the gradient once. An -inf
+// logit has p = 0 and adds nothing. A row whose token is `ignore` is not read: 0, 0, 0 and -1, and a zero gradient. A row
+// without a distribution (NaN, +inf, all -inf) gives NaN and alternatives -1; a token outside [0, V) gives NaN.
+#include <hip/hip_runtime.h>
+#include <torch/extension.h>
+#include <ATen/hip/HIPContext.h>
+#include <algorithm>
+
+#include "row_ops.h"
+
+using namespace acc;
+
+namespace {
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr int kMaxTop = 64;
+constexpr int kList = 2048;  // candidates of a row kept in shared memory
+constexpr int kBwdThreads = 256, kBwdUnroll = 4;
+
+// Keys ordered as (value, then lower index): the larger key is the better alternative. Equal values, -0 and +0 among them,
+// differ in the index alone, so all keys of a row are distinct.
+__device__ __forceinline__ uint64_t key_of(float x, int index) {
+  uint32_t u = __float_as_uint(x + 0.f);
+  u ^= (u & 0x80000000u) ? 0xffffffffu : 0x80000000u;
+  return ((uint64_t)u << 32) | (uint32_t)~index;
+}
+__device__ __forceinline__ float key_value(uint64_t k) {
+  uint32_t u = (uint32_t)(k >> 32);
+  u ^= (u & 0x80000000u) ? 0x80000000u : 0xffffffffu;
+  return __uint_as_float(u);
+}
+__device__ __forceinline__ int key_index(uint64_t k) { return (int)~(uint32_t)k; }
+
+__device__ __forceinline__ uint64_t key_max(uint64_t a, uint64_t b) { return a > b ? a : b; }
+
+// e^((x - m) * scale) for scale2 = scale * log2(e)
+__device__ __forceinline__ float exp_scaled(float d, float scale2) { return __builtin_amdgcn_exp2f(d * scale2); }
+
+template <typename T, int NT, int UNROLL>
+__global__ __launch_bounds__(NT) void token_logprobs_fwd_kernel(
+    const T* __restrict__ logits, long stride, const int64_t* __restrict__ tokens, float* __restrict__ lp_out,
+    float* __restrict__ ent_out, float* __restrict__ top_lp, int64_t* __restrict__ top_id, float* __restrict__ stats, int V, int K,
+    float inv_t, int64_t ignore) {
+  constexpr int VEC = 16 / sizeof(T), GROUPS = NT / 4;
+  __shared__ float slots[4][16];
+  __shared__ uint64_t group_key[GROUPS];
+  __shared__ uint64_t list[kList];
+  __shared__ uint64_t threshold, round_key[NT / 64];
+  __shared__ int n_list, n_threads, threads_list[NT];
+  const long row = blockIdx.x;
+  const int tid = threadIdx.x;
+  const int64_t tok = tokens[row];
+  if (tok == ignore) {  // uniform over the block
+    if (tid == 0) {
+      lp_out[row] = 0.f;
+      ent_out[row] = 0.f;
+    }
+    for (int j = tid; j < K; j += NT) {
+      top_lp[row * K + j] = 0.f;
+      top_id[row * K + j] = -1;
+    }
+    return;
+  }
+  const T* x = logits + row * stride;
+  const int nfull = V / VEC, tail = V % VEC, chunks = nfull + (tail > 0);
+  const float scale2 = inv_t * kLog2e;
+
+  // one pass: running maximum, sum and weighted sum per thread, and the chunk that holds the thread's maximum
+  float m = -INFINITY, sum = 0.f, wsum = 0.f;
+  int best = -1;
+  auto take = [&](const float (&f)[VEC], int c) {
+    float hi = f[0];
+#pragma unroll
+    for (int j = 1; j < VEC; ++j) hi = fmaxf(hi, f[j]);
+    if (hi > m) {
+      if (m > -INFINITY) {
+        const float a = exp_scaled(m - hi, scale2);
+        wsum = (wsum + fmaxf(m - hi, -1e30f) * sum) * a;
+        sum *= a;
+      }
+      m = hi;
+      best = c;
+    }
+    const float base = m > -INFINITY ? m : 0.f;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      const float d = f[j] - base, e = exp_scaled(d, scale2);
+      sum += e;
+      wsum = fmaf(fmaxf(d, -1e30f), e, wsum);  // -inf: a finite distance times zero
+    }
+  };
+  int c = tid;
+  for (; c + (UNROLL - 1) * NT < nfull; c += UNROLL * NT) {
+    Pack<T, VEC> p[UNROLL];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) p[u] = load_any<T, VEC>(x + (long)(c + u * NT) * VEC);
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      float f[VEC];
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) f[j] = to_f<T>(p[u].v[j]);
+      take(f, c + u * NT);
+    }
+  }
+  for (; c < chunks; c += NT) {
+    float f[VEC];
+    if (c < nfull) {
+      const Pack<T, VEC> p = load_any<T, VEC>(x + (long)c * VEC);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) f[j] = to_f<T>(p.v[j]);
+    } else {
+      const Pack<T, VEC> p = load_part<T, VEC>(x + (long)c * VEC, tail);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) f[j] = j < tail ? to_f<T>(p.v[j]) : -INFINITY;
+    }
+    take(f, c);
+  }
+  const float gm = row_reduce<OpMax, NT>(m, slots[0]);
+  if (m > -INFINITY && gm < INFINITY) {
+    const float a = exp_scaled(m - gm, scale2);
+    wsum = (wsum + fmaxf(m - gm, -1e30f) * sum) * a;
+    sum *= a;
+  }
+  const float S = row_reduce<OpSum, NT>(sum, slots[1]), U = row_reduce<OpSum, NT>(wsum, slots[2]);
+  const bool sound = S > 0.f && S < INFINITY;  // false for NaN too
+  const float log_s = sound ? logf(S) : NAN;
+  const float ent = sound ? log_s - inv_t * (U / S) : NAN;
+  if (tid == 0) {
+    const bool named = tok >= 0 && tok < V;
+    ACC_CHECK(named, kChkXentLabel);
+    lp_out[row] = named && sound ? (to_f<T>(x[named ? tok : 0]) - gm) * inv_t - log_s : NAN;
+    ent_out[row] = ent;
+    if (stats != nullptr) {
+      stats[row * 3] = gm;
+      stats[row * 3 + 1] = log_s;
+      stats[row * 3 + 2] = ent;
+    }
+  }
+  if (K == 0) return;
+  if (!sound) {
+    for (int j = tid; j < K; j += NT) {
+      top_lp[row * K + j] = NAN;
+      top_id[row * K + j] = -1;
+    }
+    return;
+  }
+
+  // The K best alternatives. Each group of four threads has its best key; the K-th best of those is a bound that K elements
+  // at least reach and few exceed. The threads whose own best reaches it read their chunks again (a few of them, from the
+  // cache) and list every element that does; the list is ranked by counting.
+  uint64_t mine = 0;
+  if (tid < chunks) {
+    if (best < 0) best = tid;  // nothing above -inf: the first element stands for the thread
+    const int n = best < nfull ? VEC : tail;
+    for (int j = n - 1; j >= 0; --j) {
+      const float f = to_f<T>(x[(long)best * VEC + j]);
+      if (f == m) mine = key_of(f, best * VEC + j);
+    }
+  }
+  uint64_t g = mine;
+  g = key_max(g, (uint64_t)__shfl_xor((unsigned long long)g, 1, 64));
+  g = key_max(g, (uint64_t)__shfl_xor((unsigned long long)g, 2, 64));
+  if ((tid & 3) == 0) group_key[tid >> 2] = g;
+  if (tid == 0) {
+    threshold = 0;
+    n_list = 0;
+    n_threads = 0;
+  }
+  __syncthreads();
+  {
+    int above = 0;
+    for (int i = 0; i < GROUPS / 4; ++i) above += group_key[(tid & 3) * (GROUPS / 4) + i] > g;
+    above += __shfl_xor(above, 1, 64);
+    above += __shfl_xor(above, 2, 64);
+    if ((tid & 3) == 0 && above == K - 1 && g != 0) threshold = g;  // one group: the keys differ
+  }
+  __syncthreads();
+  const uint64_t bound = threshold;
+  if (mine != 0 && mine >= bound) threads_list[atomicAdd(&n_threads, 1)] = tid;
+  __syncthreads();
+  {
+    const int lane = tid & 63, waves = NT / 64, nt = n_threads;
+    for (int i = tid >> 6; i < nt; i += waves) {
+      for (int cc = threads_list[i] + lane * NT; cc < chunks; cc += 64 * NT) {
+        const int n = cc < nfull ? VEC : tail;
+        const Pack<T, VEC> p = n == VEC ? load_any<T, VEC>(x + (long)cc * VEC) : load_part<T, VEC>(x + (long)cc * VEC, n);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const uint64_t k = key_of(to_f<T>(p.v[j]), cc * VEC + j);
+          if (j < n && k >= bound) {
+            const int at = atomicAdd(&n_list, 1);
+            if (at < kList) list[at] = k;
+          }
+        }
+      }
+    }
+  }
+  __syncthreads();
+  const int n = n_list;
+  if (n <= kList) {
+    for (int i = tid; i < n; i += NT) {
+      const uint64_t k = list[i];
+      int rank = 0;
+      for (int q = 0; q < n; ++q) rank += list[q] > k;
+      if (rank < K) {
+        top_lp[row * K + rank] = (key_value(k) - gm) * inv_t - log_s;
+        top_id[row * K + rank] = key_index(k);
+      }
+    }
+    return;
+  }
+  // More elements of a few threads than the list holds reach the bound (a row whose largest values all lie one thread's
+  // stride apart): the best one below the last, K times over the row.
+  uint64_t last = ~0ull;
+  for (int r = 0; r < K; ++r) {
+    uint64_t k = 0;
+    for (int cc = tid; cc < chunks; cc += NT) {
+      const int nn = cc < nfull ? VEC : tail;
+      for (int j = 0; j < nn; ++j) {
+        const uint64_t q = key_of(to_f<T>(x[(long)cc * VEC + j]), cc * VEC + j);
+        if (q < last) k = key_max(k, q);
+      }
+    }
+    for (int o = 1; o < 64; o <<= 1) k = key_max(k, (uint64_t)__shfl_xor((unsigned long long)k, o, 64));
+    __syncthreads();
+    if ((tid & 63) == 0) round_key[tid >> 6] = k;
+    __syncthreads();
+    for (int i = 0; i < NT / 64; ++i) k = key_max(k, round_key[i]);
+    last = k;
+    if (tid == 0) {
+      top_lp[row * K + r] = (key_value(k) - gm) * inv_t - log_s;
+      top_id[row * K + r] = key_index(k);
+    }
+  }
+}
+
+// blockIdx.x: a span of kBwdThreads * kBwdUnroll chunks, blockIdx.y / z: the row.
+template <typename T>
+__global__ __launch_bounds__(kBwdThreads) void token_logprobs_bwd_kernel(
+    const T* __restrict__ logits, long stride, const int64_t* __restrict__ tokens, const float* __restrict__ stats,
+    const int64_t* __restrict__ top_id, const float* __restrict__ g_lp, long g_lp_stride, const float* __restrict__ g_ent,
+    long g_ent_stride, const float* __restrict__ g_top, T* __restrict__ out, long rows, int V, int K, float inv_t, int64_t ignore,
+    int spans) {
+  constexpr int VEC = 16 / sizeof(T);
+  const long row = blockIdx.x / spans;
+  const int span = (int)(blockIdx.x - row * spans), tid = threadIdx.x;
+  const int nfull = V / VEC, tail = V % VEC, chunks = nfull + (tail > 0);
+  const int64_t tok = tokens[row];
+  const int c0 = span * kBwdThreads * kBwdUnroll;
+  T* o = out + row * (long)V;
+  if (tok == ignore) {
+    Pack<T, VEC> z;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) z.v[j] = T(0);
+    for (int u = 0; u < kBwdUnroll; ++u) {
+      const int c = c0 + u * kBwdThreads + tid;
+      if (c < nfull) store_any<T, VEC>(o + (long)c * VEC, z);
+      else if (c < chunks) store_part<T, VEC>(o + (long)c * VEC, z, tail);
+    }
+    return;
+  }
+  const T* x = logits + row * stride;
+  Pack<T, VEC> p[kBwdUnroll];
+#pragma unroll
+  for (int u = 0; u < kBwdUnroll; ++u) {
+    const int c = c0 + u * kBwdThreads + tid;
+    if (c < nfull) p[u] = load_any<T, VEC>(x + (long)c * VEC);
+    else if (c < chunks) p[u] = load_part<T, VEC>(x + (long)c * VEC, tail);
+  }
+  const float gm = stats[row * 3], log_s = stats[row * 3 + 1], ent = stats[row * 3 + 2];
+  const float gl = g_lp != nullptr ? g_lp[row * g_lp_stride] : 0.f, gh = g_ent != nullptr ? g_ent[row * g_ent_stride] : 0.f;
+  float total = gl;
+  if (g_top != nullptr)
+    for (int j = 0; j < K; ++j) total += g_top[row * K + j];
+  // a token outside [0, V) had no log-probability: the row's gradient is NaN with it
+  if (tok < 0 || tok >= V) total = NAN;
+  auto value = [&](float f) {
+    const float lp = fmaxf((f - gm) * inv_t, -1e30f) - log_s;
+    const float prob = exp_scaled(f - gm, inv_t * kLog2e) * __builtin_amdgcn_exp2f(-log_s * kLog2e);
+    return -prob * (total + gh * (lp + ent));
+  };
+#pragma unroll
+  for (int u = 0; u < kBwdUnroll; ++u) {
+    const int c = c0 + u * kBwdThreads + tid;
+    if (c >= chunks) continue;
+    Pack<T, VEC> q;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) q.v[j] = from_f<T>(value(to_f<T>(p[u].v[j])) * inv_t);
+    if (c < nfull) store_any<T, VEC>(o + (long)c * VEC, q);
+    else store_part<T, VEC>(o + (long)c * VEC, q, tail);
+  }
+  // the named elements of this span, each written again by one thread with all its terms and one rounding
+  __syncthreads();
+  const int named = g_top != nullptr ? K : 0;
+  if (tid > named) return;
+  const int64_t id = tid < named ? top_id[row * K + tid] : tok;
+  const long lo = (long)c0 * VEC, hi = lo + (long)kBwdThreads * kBwdUnroll * VEC;
+  if (id < lo || id >= hi || id >= V) return;  // -1 (no alternatives in this row) falls out here
+  float extra = 0.f;
+  if (tid < named) {
+    extra = g_top[row * K + tid] + (id == tok ? gl : 0.f);
+  } else {
+    for (int j = 0; j < named; ++j)
+      if (top_id[row * K + j] == tok) return;  // that alternative's thread writes it
+    extra = gl;
+  }
+  o[id] = from_f<T>((value(to_f<T>(x[id])) + extra) * inv_t);
+}
+
+void check_logits(const torch::Tensor& logits, const torch::Tensor& tokens) {
+  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && (logits.stride(1) == 1 || logits.size(1) == 1 || logits.numel() == 0),
+              "token_logprobs: logits must be a 2-D HIP tensor with contiguous rows");
+  TORCH_CHECK(logits.size(1) >= 1 && logits.size(1) < (1L << 31) - 65536, "token_logprobs: 1 to 2^31 - 65536 columns expected");
+  TORCH_CHECK(tokens.dim() == 1 && tokens.size(0) == logits.size(0) && tokens.scalar_type() == at::kLong &&
+                  tokens.is_contiguous() && tokens.device() == logits.device(),
+              "token_logprobs: tokens must be a contiguous int64 [rows] tensor on the logits' device");
+  TORCH_CHECK(logits.size(0) < (1L << 31), "token_logprobs: too many rows");
+}
+
+}  // namespace
+
+ACC_DEBUG_TAKE_FN(acc_dbg_take_token_logprobs)
+
+// logprobs [rows], entropy [rows], top log-probabilities and tokens [rows, K] (K > 0), stats [rows, 3] (`want_stats`).
+std::vector<torch::Tensor> token_logprobs_fwd(torch::Tensor logits, torch::Tensor tokens, int64_t K, double inv_t, int64_t ignore,
+                                              bool want_stats) {
+  check_logits(logits, tokens);
+  const long rows = logits.size(0), V = logits.size(1);
+  TORCH_CHECK(K >= 0 && K <= kMaxTop && K <= V, "token_logprobs: 0 to ", kMaxTop, " alternatives, no more than the vocabulary");
+  const c10::DeviceGuard guard(logits.device());
+  const auto fopt = logits.options().dtype(torch::kFloat32);
+  auto lp = torch::empty({rows}, fopt), ent = torch::empty({rows}, fopt);
+  torch::Tensor top_lp, top_id, stats;
+  if (K > 0) {
+    top_lp = torch::empty({rows, K}, fopt);
+    top_id = torch::empty({rows, K}, fopt.dtype(torch::kInt64));
+  }
+  if (want_stats) stats = torch::empty({rows, 3}, fopt);
+  if (rows > 0) {
+    auto stream = at::hip::getCurrentHIPStream();
+    ACC_FOR_FLOAT_TYPES(logits.scalar_type(), "token_logprobs", {
+      hipLaunchKernelGGL((token_logprobs_fwd_kernel<scalar, 512, 4>), dim3((unsigned)rows), dim3(512), 0, stream,
+                         reinterpret_cast<const scalar*>(logits.data_ptr()), logits.stride(0), tokens.data_ptr<int64_t>(),
+                         lp.data_ptr<float>(), ent.data_ptr<float>(), K > 0 ? top_lp.data_ptr<float>() : nullptr,
+                         K > 0 ? top_id.data_ptr<int64_t>() : nullptr, want_stats ? stats.data_ptr<float>() : nullptr, (int)V,
+                         (int)K, (float)inv_t, ignore);
+    });
+  }
+  return {lp, ent, top_lp, top_id, stats};
+}
+
+torch::Tensor token_logprobs_bwd(torch::Tensor logits, torch::Tensor tokens, torch::Tensor stats,
+                                 c10::optional<torch::Tensor> top_id, c10::optional<torch::Tensor> g_lp,
+                                 c10::optional<torch::Tensor> g_ent, c10::optional<torch::Tensor> g_top, double inv_t,
+                                 int64_t ignore) {
+  check_logits(logits, tokens);
+  const long rows = logits.size(0), V = logits.size(1);
+  const c10::DeviceGuard guard(logits.device());
+  TORCH_CHECK(stats.scalar_type() == at::kFloat && stats.is_contiguous() && stats.numel() == rows * 3, "token_logprobs: stats");
+  for (const auto& g : {g_lp, g_ent})
+    TORCH_CHECK(!g.has_value() || (g->scalar_type() == at::kFloat && g->dim() == 1 && g->size(0) == rows && g->device() == logits.device()),
+                "token_logprobs: gradients must be fp32 [rows]");
+  long K = 0;
+  if (g_top.has_value()) {
+    TORCH_CHECK(top_id.has_value() && top_id->dim() == 2 && top_id->scalar_type() == at::kLong && top_id->is_contiguous() &&
+                    g_top->scalar_type() == at::kFloat && g_top->is_contiguous() && g_top->sizes() == top_id->sizes() &&
+                    top_id->size(0) == rows && top_id->size(1) <= kMaxTop && g_top->device() == logits.device(),
+                "token_logprobs: the alternatives' gradients must be fp32 [rows, K]");
+    K = top_id->size(1);
+  }
+  auto out = torch::empty({rows, V}, logits.options());
+  if (rows == 0) return out;
+  auto stream = at::hip::getCurrentHIPStream();
+  ACC_FOR_FLOAT_TYPES(logits.scalar_type(), "token_logprobs", {
+    constexpr long per = 16 / sizeof(scalar) * kBwdThreads * kBwdUnroll;
+    const long spans = (V + per - 1) / per;
+    TORCH_CHECK(rows * spans < (1L << 31), "token_logprobs: too many rows in one call");
+    hipLaunchKernelGGL((token_logprobs_bwd_kernel<scalar>), dim3((unsigned)(rows * spans)), dim3(kBwdThreads), 0, stream,
+                       reinterpret_cast<const scalar*>(logits.data_ptr()), logits.stride(0), tokens.data_ptr<int64_t>(),
+                       stats.data_ptr<float>(), K > 0 ? top_id->data_ptr<int64_t>() : nullptr,
+                       g_lp.has_value() ? g_lp->data_ptr<float>() : nullptr, g_lp.has_value() ? g_lp->stride(0) : 0,
+                       g_ent.has_value() ? g_ent->data_ptr<float>() : nullptr, g_ent.has_value() ? g_ent->stride(0) : 0,
+                       K > 0 ? g_top->data_ptr<float>() : nullptr, reinterpret_cast<scalar*>(out.data_ptr()), rows, (int)V, (int)K,
+                       (float)inv_t, ignore, (int)spans);
+  });
+  return out;
+}

@@ -39,10 +39,16 @@ class LlamaConfig:
     rms_norm_eps: float = 1e-5
     rope_theta: float = 500000.0
     rope_scaling: Optional[dict] = None
+    rope_interleaved: bool = False  # pairs (2i, 2i + 1) instead of (i, i + R/2)
+    partial_rotary_factor: float = 1.0  # the share of each head that is rotated
     max_position_embeddings: int = 8192
     tie_word_embeddings: bool = False
     initializer_range: float = 0.02
     activation_checkpointing: bool = False
+
+    @property
+    def rotary_dim(self) -> int:
+        return int(self.head_dim * self.partial_rotary_factor)
 
     @property
     def num_params(self) -> int:
@@ -120,7 +126,7 @@ class LlamaAttention(nn.Module):
         qkv = self.qkv_proj(x)
         S = qkv.shape[1]  # sequence-parallel TP gathers the sequence inside qkv_proj
         qkv = qkv.view(B, S, self.n_q + 2 * self.n_kv, self.head_dim)
-        qkv = apply_rope(qkv, cos, sin, self.n_q + self.n_kv, position_ids)
+        qkv = apply_rope(qkv, cos, sin, self.n_q + self.n_kv, position_ids, self.cfg.rope_interleaved, self.cfg.rotary_dim)
         if self.attention_impl is not None:
             o = self.attention_impl(qkv, self.n_q, self.n_kv)
         else:
@@ -204,7 +210,7 @@ class LlamaForCausalLM(nn.Module):
         key = (S, str(device))
         if key not in self._rope_cache:
             n = max(S, self.config.max_position_embeddings if S > self.config.max_position_embeddings else S)
-            self._rope_cache[key] = rope_tables(n, self.config.head_dim, self.config.rope_theta, device, self.config.rope_scaling)
+            self._rope_cache[key] = rope_tables(n, self.config.rotary_dim, self.config.rope_theta, device, self.config.rope_scaling)
         return self._rope_cache[key]
 
     def forward(self, input_ids, labels=None, position_ids=None, attention_mask=None, return_logits: bool = True,

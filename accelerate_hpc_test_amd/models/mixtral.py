@@ -34,6 +34,11 @@ class MixtralConfig(LlamaConfig):
     num_experts_per_tok: int = 2
     router_aux_loss_coef: float = 0.02
     output_router_logits: bool = False
+    # the router's form (models/moe.py `MoELayer`): Mixtral's plain softmax top-k unless set
+    router_scoring: str = "softmax"
+    router_n_groups: int = 1
+    router_topk_groups: int = 1
+    routed_scaling_factor: float = 1.0
 
     @property
     def num_params(self) -> int:
@@ -74,7 +79,9 @@ class MixtralDecoderLayer(nn.Module):
         self.input_layernorm = RMSNorm(cfg.hidden_size, cfg.rms_norm_eps)
         self.self_attn = LlamaAttention(cfg)
         self.post_attention_layernorm = RMSNorm(cfg.hidden_size, cfg.rms_norm_eps)
-        self.block_sparse_moe = MoELayer(cfg.hidden_size, cfg.intermediate_size, cfg.num_local_experts, cfg.num_experts_per_tok)
+        self.block_sparse_moe = MoELayer(cfg.hidden_size, cfg.intermediate_size, cfg.num_local_experts, cfg.num_experts_per_tok,
+                                         scoring=cfg.router_scoring, n_groups=cfg.router_n_groups,
+                                         topk_groups=cfg.router_topk_groups, scale=cfg.routed_scaling_factor)
 
     def forward(self, hidden, residual, cos, sin, position_ids=None):
         x, residual = self.input_layernorm(hidden, residual)
@@ -139,7 +146,7 @@ class MixtralForCausalLM(nn.Module):
     def _rope(self, S, device):
         key = (S, str(device))
         if key not in self._rope_cache:
-            self._rope_cache[key] = rope_tables(S, self.config.head_dim, self.config.rope_theta, device, self.config.rope_scaling)
+            self._rope_cache[key] = rope_tables(S, self.config.rotary_dim, self.config.rope_theta, device, self.config.rope_scaling)
         return self._rope_cache[key]
 
     def forward(self, input_ids, labels=None, position_ids=None, attention_mask=None, return_logits: bool = True,

@@ -34,6 +34,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from ..ops._ext import ext, use_native
+from ..ops.routing import route_experts
 from ..parallel import comm
 
 
@@ -512,9 +513,14 @@ class MoEExperts(nn.Module):
 
 
 class MoELayer(nn.Module):
-    def __init__(self, hidden: int, intermediate: int, num_experts: int, top_k: int, norm_topk: bool = True):
+    """`scoring` ("softmax" or "sigmoid"), `n_groups` / `topk_groups` (experts chosen within the best groups only) and `scale` (on
+    the weights): the router's form, see `ops/routing.py` `route_experts`; the defaults are Mixtral's."""
+
+    def __init__(self, hidden: int, intermediate: int, num_experts: int, top_k: int, norm_topk: bool = True,
+                 scoring: str = "softmax", n_groups: int = 1, topk_groups: int = 1, scale: float = 1.0):
         super().__init__()
         self.num_experts, self.top_k, self.norm_topk = num_experts, top_k, norm_topk
+        self.scoring, self.n_groups, self.topk_groups, self.scale = scoring, n_groups, topk_groups, scale
         self.gate = nn.Linear(hidden, num_experts, bias=False)
         self.experts = MoEExperts(num_experts, hidden, intermediate)
         self.ep_group = None
@@ -555,14 +561,7 @@ class MoELayer(nn.Module):
         T = t.shape[0]
         logits = self.gate(t)
         self.last_router_logits = logits
-        probs = torch.softmax(logits.float(), dim=-1)
-        if self.router_bias is None:
-            w, idx = torch.topk(probs, self.top_k, dim=-1)
-        else:
-            idx = torch.topk(probs + self.router_bias.to(probs), self.top_k, dim=-1)[1]
-            w = probs.gather(-1, idx)
-        if self.norm_topk:
-            w = w / w.sum(-1, keepdim=True)
+        w, idx = self._route(logits)
         w = w.to(t.dtype)
         flat_e = idx.reshape(-1)
         if self.ep_group is None or comm.group_size(self.ep_group) == 1:
@@ -597,6 +596,21 @@ class MoELayer(nn.Module):
             y_sorted = self._ep_experts(t.index_select(0, src_tok), flat_e[order])
         out = torch.zeros_like(t).index_add_(0, src_tok, y_sorted * w_sorted.unsqueeze(-1))
         return out.view(shape)
+
+    def _route(self, logits):
+        """Weights (fp32) and experts [T, k] of the router's logits."""
+        if self.scoring != "softmax" or self.topk_groups != self.n_groups or self.scale != 1.0:
+            return route_experts(logits, self.top_k, self.scoring, self.router_bias, self.n_groups, self.topk_groups,
+                                 self.norm_topk, self.scale)
+        probs = torch.softmax(logits.float(), dim=-1)
+        if self.router_bias is None:
+            w, idx = torch.topk(probs, self.top_k, dim=-1)
+        else:
+            idx = torch.topk(probs + self.router_bias.to(probs), self.top_k, dim=-1)[1]
+            w = probs.gather(-1, idx)
+        if self.norm_topk:
+            w = w / w.sum(-1, keepdim=True)
+        return w, idx
 
     def _ep_experts(self, x_sorted, e_sorted):
         """Expert-parallel dispatch / combine. `x_sorted` rows are sorted by global expert id, so the rows bound for

@@ -1,4 +1,4 @@
-"""Autograd wrappers for the fused transformer-block kernels (RMSNorm, SwiGLU, RoPE, cross-entropy, flash
+"""Autograd wrappers for the fused transformer-block kernels (RMSNorm, layer norm, SwiGLU, RoPE, cross-entropy, flash
 attention). GPU tensors run the HIP kernels in `csrc/kernels/*.hip`; CPU tensors run a PyTorch fp32 reference of
 the same op (the reference is also the numerics oracle in tests/test_kernels_gpu.py).
 """
@@ -10,8 +10,12 @@ import os
 from typing import Optional
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from ._ext import ext, use_native
+
+# element types of the row operators (layer norm, RoPE in every layout, ops/logprobs.py, ops/routing.py)
+ROW_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 # dgrad through a transposed weight copy (ACCELERATE_DGRAD_WT=0 turns it off)
 _DGRAD_WT = os.environ.get("ACCELERATE_DGRAD_WT", "1") != "0"
@@ -182,6 +186,92 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual:
 
 
 # ----------------------------------------------------------------------------------------------------------
+# Layer norm (optionally fused with the residual add)
+# ----------------------------------------------------------------------------------------------------------
+# widest row of the HIP kernel, in bytes: 4096 chunks of 16
+_LAYER_NORM_MAX_BYTES = 65536
+
+
+def layer_norm_reference(x, weight=None, bias=None, eps=1e-5, residual=None):
+    acc = torch.float64 if x.dtype == torch.float64 else torch.float32
+    xf = x.to(acc)
+    if residual is not None:
+        total = xf + residual.to(acc)
+        x = total.to(x.dtype)
+        xf = total + (x.to(acc) - total).detach()  # the stored sum's value; its gradient is not rounded on the way back
+    d = xf - xf.mean(-1, keepdim=True)
+    y = d * torch.rsqrt(d.pow(2).mean(-1, keepdim=True) + eps)
+    if weight is not None:
+        y = y * weight.to(acc)
+    if bias is not None:
+        y = y + bias.to(acc)
+    return y.to(x.dtype), x
+
+
+def _rows(t: torch.Tensor, width: int) -> torch.Tensor:
+    """`t` as [rows, width] with contiguous rows at one stride: a view where its strides allow that, else a copy."""
+    t = t.reshape(math.prod(t.shape[:-1]), width)
+    return t if width == 1 or t.stride(1) == 1 else t.contiguous()
+
+
+class _LayerNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, eps):
+        H = x.shape[-1]
+        x2 = _rows(x, H)
+        y, s, mean, rstd = ext().layer_norm_fwd(x2, None if residual is None else _rows(residual, H), weight, bias, eps, True)
+        ctx.save_for_backward(x2 if s is None else s, weight, mean, rstd)
+        ctx.param_dtype = weight.dtype if weight is not None else bias.dtype if bias is not None else x.dtype
+        ctx.set_materialize_grads(False)
+        return y.view(x.shape), None if s is None else s.view(x.shape)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dres):
+        s, weight, mean, rstd = ctx.saved_tensors
+        need_x, need_w, need_b, need_res, _ = ctx.needs_input_grad
+        if dy is None:  # y unused: only the residual stream carries a gradient
+            return dres if need_x else None, None, None, dres if need_res else None, None
+        H = s.shape[1]
+        dx, dw, db = ext().layer_norm_bwd(_rows(dy, H), s, weight, mean, rstd, None if dres is None else _rows(dres, H),
+                                          need_w, need_b, ctx.param_dtype == torch.float32)
+        dx = dx.view(dy.shape)
+        # d(x + residual) flows to both summands
+        return dx if need_x else None, dw, db, dx if need_res else None, None
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, eps: float = 1e-5,
+               residual: Optional[torch.Tensor] = None):
+    """y = (s - mean(s)) / sqrt(var(s) + eps) * weight + bias over the last dimension, with s = x [+ residual].
+    Returns (y, residual_out) where residual_out = s in x's type, as `rms_norm` does (s is what is normalised), or x itself.
+
+    x and residual: one shape and one type (bf16, fp16 or fp32), any strides; weight / bias: [hidden], each optional, in x's
+    type or fp32. Statistics and the weight's gradient sums are fp32. On a GPU the row takes at most 64 KiB."""
+    H = x.shape[-1] if x.dim() else 0
+    if H < 1:
+        raise ValueError(f"layer_norm: x must have a last dimension to normalise, got shape {tuple(x.shape)}")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):
+        raise ValueError("layer_norm: residual must have x's shape, type and device")
+    for name, p in (("weight", weight), ("bias", bias)):
+        if p is not None and (p.shape != (H,) or p.device != x.device):
+            raise ValueError(f"layer_norm: {name} must be a [{H}] tensor on x's device")
+    if not (use_native(x) and x.dtype in ROW_DTYPES):
+        return layer_norm_reference(x, weight, bias, eps, residual)
+    if H * x.element_size() > _LAYER_NORM_MAX_BYTES:
+        raise ValueError(f"HIP layer norm needs rows of at most {_LAYER_NORM_MAX_BYTES} bytes (got {H} x {x.dtype})")
+    # the kernel takes both parameters in one type: x's, or fp32
+    wide = any(p is not None and p.dtype == torch.float32 for p in (weight, bias))
+    dtype = torch.float32 if wide else x.dtype
+    weight, bias = (None if p is None else p.to(dtype).contiguous() for p in (weight, bias))
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+        y, s = _LayerNormFn.apply(x, weight, bias, residual, eps)
+    else:
+        y, s, _, _ = ext().layer_norm_fwd(_rows(x, H), None if residual is None else _rows(residual, H), weight, bias, eps, False)
+        y, s = y.view(x.shape), None if s is None else s.view(x.shape)
+    return y, (x if residual is None else s)
+
+
+# ----------------------------------------------------------------------------------------------------------
 # SwiGLU on a fused [..., 2F] gate|up projection
 # ----------------------------------------------------------------------------------------------------------
 def swiglu_reference(gu):
@@ -231,12 +321,48 @@ def swiglu(gu: torch.Tensor, amax: bool = False, grad_amax: bool = False) -> tor
 
 
 # ----------------------------------------------------------------------------------------------------------
-# Rotary embeddings (rotate-half convention, as Llama) applied to the Q and K heads of a fused QKV tensor
+# Rotary embeddings applied to the Q and K heads of a fused QKV tensor: half layout (rotate-half, as Llama) or interleaved
+# pairs, over the whole head or its first values
 # ----------------------------------------------------------------------------------------------------------
+def _yarn_inv_freq(inv, head_dim, theta, scaling):
+    """YaRN (Peng et al., 2023): frequencies that turn fewer than `beta_slow` times over the original context are divided by
+    the factor, those that turn more than `beta_fast` times stay, a linear ramp over the dimensions joins them."""
+    factor = scaling["factor"]
+    old = scaling["original_max_position_embeddings"]
+
+    def dim_of(turns):
+        return head_dim * math.log(old / (turns * 2 * math.pi)) / (2 * math.log(theta))
+
+    low, high = dim_of(scaling.get("beta_fast") or 32), dim_of(scaling.get("beta_slow") or 1)
+    if scaling.get("truncate", True):
+        low, high = math.floor(low), math.ceil(high)
+    low, high = max(low, 0), min(high, head_dim - 1)
+    if low == high:
+        high += 0.001
+    ramp = ((torch.arange(head_dim // 2, dtype=torch.float64, device="cpu") - low) / (high - low)).clamp(0, 1)
+    return inv / factor * ramp + inv * (1 - ramp)
+
+
+def _yarn_attention_factor(scaling):
+    """The factor on cos and sin (so, squared, on the attention scores) that goes with YaRN's longer context."""
+    if scaling.get("attention_factor") is not None:
+        return scaling["attention_factor"]
+
+    def of(factor, m):
+        return 0.1 * m * math.log(factor) + 1.0 if factor > 1 else 1.0
+
+    m, m_all = scaling.get("mscale"), scaling.get("mscale_all_dim")
+    return of(scaling["factor"], m) / of(scaling["factor"], m_all) if m and m_all else of(scaling["factor"], 1.0)
+
+
 def rope_tables(seq_len: int, head_dim: int, theta: float = 500000.0, device=None, scaling: Optional[dict] = None):
-    """fp32 cos/sin tables [S, D/2]. `scaling` supports Llama-3.1 style frequency scaling."""
+    """fp32 cos/sin tables [S, D/2], the angles evaluated in 64 bits; D = `head_dim` is the rotated part of a head. `scaling`
+    is a transformers-style `rope_scaling` dict with `rope_type` "llama3", "linear" (positions divided by `factor`),
+    "dynamic" (theta grown for `seq_len` tokens past `original_max_position_embeddings`) or "yarn"."""
     inv = 1.0 / (theta ** (torch.arange(0, head_dim, 2, dtype=torch.float64, device="cpu") / head_dim))
-    if scaling is not None and scaling.get("rope_type", scaling.get("type")) == "llama3":
+    kind = None if scaling is None else scaling.get("rope_type", scaling.get("type"))
+    amplitude = 1.0
+    if kind == "llama3":
         factor = scaling["factor"]
         low, high = scaling["low_freq_factor"], scaling["high_freq_factor"]
         old = scaling["original_max_position_embeddings"]
@@ -247,28 +373,52 @@ def rope_tables(seq_len: int, head_dim: int, theta: float = 500000.0, device=Non
         mid = (1 - smooth) * scaled / factor + smooth * scaled
         is_mid = (wl <= low_wl) & (wl >= high_wl)
         inv = torch.where(is_mid, mid, scaled)
+    elif kind == "linear":
+        inv = inv / scaling["factor"]
+    elif kind == "dynamic":
+        old = scaling["original_max_position_embeddings"]
+        if seq_len > old and head_dim > 2:
+            factor = scaling["factor"]
+            theta = theta * (factor * seq_len / old - (factor - 1)) ** (head_dim / (head_dim - 2))
+            inv = 1.0 / (theta ** (torch.arange(0, head_dim, 2, dtype=torch.float64, device="cpu") / head_dim))
+    elif kind == "yarn":
+        inv = _yarn_inv_freq(inv, head_dim, theta, scaling)
+        amplitude = _yarn_attention_factor(scaling)
     t = torch.arange(seq_len, dtype=torch.float64)
     f = torch.outer(t, inv)
-    return f.cos().float().to(device), f.sin().float().to(device)
+    cos, sin = f.cos(), f.sin()
+    if amplitude != 1.0:
+        cos, sin = cos * amplitude, sin * amplitude
+    return cos.float().to(device), sin.float().to(device)
 
 
-def rope_reference(qkv, cos, sin, n_rot_heads, positions=None):
-    """qkv [..., T, Htot, D] (token-major). Rotates heads [0, n_rot_heads)."""
+def rope_reference(qkv, cos, sin, n_rot_heads, positions=None, interleaved=False, rotary_dim=None):
+    """qkv [..., T, Htot, D] (token-major). Rotates the first `rotary_dim` values (all of them: None) of heads
+    [0, n_rot_heads), in half pairs (i, i + R/2) or interleaved pairs (2i, 2i + 1)."""
     T = qkv.shape[-3]
-    D = qkv.shape[-1]
+    R = qkv.shape[-1] if rotary_dim is None else rotary_dim
     if positions is None:
         c, s = cos[:T], sin[:T]
     else:
         c, s = cos[positions.reshape(-1)], sin[positions.reshape(-1)]
-        c = c.view(*positions.shape, D // 2)
-        s = s.view(*positions.shape, D // 2)
-    c = torch.cat([c, c], dim=-1).unsqueeze(-2)
-    s = torch.cat([s, s], dim=-1).unsqueeze(-2)
-    x = qkv[..., :n_rot_heads, :].float()
-    x1, x2 = x[..., : D // 2], x[..., D // 2 :]
-    rot = torch.cat([-x2, x1], dim=-1)
-    out = x * c + rot * s
-    return torch.cat([out.to(qkv.dtype), qkv[..., n_rot_heads:, :]], dim=-2)
+        c = c.view(*positions.shape, R // 2)
+        s = s.view(*positions.shape, R // 2)
+    x = qkv[..., :n_rot_heads, :R]
+    x = x if x.dtype == torch.float64 else x.float()
+    if interleaved:
+        c, s = c.unsqueeze(-2), s.unsqueeze(-2)
+        x1, x2 = x[..., 0::2], x[..., 1::2]
+        out = torch.stack([x1 * c - x2 * s, x2 * c + x1 * s], dim=-1).flatten(-2)
+    else:
+        c = torch.cat([c, c], dim=-1).unsqueeze(-2)
+        s = torch.cat([s, s], dim=-1).unsqueeze(-2)
+        x1, x2 = x[..., : R // 2], x[..., R // 2 :]
+        rot = torch.cat([-x2, x1], dim=-1)
+        out = x * c + rot * s
+    out = out.to(qkv.dtype)
+    if R < qkv.shape[-1]:
+        out = torch.cat([out, qkv[..., :n_rot_heads, R:]], dim=-1)
+    return torch.cat([out, qkv[..., n_rot_heads:, :]], dim=-2)
 
 
 class _RopeFn(torch.autograd.Function):
@@ -289,11 +439,64 @@ class _RopeFn(torch.autograd.Function):
         return ext().rope_out(g, cos, sin, pos if has_pos else None, n_rot, Htot, D, -1.0), None, None, None, None
 
 
-def apply_rope(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, n_rot_heads: int, positions=None):
-    """qkv: [B, S, Htot, D]; rotates the first `n_rot_heads` heads (Q heads then K heads)."""
-    if use_native(qkv) and qkv.dtype == torch.bfloat16 and qkv.shape[-1] % 8 == 0:
+class _RopeAnyFn(torch.autograd.Function):
+    """Every layout, type and stride (csrc/kernels/rope.hip)."""
+
+    @staticmethod
+    def forward(ctx, qkv, cos, sin, n_rot_heads, positions, interleaved):
+        ctx.save_for_backward(cos, sin, positions)
+        ctx.meta = (n_rot_heads, interleaved)
+        return ext().rope_any(qkv, cos, sin, positions, n_rot_heads, interleaved, 1.0)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        cos, sin, positions = ctx.saved_tensors
+        n_rot_heads, interleaved = ctx.meta
+        g = g if g.stride(-1) == 1 else g.contiguous()
+        return ext().rope_any(g, cos, sin, positions, n_rot_heads, interleaved, -1.0), None, None, None, None, None
+
+
+def apply_rope(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, n_rot_heads: int, positions=None,
+               interleaved: bool = False, rotary_dim: Optional[int] = None):
+    """qkv: [B, S, Htot, D]; rotates the first `n_rot_heads` heads (Q heads then K heads) by the fp32 tables cos / sin
+    [positions, R/2] of `rope_tables`, in half pairs (i, i + R/2) or, `interleaved`, pairs (2i, 2i + 1).
+
+    `rotary_dim`: R, the rotated first values of each head, even; None rotates the whole head. `positions`: integers [B, S]
+    (or [1, S], [S] for every batch row), each token's row of the tables; None counts from 0. The result is a new contiguous
+    tensor. On a GPU any strides and even R are taken, in bf16, fp16 and fp32, with D up to 1000; a position outside the
+    tables gives NaN in its rotated values."""
+    S, Htot, D = qkv.shape[-3:]
+    R = D if rotary_dim is None else rotary_dim
+    if R < 2 or R % 2 or R > D:
+        raise ValueError(f"apply_rope: the rotated part must be even and within the head ({R} of {D})")
+    if cos.dim() != 2 or cos.shape != sin.shape or cos.shape[1] != R // 2:
+        raise ValueError(f"apply_rope: cos and sin must be [positions, {R // 2}] tables, got {tuple(cos.shape)}, {tuple(sin.shape)}")
+    if not 0 <= n_rot_heads <= Htot:
+        raise ValueError(f"apply_rope: {n_rot_heads} of {Htot} heads to rotate")
+    if positions is None and S > cos.shape[0]:
+        raise ValueError(f"apply_rope: {S} tokens, but tables for {cos.shape[0]} positions")
+    if not (use_native(qkv) and qkv.dtype in ROW_DTYPES):
+        return rope_reference(qkv, cos, sin, n_rot_heads, positions, interleaved, rotary_dim)
+    if qkv.dim() != 4:
+        raise ValueError(f"apply_rope: qkv must be [B, S, heads, D], got shape {tuple(qkv.shape)}")
+    B = qkv.shape[0]
+    if positions is None:
+        cos, sin = cos[:S], sin[:S]  # one row per token of the sequence
+    if (qkv.dtype == torch.bfloat16 and D % 8 == 0 and R == D and not interleaved
+            and (positions is None or (positions.dtype == torch.int64 and positions.numel() == B * S))):
         return _RopeFn.apply(qkv, cos, sin, n_rot_heads, positions)
-    return rope_reference(qkv, cos, sin, n_rot_heads, positions)
+    if D > 1000:
+        raise ValueError(f"HIP rope needs a head size of at most 1000 (got {D})")
+    if positions is not None:
+        positions = positions.view(B, S) if positions.numel() == B * S else positions.expand(B, S)
+        positions = positions.to(torch.int64)
+    if D > 1 and qkv.stride(-1) != 1:
+        qkv = qkv.contiguous()
+    cos, sin = cos.float().contiguous(), sin.float().contiguous()
+    if torch.is_grad_enabled() and qkv.requires_grad:
+        return _RopeAnyFn.apply(qkv, cos, sin, n_rot_heads, positions, interleaved)
+    return ext().rope_any(qkv, cos, sin, positions, n_rot_heads, interleaved, 1.0)
 
 
 # ----------------------------------------------------------------------------------------------------------

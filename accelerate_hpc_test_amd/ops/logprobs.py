@@ -1,0 +1,105 @@
+"""Log-probabilities of given tokens, the entropy of their distributions and the best alternatives, with gradients: what
+preference, policy and distillation losses read from a language model's logits. GPU tensors run
+`csrc/kernels/token_logprobs.hip` (the logits are read once forward, read once and their gradient written once backward; no
+[rows, vocabulary] tensor of probabilities exists); CPU tensors run the PyTorch reference below.
+"""
+
+from __future__ import annotations
+
+import math
+from typing import NamedTuple, Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from ._ext import ext, use_native
+from .fused import ROW_DTYPES, _rows
+
+MAX_TOP_K = 64  # alternatives per row on a GPU
+
+
+class TokenLogprobs(NamedTuple):
+    logprobs: torch.Tensor  # fp32 [...]
+    entropy: torch.Tensor  # fp32 [...]
+    top_logprobs: Optional[torch.Tensor]  # fp32 [..., top_k], falling; None without alternatives
+    top_tokens: Optional[torch.Tensor]  # int64 [..., top_k]; equal logits: the lower token first
+
+
+def token_logprobs_reference(logits, tokens, top_k=0, temperature=1.0, ignore_index=-100):
+    acc = logits if logits.dtype == torch.float64 else logits.float()
+    counts = tokens != ignore_index
+    named = (tokens >= 0) & (tokens < logits.shape[-1])
+    z = acc / temperature
+    logp = torch.log_softmax(z, dim=-1)
+    zero = torch.zeros((), dtype=logp.dtype, device=logp.device)
+    at = torch.where(named, tokens, torch.zeros_like(tokens)).unsqueeze(-1)
+    lp = logp.gather(-1, at).squeeze(-1)
+    lp = torch.where(named, lp, torch.full_like(lp, math.nan))
+    p = logp.exp()
+    gone = p == 0  # p log p is 0 there
+    entropy = -(p * logp.masked_fill(gone, 0.0)).masked_fill(gone, 0.0).sum(-1)
+    top_lp = top_id = None
+    if top_k:
+        sound = ~entropy.detach().isnan().unsqueeze(-1)
+        top_id = torch.sort(acc.detach(), dim=-1, descending=True, stable=True)[1][..., :top_k]
+        top_lp = torch.where(counts.unsqueeze(-1), logp.gather(-1, top_id), zero)
+        top_id = torch.where(counts.unsqueeze(-1) & sound, top_id, torch.full_like(top_id, -1))
+    return TokenLogprobs(torch.where(counts, lp, zero), torch.where(counts, entropy, zero), top_lp, top_id)
+
+
+class _TokenLogprobsFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, top_k, inv_t, ignore_index):
+        lp, ent, top_lp, top_id, stats = ext().token_logprobs_fwd(logits, tokens, top_k, inv_t, ignore_index, True)
+        ctx.save_for_backward(logits, tokens, stats, top_id)
+        ctx.meta = (inv_t, ignore_index)
+        ctx.set_materialize_grads(False)
+        if top_id is not None:
+            ctx.mark_non_differentiable(top_id)
+        return lp, ent, top_lp, top_id
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_lp, g_ent, g_top, _):
+        if g_lp is None and g_ent is None and g_top is None:
+            return None, None, None, None, None
+        logits, tokens, stats, top_id = ctx.saved_tensors
+        g_top = None if g_top is None else g_top.contiguous()
+        return (ext().token_logprobs_bwd(logits, tokens, stats, top_id, g_lp, g_ent, g_top, *ctx.meta), None, None, None, None)
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0, temperature: float = 1.0,
+                   ignore_index: int = -100) -> TokenLogprobs:
+    """log softmax(logits / temperature) at `tokens`, the entropy of that distribution, and its `top_k` best alternatives.
+
+    logits [..., V] in bf16, fp16 or fp32; tokens: integers [...]. All outputs are fp32 and differentiable with respect to the
+    logits (the alternatives at their chosen tokens). Rows whose token is `ignore_index` give 0, 0, 0 and -1 and no gradient;
+    a token outside [0, V) gives NaN. Logits of -inf are impossible tokens: probability 0, nothing added to the entropy. A row
+    with NaN or +inf, or of -inf alone, has no distribution: NaN, and -1 for the alternatives."""
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError(f"token_logprobs: logits must be [..., vocabulary], got shape {tuple(logits.shape)}")
+    V = logits.shape[-1]
+    if tokens.shape != logits.shape[:-1] or tokens.device != logits.device:
+        raise ValueError(f"token_logprobs: tokens must be {tuple(logits.shape[:-1])} on the logits' device, got {tuple(tokens.shape)}")
+    if tokens.is_floating_point() or tokens.is_complex() or tokens.dtype == torch.bool:
+        raise TypeError(f"token_logprobs: tokens must be integers, got {tokens.dtype}")
+    if not 0 <= top_k <= V:
+        raise ValueError(f"token_logprobs: top_k must be within the vocabulary ({top_k} of {V})")
+    if not (temperature > 0 and math.isfinite(temperature)):
+        raise ValueError(f"token_logprobs: temperature must be positive and finite, got {temperature}")
+    tokens = tokens.to(torch.int64)
+    if not (use_native(logits) and logits.dtype in ROW_DTYPES):
+        return token_logprobs_reference(logits, tokens, top_k, temperature, ignore_index)
+    if top_k > MAX_TOP_K:
+        raise ValueError(f"HIP token_logprobs gives at most {MAX_TOP_K} alternatives (got top_k={top_k})")
+    l2, t2 = _rows(logits, V), tokens.reshape(-1).contiguous()
+    if torch.is_grad_enabled() and logits.requires_grad:
+        lp, ent, top_lp, top_id = _TokenLogprobsFn.apply(l2, t2, top_k, 1.0 / temperature, ignore_index)
+    else:
+        lp, ent, top_lp, top_id, _ = ext().token_logprobs_fwd(l2, t2, top_k, 1.0 / temperature, ignore_index, False)
+    if logits.dim() != 2:
+        shape = logits.shape[:-1]
+        lp, ent = lp.view(shape), ent.view(shape)
+        if top_k:
+            top_lp, top_id = top_lp.view(*shape, top_k), top_id.view(*shape, top_k)
+    return TokenLogprobs(lp, ent, top_lp, top_id)

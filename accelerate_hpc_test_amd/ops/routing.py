@@ -1,0 +1,102 @@
+"""Routing to experts: which experts a token goes to and with what weights, from the router's logits, with the logits'
+gradient (`models/moe.py` calls it for every form beyond the plain softmax top-k). GPU tensors run
+`csrc/kernels/route_experts.hip`, one launch forward and one backward; CPU tensors run the PyTorch reference below.
+"""
+
+from __future__ import annotations
+
+import math
+from typing import Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from ._ext import ext, use_native
+from .fused import ROW_DTYPES, _rows
+
+MAX_EXPERTS, MAX_TOP_K, MAX_GROUPS = 1024, 64, 64  # of the HIP kernel
+_TINY = torch.finfo(torch.float32).tiny
+
+
+def route_experts_reference(logits, top_k, scoring="softmax", bias=None, n_groups=1, topk_groups=1, renormalize=True, scale=1.0):
+    x = logits if logits.dtype == torch.float64 else logits.float()
+    T, E = x.shape
+    score = torch.softmax(x, -1) if scoring == "softmax" else torch.sigmoid(x)
+    with torch.no_grad():
+        if bias is None and topk_groups == n_groups:
+            key = x.double()  # the scores' own order
+        else:  # sums of scores and a bias, in 64 bits: the order must not hang on a rounding
+            key = torch.softmax(x.double(), -1) if scoring == "softmax" else torch.sigmoid(x.double())
+            if bias is not None:
+                key = key + bias.double()
+        key = torch.where(key.isnan(), torch.full_like(key, -math.inf), key)
+        if topk_groups < n_groups:
+            size = E // n_groups
+            rating = torch.topk(key.view(T, n_groups, size), min(2, size), dim=-1)[0].sum(-1)
+            best = torch.sort(rating, dim=-1, descending=True, stable=True)[1][:, :topk_groups]
+            closed = torch.ones_like(rating, dtype=torch.bool).scatter_(1, best, False)
+            # closed experts sort behind every open one, -inf among them
+            order = torch.sort(key, dim=-1, descending=True, stable=True)[1]
+            shut = closed.repeat_interleave(size, 1).gather(1, order)
+            ids = order.gather(1, torch.sort(shut.to(torch.int8), dim=-1, stable=True)[1])[:, :top_k]
+        else:
+            ids = torch.sort(key, dim=-1, descending=True, stable=True)[1][:, :top_k]
+    w = score.gather(1, ids)
+    if renormalize:
+        w = w / w.sum(-1, keepdim=True).clamp_min(_TINY)
+    return w * scale, ids
+
+
+class _RouteExpertsFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, top_k, softmax, bias, n_groups, topk_groups, renormalize, scale):
+        w, ids = ext().route_experts_fwd(logits, top_k, softmax, bias, n_groups, topk_groups, renormalize, scale)
+        ctx.save_for_backward(logits, w, ids)
+        ctx.meta = (softmax, renormalize, scale)
+        ctx.mark_non_differentiable(ids)
+        return w, ids
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dw, _):
+        logits, w, ids = ctx.saved_tensors
+        return ext().route_experts_bwd(logits, w, ids, dw.contiguous(), *ctx.meta), None, None, None, None, None, None, None
+
+
+def route_experts(logits: torch.Tensor, top_k: int, scoring: str = "softmax", bias: Optional[torch.Tensor] = None,
+                  n_groups: int = 1, topk_groups: int = 1, renormalize: bool = True, scale: float = 1.0):
+    """The `top_k` experts of each token and their weights from router logits [T, E] (bf16, fp16 or fp32).
+
+    Scores are softmax(logits) or sigmoid(logits) (`scoring`). Experts are chosen by score + `bias` ([E], optional: it steers the
+    choice alone, balances the load, and gets no gradient), within the `topk_groups` of `n_groups` equal groups whose two best
+    keys have the largest sum; equal keys go to the lower index, keys are compared in 64 bits. Weights are the chosen scores,
+    divided by their sum (`renormalize`), times `scale`. Returns (weights fp32 [T, k], experts int64 [T, k]) in falling order of
+    the keys; the weights are differentiable with respect to the logits."""
+    if logits.dim() != 2 or logits.shape[1] < 1:
+        raise ValueError(f"route_experts: logits must be [tokens, experts], got shape {tuple(logits.shape)}")
+    E = logits.shape[1]
+    if scoring not in ("softmax", "sigmoid"):
+        raise ValueError(f"route_experts: scoring must be 'softmax' or 'sigmoid', got {scoring!r}")
+    if n_groups < 1 or E % n_groups or not 1 <= topk_groups <= n_groups:
+        raise ValueError(f"route_experts: {topk_groups} of {n_groups} groups over {E} experts")
+    if not 1 <= top_k <= E // n_groups * topk_groups:
+        raise ValueError(f"route_experts: top_k={top_k} of {E // n_groups * topk_groups} experts within reach")
+    if not (math.isfinite(scale) and scale != 0):
+        raise ValueError(f"route_experts: scale must be finite and not zero, got {scale}")
+    if bias is not None:
+        if bias.shape != (E,) or bias.device != logits.device:
+            raise ValueError(f"route_experts: bias must be a [{E}] tensor on the logits' device")
+        bias = bias.detach()
+    if not (use_native(logits) and logits.dtype in ROW_DTYPES):
+        return route_experts_reference(logits, top_k, scoring, bias, n_groups, topk_groups, renormalize, scale)
+    if E > MAX_EXPERTS or top_k > MAX_TOP_K or n_groups > MAX_GROUPS:
+        raise ValueError(f"HIP route_experts takes at most {MAX_EXPERTS} experts, {MAX_TOP_K} choices and {MAX_GROUPS} groups "
+                         f"(got {E}, {top_k}, {n_groups})")
+    if bias is not None:
+        bias = bias.float().contiguous()
+    l2 = _rows(logits, E)
+    args = (l2, top_k, scoring == "softmax", bias, n_groups, topk_groups, renormalize, scale)
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return _RouteExpertsFn.apply(*args)
+    w, ids = ext().route_experts_fwd(*args)
+    return w, ids
