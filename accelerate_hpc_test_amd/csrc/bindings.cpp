@@ -45,27 +45,6 @@ void rope_inplace(torch::Tensor qkv, torch::Tensor cos, torch::Tensor sin, c10::
                   int64_t n_rot_heads, int64_t n_heads_total, int64_t head_dim, double sign);
 torch::Tensor rope_out(torch::Tensor src, torch::Tensor cos, torch::Tensor sin, c10::optional<torch::Tensor> pos,
                        int64_t n_rot_heads, int64_t n_heads_total, int64_t head_dim, double sign);
-// layer_norm.hip
-std::vector<torch::Tensor> layer_norm_fwd(torch::Tensor x, c10::optional<torch::Tensor> residual, c10::optional<torch::Tensor> w,
-                                          c10::optional<torch::Tensor> b, double eps, bool stats);
-std::vector<torch::Tensor> layer_norm_bwd(torch::Tensor dy, torch::Tensor s, c10::optional<torch::Tensor> w, torch::Tensor mean,
-                                          torch::Tensor rstd, c10::optional<torch::Tensor> dres, bool want_dw, bool want_db,
-                                          bool wide_params);
-// rope.hip
-torch::Tensor rope_any(torch::Tensor src, torch::Tensor cos, torch::Tensor sin, c10::optional<torch::Tensor> pos, int64_t n_rot,
-                       bool interleaved, double sign);
-// token_logprobs.hip
-std::vector<torch::Tensor> token_logprobs_fwd(torch::Tensor logits, torch::Tensor tokens, int64_t K, double inv_t, int64_t ignore,
-                                              bool want_stats);
-torch::Tensor token_logprobs_bwd(torch::Tensor logits, torch::Tensor tokens, torch::Tensor stats,
-                                 c10::optional<torch::Tensor> top_id, c10::optional<torch::Tensor> g_lp,
-                                 c10::optional<torch::Tensor> g_ent, c10::optional<torch::Tensor> g_top, double inv_t,
-                                 int64_t ignore);
-// route_experts.hip
-std::vector<torch::Tensor> route_experts_fwd(torch::Tensor logits, int64_t k, bool softmax, c10::optional<torch::Tensor> bias,
-                                             int64_t groups, int64_t top_groups, bool renorm, double scale);
-torch::Tensor route_experts_bwd(torch::Tensor logits, torch::Tensor weights, torch::Tensor experts, torch::Tensor dw, bool softmax,
-                                bool renorm, double scale);
 // xent_optim.hip
 std::vector<torch::Tensor> xent_fwd(torch::Tensor logits, torch::Tensor labels, int64_t ignore_index);
 void xent_bwd(torch::Tensor logits, torch::Tensor labels, torch::Tensor lse, torch::Tensor scale, torch::Tensor out,
@@ -137,6 +116,7 @@ void grad_shard_update(torch::Tensor dst, torch::Tensor src, double scale, bool 
 // runtime/*.cpp
 void register_runtime(pybind11::module& m);
 void register_d2h_writer(pybind11::module& m);
+void register_row_autograd(pybind11::module& m);
 void cpu_adam_step(torch::Tensor p, torch::Tensor g, torch::Tensor m, torch::Tensor v, c10::optional<torch::Tensor> shadow,
                    double lr, double beta1, double beta2, double eps, double wd, double bc1, double bc2_sqrt, bool adamw);
 bool blaslt_wgrad_f32(torch::Tensor dy, torch::Tensor x, torch::Tensor out, bool accumulate, bool x_t, bool dy_t);
@@ -160,13 +140,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("swiglu_bwd", &swiglu_bwd, pybind11::arg("gu"), pybind11::arg("dh"), pybind11::arg("amax") = pybind11::none());
   m.def("rope_inplace", &rope_inplace);
   m.def("rope_out", &rope_out);
-  m.def("layer_norm_fwd", &layer_norm_fwd);
-  m.def("layer_norm_bwd", &layer_norm_bwd);
-  m.def("rope_any", &rope_any);
-  m.def("token_logprobs_fwd", &token_logprobs_fwd);
-  m.def("token_logprobs_bwd", &token_logprobs_bwd);
-  m.def("route_experts_fwd", &route_experts_fwd);
-  m.def("route_experts_bwd", &route_experts_bwd);
   m.def("xent_fwd", &xent_fwd);
   m.def("xent_bwd", &xent_bwd);
   m.def("adam_multi_tensor", &adam_multi_tensor);
@@ -227,6 +200,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("fp8_gemm_select", &fp8_gemm_select, pybind11::arg("variant"), pybind11::arg("group_m") = 0);
   register_runtime(m);
   register_d2h_writer(m);
+  register_row_autograd(m);
   m.def("blaslt_dgrad_bf16", &blaslt_dgrad_bf16, pybind11::arg("dy"), pybind11::arg("w"), pybind11::arg("out"),
         "dx = dy . W (bf16, both row-major: the NN layout) on a searched hipBLASLt algorithm; False if none");
   m.def("blaslt_wgrad_f32", &blaslt_wgrad_f32, pybind11::arg("dy"), pybind11::arg("x"), pybind11::arg("out"), pybind11::arg("accumulate"),

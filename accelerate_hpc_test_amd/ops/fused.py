@@ -10,7 +10,6 @@ import os
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from ._ext import ext, use_native
 
@@ -208,38 +207,6 @@ def layer_norm_reference(x, weight=None, bias=None, eps=1e-5, residual=None):
     return y.to(x.dtype), x
 
 
-def _rows(t: torch.Tensor, width: int) -> torch.Tensor:
-    """`t` as [rows, width] with contiguous rows at one stride: a view where its strides allow that, else a copy."""
-    t = t.reshape(math.prod(t.shape[:-1]), width)
-    return t if width == 1 or t.stride(1) == 1 else t.contiguous()
-
-
-class _LayerNormFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, residual, eps):
-        H = x.shape[-1]
-        x2 = _rows(x, H)
-        y, s, mean, rstd = ext().layer_norm_fwd(x2, None if residual is None else _rows(residual, H), weight, bias, eps, True)
-        ctx.save_for_backward(x2 if s is None else s, weight, mean, rstd)
-        ctx.param_dtype = weight.dtype if weight is not None else bias.dtype if bias is not None else x.dtype
-        ctx.set_materialize_grads(False)
-        return y.view(x.shape), None if s is None else s.view(x.shape)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy, dres):
-        s, weight, mean, rstd = ctx.saved_tensors
-        need_x, need_w, need_b, need_res, _ = ctx.needs_input_grad
-        if dy is None:  # y unused: only the residual stream carries a gradient
-            return dres if need_x else None, None, None, dres if need_res else None, None
-        H = s.shape[1]
-        dx, dw, db = ext().layer_norm_bwd(_rows(dy, H), s, weight, mean, rstd, None if dres is None else _rows(dres, H),
-                                          need_w, need_b, ctx.param_dtype == torch.float32)
-        dx = dx.view(dy.shape)
-        # d(x + residual) flows to both summands
-        return dx if need_x else None, dw, db, dx if need_res else None, None
-
-
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, eps: float = 1e-5,
                residual: Optional[torch.Tensor] = None):
     """y = (s - mean(s)) / sqrt(var(s) + eps) * weight + bias over the last dimension, with s = x [+ residual].
@@ -260,15 +227,15 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     if H * x.element_size() > _LAYER_NORM_MAX_BYTES:
         raise ValueError(f"HIP layer norm needs rows of at most {_LAYER_NORM_MAX_BYTES} bytes (got {H} x {x.dtype})")
     # the kernel takes both parameters in one type: x's, or fp32
-    wide = any(p is not None and p.dtype == torch.float32 for p in (weight, bias))
-    dtype = torch.float32 if wide else x.dtype
-    weight, bias = (None if p is None else p.to(dtype).contiguous() for p in (weight, bias))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
-        y, s = _LayerNormFn.apply(x, weight, bias, residual, eps)
-    else:
-        y, s, _, _ = ext().layer_norm_fwd(_rows(x, H), None if residual is None else _rows(residual, H), weight, bias, eps, False)
-        y, s = y.view(x.shape), None if s is None else s.view(x.shape)
-    return y, (x if residual is None else s)
+    dtype = x.dtype
+    if any(p is not None and p.dtype == torch.float32 for p in (weight, bias)):
+        dtype = torch.float32
+    if weight is not None and not (weight.dtype == dtype and weight.is_contiguous()):
+        weight = weight.to(dtype).contiguous()
+    if bias is not None and not (bias.dtype == dtype and bias.is_contiguous()):
+        bias = bias.to(dtype).contiguous()
+    out = ext().layer_norm(x, weight, bias, residual, eps)
+    return out[0], (x if residual is None else out[1])
 
 
 # ----------------------------------------------------------------------------------------------------------
@@ -439,24 +406,6 @@ class _RopeFn(torch.autograd.Function):
         return ext().rope_out(g, cos, sin, pos if has_pos else None, n_rot, Htot, D, -1.0), None, None, None, None
 
 
-class _RopeAnyFn(torch.autograd.Function):
-    """Every layout, type and stride (csrc/kernels/rope.hip)."""
-
-    @staticmethod
-    def forward(ctx, qkv, cos, sin, n_rot_heads, positions, interleaved):
-        ctx.save_for_backward(cos, sin, positions)
-        ctx.meta = (n_rot_heads, interleaved)
-        return ext().rope_any(qkv, cos, sin, positions, n_rot_heads, interleaved, 1.0)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
-        cos, sin, positions = ctx.saved_tensors
-        n_rot_heads, interleaved = ctx.meta
-        g = g if g.stride(-1) == 1 else g.contiguous()
-        return ext().rope_any(g, cos, sin, positions, n_rot_heads, interleaved, -1.0), None, None, None, None, None
-
-
 def apply_rope(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, n_rot_heads: int, positions=None,
                interleaved: bool = False, rotary_dim: Optional[int] = None):
     """qkv: [B, S, Htot, D]; rotates the first `n_rot_heads` heads (Q heads then K heads) by the fp32 tables cos / sin
@@ -491,12 +440,7 @@ def apply_rope(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, n_rot_he
     if positions is not None:
         positions = positions.view(B, S) if positions.numel() == B * S else positions.expand(B, S)
         positions = positions.to(torch.int64)
-    if D > 1 and qkv.stride(-1) != 1:
-        qkv = qkv.contiguous()
-    cos, sin = cos.float().contiguous(), sin.float().contiguous()
-    if torch.is_grad_enabled() and qkv.requires_grad:
-        return _RopeAnyFn.apply(qkv, cos, sin, n_rot_heads, positions, interleaved)
-    return ext().rope_any(qkv, cos, sin, positions, n_rot_heads, interleaved, 1.0)
+    return ext().rope(qkv, cos.float().contiguous(), sin.float().contiguous(), positions, n_rot_heads, interleaved)
 
 
 # ----------------------------------------------------------------------------------------------------------

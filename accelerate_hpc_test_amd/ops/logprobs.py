@@ -10,10 +10,9 @@ import math
 from typing import NamedTuple, Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from ._ext import ext, use_native
-from .fused import ROW_DTYPES, _rows
+from .fused import ROW_DTYPES
 
 MAX_TOP_K = 64  # alternatives per row on a GPU
 
@@ -47,27 +46,6 @@ def token_logprobs_reference(logits, tokens, top_k=0, temperature=1.0, ignore_in
     return TokenLogprobs(torch.where(counts, lp, zero), torch.where(counts, entropy, zero), top_lp, top_id)
 
 
-class _TokenLogprobsFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, tokens, top_k, inv_t, ignore_index):
-        lp, ent, top_lp, top_id, stats = ext().token_logprobs_fwd(logits, tokens, top_k, inv_t, ignore_index, True)
-        ctx.save_for_backward(logits, tokens, stats, top_id)
-        ctx.meta = (inv_t, ignore_index)
-        ctx.set_materialize_grads(False)
-        if top_id is not None:
-            ctx.mark_non_differentiable(top_id)
-        return lp, ent, top_lp, top_id
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g_lp, g_ent, g_top, _):
-        if g_lp is None and g_ent is None and g_top is None:
-            return None, None, None, None, None
-        logits, tokens, stats, top_id = ctx.saved_tensors
-        g_top = None if g_top is None else g_top.contiguous()
-        return (ext().token_logprobs_bwd(logits, tokens, stats, top_id, g_lp, g_ent, g_top, *ctx.meta), None, None, None, None)
-
-
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0, temperature: float = 1.0,
                    ignore_index: int = -100) -> TokenLogprobs:
     """log softmax(logits / temperature) at `tokens`, the entropy of that distribution, and its `top_k` best alternatives.
@@ -92,14 +70,5 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0, t
         return token_logprobs_reference(logits, tokens, top_k, temperature, ignore_index)
     if top_k > MAX_TOP_K:
         raise ValueError(f"HIP token_logprobs gives at most {MAX_TOP_K} alternatives (got top_k={top_k})")
-    l2, t2 = _rows(logits, V), tokens.reshape(-1).contiguous()
-    if torch.is_grad_enabled() and logits.requires_grad:
-        lp, ent, top_lp, top_id = _TokenLogprobsFn.apply(l2, t2, top_k, 1.0 / temperature, ignore_index)
-    else:
-        lp, ent, top_lp, top_id, _ = ext().token_logprobs_fwd(l2, t2, top_k, 1.0 / temperature, ignore_index, False)
-    if logits.dim() != 2:
-        shape = logits.shape[:-1]
-        lp, ent = lp.view(shape), ent.view(shape)
-        if top_k:
-            top_lp, top_id = top_lp.view(*shape, top_k), top_id.view(*shape, top_k)
-    return TokenLogprobs(lp, ent, top_lp, top_id)
+    out = ext().token_logprobs(logits, tokens, top_k, 1.0 / temperature, ignore_index)
+    return TokenLogprobs(*out) if top_k else TokenLogprobs(*out, None, None)

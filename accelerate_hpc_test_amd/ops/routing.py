@@ -9,10 +9,9 @@ import math
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from ._ext import ext, use_native
-from .fused import ROW_DTYPES, _rows
+from .fused import ROW_DTYPES
 
 MAX_EXPERTS, MAX_TOP_K, MAX_GROUPS = 1024, 64, 64  # of the HIP kernel
 _TINY = torch.finfo(torch.float32).tiny
@@ -47,22 +46,6 @@ def route_experts_reference(logits, top_k, scoring="softmax", bias=None, n_group
     return w * scale, ids
 
 
-class _RouteExpertsFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, top_k, softmax, bias, n_groups, topk_groups, renormalize, scale):
-        w, ids = ext().route_experts_fwd(logits, top_k, softmax, bias, n_groups, topk_groups, renormalize, scale)
-        ctx.save_for_backward(logits, w, ids)
-        ctx.meta = (softmax, renormalize, scale)
-        ctx.mark_non_differentiable(ids)
-        return w, ids
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dw, _):
-        logits, w, ids = ctx.saved_tensors
-        return ext().route_experts_bwd(logits, w, ids, dw.contiguous(), *ctx.meta), None, None, None, None, None, None, None
-
-
 def route_experts(logits: torch.Tensor, top_k: int, scoring: str = "softmax", bias: Optional[torch.Tensor] = None,
                   n_groups: int = 1, topk_groups: int = 1, renormalize: bool = True, scale: float = 1.0):
     """The `top_k` experts of each token and their weights from router logits [T, E] (bf16, fp16 or fp32).
@@ -94,9 +77,5 @@ def route_experts(logits: torch.Tensor, top_k: int, scoring: str = "softmax", bi
                          f"(got {E}, {top_k}, {n_groups})")
     if bias is not None:
         bias = bias.float().contiguous()
-    l2 = _rows(logits, E)
-    args = (l2, top_k, scoring == "softmax", bias, n_groups, topk_groups, renormalize, scale)
-    if torch.is_grad_enabled() and logits.requires_grad:
-        return _RouteExpertsFn.apply(*args)
-    w, ids = ext().route_experts_fwd(*args)
+    w, ids = ext().route_experts(logits, top_k, scoring == "softmax", bias, n_groups, topk_groups, renormalize, scale)
     return w, ids
