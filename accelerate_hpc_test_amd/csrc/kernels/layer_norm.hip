@@ -19,6 +19,25 @@ namespace {
 
 constexpr int kMaxChunks = 4096;  // 16-byte chunks in a row: 32768 elements of 16 bits, 16384 of 32
 
+// A chunk of n elements: VEC, the few at the end of a row whose width is no multiple of VEC, or 0 past it.
+template <typename T, int VEC>
+__device__ __forceinline__ Pack<T, VEC> get_chunk(const T* p, int n) {
+  return n == VEC ? load_any<T, VEC>(p) : load_part<T, VEC>(p, n);
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void put_chunk(T* p, const Pack<T, VEC>& x, int n) {
+  if (n == VEC) store_any<T, VEC>(p, x);
+  else store_part<T, VEC>(p, x, n);
+}
+template <int VEC>
+__device__ __forceinline__ int chunk_size(int c, int nfull, int tail) { return c < nfull ? VEC : c == nfull ? tail : 0; }
+
+// The row that this thread works on is the same for its whole wave: kept in scalar registers, as are the row's addresses.
+template <int TPR, int ROWS>
+__device__ __forceinline__ long first_row() {
+  return (long)blockIdx.x * ROWS + (ROWS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / TPR));
+}
+
 template <typename T, typename W, int TPR, int VPT>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_fwd_kernel(
     const T* __restrict__ x, long x_stride, const T* __restrict__ res, long res_stride, const W* __restrict__ w,
@@ -26,10 +45,23 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_fwd_kernel(
     float* __restrict__ rstd_out, long rows, int H, float eps) {
   constexpr int VEC = 16 / sizeof(T), NT = TPR < 256 ? 256 : TPR, ROWS = NT / TPR;
   __shared__ float slots[2][16];
-  const int li = threadIdx.x % TPR, nfull = H / VEC, tail = H % VEC;
+  const int li = ROWS == 1 ? threadIdx.x : threadIdx.x % TPR, nfull = H / VEC, tail = H % VEC;
   const float width = (float)H;
+  // Up to two chunks per thread the parameters are loaded once, ahead of the first row's sums; wider rows load them again
+  // for each row, from the cache.
+  constexpr bool kHold = VPT <= 2;
+  Pack<W, VEC> wv[VPT], bv[VPT];
+  auto load_params = [&](int i) {
+    const int c = li + i * TPR, n = chunk_size<VEC>(c, nfull, tail);
+    if (w != nullptr) wv[i] = get_chunk<W, VEC>(w + c * VEC, n);
+    if (b != nullptr) bv[i] = get_chunk<W, VEC>(b + c * VEC, n);
+  };
+  if constexpr (kHold) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) load_params(i);
+  }
   // the trip count is uniform over each row's threads: one wave, or the whole block where barriers are used
-  for (long row = (long)blockIdx.x * ROWS + threadIdx.x / TPR; row < rows; row += (long)gridDim.x * ROWS) {
+  for (long row = first_row<TPR, ROWS>(); row < rows; row += (long)gridDim.x * ROWS) {
     const T* xr = x + row * x_stride;
     const T* rr = res == nullptr ? nullptr : res + row * res_stride;
     float v[VPT][VEC];
@@ -37,19 +69,20 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_fwd_kernel(
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int c = li + i * TPR;
-      const int n = c < nfull ? VEC : (c == nfull ? tail : 0);
-      Pack<T, VEC> a = n == VEC ? load_any<T, VEC>(xr + c * VEC) : load_part<T, VEC>(xr + c * VEC, n);
+      const int n = chunk_size<VEC>(c, nfull, tail);
+      Pack<T, VEC> a = get_chunk<T, VEC>(xr + c * VEC, n);
       if (rr != nullptr) {
-        const Pack<T, VEC> r = n == VEC ? load_any<T, VEC>(rr + c * VEC) : load_part<T, VEC>(rr + c * VEC, n);
+        const Pack<T, VEC> r = get_chunk<T, VEC>(rr + c * VEC, n);
+        float f[VEC];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) a.v[j] = from_f<T>(to_f<T>(a.v[j]) + to_f<T>(r.v[j]));
+        for (int j = 0; j < VEC; ++j) f[j] = a.get(j) + r.get(j);
+        a = Pack<T, VEC>::of(f);
         // what is normalised is what the residual stream stores
-        if (n == VEC) store_any<T, VEC>(sum_out + row * H + c * VEC, a);
-        else store_part<T, VEC>(sum_out + row * H + c * VEC, a, n);
+        put_chunk<T, VEC>(sum_out + row * H + c * VEC, a, n);
       }
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        v[i][j] = to_f<T>(a.v[j]);
+        v[i][j] = a.get(j);
         sum += v[i][j];
       }
     }
@@ -58,19 +91,11 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_fwd_kernel(
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int c = li + i * TPR;
-      const int n = c < nfull ? VEC : (c == nfull ? tail : 0);
-      if (n == VEC) {
+      const int n = chunk_size<VEC>(c, nfull, tail);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          v[i][j] -= mean;
-          sq = fmaf(v[i][j], v[i][j], sq);
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          v[i][j] = j < n ? v[i][j] - mean : 0.f;
-          sq = fmaf(v[i][j], v[i][j], sq);
-        }
+      for (int j = 0; j < VEC; ++j) {
+        v[i][j] = j < n ? v[i][j] - mean : 0.f;
+        sq = fmaf(v[i][j], v[i][j], sq);
       }
     }
     const float rstd = 1.f / sqrtf(row_reduce<OpSum, TPR>(sq, slots[1]) / width + eps);
@@ -82,26 +107,18 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_fwd_kernel(
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int c = li + i * TPR;
-      const int n = c < nfull ? VEC : (c == nfull ? tail : 0);
+      const int n = chunk_size<VEC>(c, nfull, tail);
       if (n == 0) continue;
-      Pack<T, VEC> o;
-      Pack<W, VEC> ww, bb;
-      if (n == VEC) {
-        if (w != nullptr) ww = load_wide<W, VEC>(w + c * VEC);
-        if (b != nullptr) bb = load_wide<W, VEC>(b + c * VEC);
-      } else {
-        if (w != nullptr) ww = load_part<W, VEC>(w + c * VEC, n);
-        if (b != nullptr) bb = load_part<W, VEC>(b + c * VEC, n);
-      }
+      float o[VEC];
+      if constexpr (!kHold) load_params(i);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
         float f = v[i][j] * rstd;
-        if (w != nullptr) f *= to_f<W>(ww.v[j]);
-        if (b != nullptr) f += to_f<W>(bb.v[j]);
-        o.v[j] = from_f<T>(f);
+        if (w != nullptr) f *= wv[i].get(j);
+        if (b != nullptr) f += bv[i].get(j);
+        o[j] = f;
       }
-      if (n == VEC) store_any<T, VEC>(yr + c * VEC, o);
-      else store_part<T, VEC>(yr + c * VEC, o, n);
+      put_chunk<T, VEC>(yr + c * VEC, Pack<T, VEC>::of(o), n);
     }
   }
 }
@@ -116,42 +133,69 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_bwd_kernel(
   constexpr int VEC = 16 / sizeof(T), NT = TPR < 256 ? 256 : TPR, ROWS = NT / TPR;
   __shared__ float slots[2][2][16];
   extern __shared__ float combine[];  // ROWS > 1: [2, chunks * VEC]
-  const int li = threadIdx.x % TPR, nfull = H / VEC, tail = H % VEC, chunks = (H + VEC - 1) / VEC;
+  const int li = ROWS == 1 ? threadIdx.x : threadIdx.x % TPR, nfull = H / VEC, tail = H % VEC, chunks = (H + VEC - 1) / VEC;
   const float width = (float)H;
   float dw[VPT][VEC], db[VPT][VEC];
 #pragma unroll
   for (int i = 0; i < VPT; ++i)
 #pragma unroll
     for (int j = 0; j < VEC; ++j) dw[i][j] = db[i][j] = 0.f;
-  int parity = 0;
-  for (long row = (long)blockIdx.x * ROWS + threadIdx.x / TPR; row < rows; row += (long)gridDim.x * ROWS, parity ^= 1) {
-    const float mu = mean[row], r = rstd[row];
-    Pack<T, VEC> a[VPT], d[VPT];
+  // Up to two chunks per thread the weight stays in registers and the next row is loaded while this one is summed: a block
+  // walks its rows in sequence, and each would pay the memory's latency after the last one's barrier. Wider rows have no
+  // registers for that.
+  constexpr bool kHold = VPT <= 2;
+  Pack<W, VEC> wv[VPT];
+  auto load_w = [&](int i) {
+    const int c = li + i * TPR;
+    wv[i] = get_chunk<W, VEC>(w + c * VEC, chunk_size<VEC>(c, nfull, tail));
+  };
+  if (kHold && w != nullptr) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) load_w(i);
+  }
+  struct Row {
+    Pack<T, VEC> s[VPT], dy[VPT], dres[VPT];
+    float mean, rstd;
+  };
+  auto load_row = [&](long row, Row& r) {
+    r.mean = mean[row];
+    r.rstd = rstd[row];
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int c = li + i * TPR;
-      const int n = c < nfull ? VEC : (c == nfull ? tail : 0);
-      const T* ap = s + row * s_stride + c * VEC;
-      const T* dp = dy + row * dy_stride + c * VEC;
-      a[i] = n == VEC ? load_any<T, VEC>(ap) : load_part<T, VEC>(ap, n);
-      d[i] = n == VEC ? load_any<T, VEC>(dp) : load_part<T, VEC>(dp, n);  // zero past the row: adds nothing below
+      const T *sp = s + row * s_stride + c * VEC, *dp = dy + row * dy_stride + c * VEC, *qp = dres + row * dres_stride + c * VEC;
+      const int n = chunk_size<VEC>(c, nfull, tail);
+      r.s[i] = get_chunk<T, VEC>(sp, n);
+      r.dy[i] = get_chunk<T, VEC>(dp, n);  // zero past the row: adds nothing below
+      if (dres != nullptr) r.dres[i] = get_chunk<T, VEC>(qp, n);
     }
+  };
+  const long step = (long)gridDim.x * ROWS;
+  long row = first_row<TPR, ROWS>();
+  Row next;
+  if (kHold && row < rows) load_row(row, next);
+  int parity = 0;
+  for (; row < rows; row += step, parity ^= 1) {
+    Row cur;
+    if constexpr (kHold) {
+      cur = next;
+      if (row + step < rows) load_row(row + step, next);
+    } else {
+      load_row(row, cur);
+    }
+    const float mu = cur.mean, r = cur.rstd;
     float s1 = 0.f, s2 = 0.f;
-    float g[VPT][VEC];
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const int c = li + i * TPR;
-      const int n = c < nfull ? VEC : (c == nfull ? tail : 0);
-      Pack<W, VEC> ww;
-      if (w != nullptr) ww = n == VEC ? load_wide<W, VEC>(w + c * VEC) : load_part<W, VEC>(w + c * VEC, n);
+      if (!kHold && w != nullptr) load_w(i);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        const float dd = to_f<T>(d[i].v[j]), h = (to_f<T>(a[i].v[j]) - mu) * r;
-        g[i][j] = w != nullptr ? dd * to_f<W>(ww.v[j]) : dd;
+        const float dd = cur.dy[i].get(j), h = (cur.s[i].get(j) - mu) * r;
+        const float g = w != nullptr ? dd * wv[i].get(j) : dd;
         dw[i][j] = fmaf(dd, h, dw[i][j]);
         db[i][j] += dd;
-        s1 += g[i][j];
-        s2 = fmaf(g[i][j], h, s2);
+        s1 += g;
+        s2 = fmaf(g, h, s2);
       }
     }
     s1 = wave_reduce<OpSum>(s1);
@@ -174,22 +218,18 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_bwd_kernel(
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int c = li + i * TPR;
-      const int n = c < nfull ? VEC : (c == nfull ? tail : 0);
+      const int n = chunk_size<VEC>(c, nfull, tail);
       if (n == 0) continue;
-      Pack<T, VEC> q, o;
-      if (dres != nullptr) {
-        const T* qp = dres + row * dres_stride + c * VEC;
-        q = n == VEC ? load_any<T, VEC>(qp) : load_part<T, VEC>(qp, n);
-      }
+      float o[VEC];
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        const float h = (to_f<T>(a[i].v[j]) - mu) * r;
-        float f = r * (g[i][j] - s1 - h * s2);
-        if (dres != nullptr) f += to_f<T>(q.v[j]);
-        o.v[j] = from_f<T>(f);
+        const float dd = cur.dy[i].get(j), h = (cur.s[i].get(j) - mu) * r;
+        const float g = w != nullptr ? dd * wv[i].get(j) : dd;
+        float f = r * (g - s1 - h * s2);
+        if (dres != nullptr) f += cur.dres[i].get(j);
+        o[j] = f;
       }
-      if (n == VEC) store_any<T, VEC>(dx + row * H + c * VEC, o);
-      else store_part<T, VEC>(dx + row * H + c * VEC, o, n);
+      put_chunk<T, VEC>(dx + row * H + c * VEC, Pack<T, VEC>::of(o), n);
     }
   }
   if (part == nullptr) return;
@@ -279,13 +319,29 @@ long row_stride(const c10::optional<torch::Tensor>& t) { return t.has_value() ? 
 // Calls go(threads of a row, chunks of each) for a row of `chunks` 16-byte chunks.
 template <int N> using Const = std::integral_constant<int, N>;
 template <typename F>
-void by_width(long chunks, F go) {
+void by_width_fwd(long chunks, long rows, F go) {
+  if (chunks <= 64) return go(Const<64>{}, Const<1>{});
+  if (rows >= 1024) {  // enough rows to fill the chip: few threads for each, and no barriers up to 256 chunks
+    if (chunks <= 128) return go(Const<64>{}, Const<2>{});
+    if (chunks <= 256) return go(Const<64>{}, Const<4>{});
+    if (chunks <= 512) return go(Const<256>{}, Const<2>{});
+    if (chunks <= 1024) return go(Const<256>{}, Const<4>{});
+  }
+  // few rows: as many threads as a row feeds, for the shortest way through one
+  if (chunks <= 256) return go(Const<256>{}, Const<1>{});
+  if (chunks <= 512) return go(Const<512>{}, Const<1>{});
+  if (chunks <= 1024) return go(Const<1024>{}, Const<1>{});
+  if (chunks <= 2048) return go(Const<1024>{}, Const<2>{});
+  go(Const<1024>{}, Const<4>{});
+}
+template <typename F>
+void by_width_bwd(long chunks, F go) {
   if (chunks <= 64) go(Const<64>{}, Const<1>{});
   else if (chunks <= 128) go(Const<64>{}, Const<2>{});
-  else if (chunks <= 256) go(Const<64>{}, Const<4>{});
+  else if (chunks <= 256) go(Const<256>{}, Const<1>{});
   else if (chunks <= 512) go(Const<256>{}, Const<2>{});
-  else if (chunks <= 1024) go(Const<256>{}, Const<4>{});
-  else if (chunks <= 2048) go(Const<512>{}, Const<4>{});
+  else if (chunks <= 1024) go(Const<512>{}, Const<2>{});
+  else if (chunks <= 2048) go(Const<1024>{}, Const<2>{});
   else go(Const<1024>{}, Const<4>{});
 }
 
@@ -294,9 +350,9 @@ void launch_fwd(const torch::Tensor& x, const c10::optional<torch::Tensor>& res,
                 const c10::optional<torch::Tensor>& b, const torch::Tensor& y, const torch::Tensor& sum,
                 const torch::Tensor& mean, const torch::Tensor& rstd, float eps, hipStream_t stream) {
   const long rows = x.size(0), H = x.size(1);
-  by_width((H * (long)sizeof(T) + 15) / 16, [&](auto tpr, auto vpt) {
+  by_width_fwd((H * (long)sizeof(T) + 15) / 16, rows, [&](auto tpr, auto vpt) {
     constexpr int TPR = decltype(tpr)::value, VPT = decltype(vpt)::value, NT = TPR < 256 ? 256 : TPR, per = NT / TPR;
-    const long want = (rows + per - 1) / per, most = 2048L * 256 / NT;
+    const long want = (rows + per - 1) / per, most = 1024L * 256 / NT;
     hipLaunchKernelGGL((layer_norm_fwd_kernel<T, W, TPR, VPT>), dim3((unsigned)std::min(want, most)), dim3(NT), 0, stream,
                        reinterpret_cast<const T*>(x.data_ptr()), x.stride(0), ptr<T>(res), row_stride(res), ptr<W>(w), ptr<W>(b),
                        out_ptr<T>(y), out_ptr<T>(sum), out_ptr<float>(mean), out_ptr<float>(rstd), rows, (int)H, eps);
@@ -312,7 +368,7 @@ void launch_bwd(const torch::Tensor& dy, const torch::Tensor& s, const c10::opti
   const bool sums = dw.defined() || db.defined();
   torch::Tensor part;
   long blocks = 0;
-  by_width(chunks, [&](auto tpr, auto vpt) {
+  by_width_bwd(chunks, [&](auto tpr, auto vpt) {
     constexpr int TPR = decltype(tpr)::value, VPT = decltype(vpt)::value, NT = TPR < 256 ? 256 : TPR, per = NT / TPR;
     blocks = std::min((rows + per - 1) / per, 512L * 256 / NT);
     if (sums) part = torch::empty({blocks, 2, pitch}, s.options().dtype(at::kFloat));

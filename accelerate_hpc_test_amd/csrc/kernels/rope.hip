@@ -1,11 +1,13 @@
 // Rotary positions in every layout: half pairs (i, i + R/2) or interleaved pairs (2i, 2i + 1) of the first R of D values of
 // heads [0, n_rot), the rest of the head and the other heads copied; bf16 / fp16 / fp32, fp32 cos / sin tables [S, R/2]:
 //   out_a = a cos - b sin,  out_b = b cos + a sin;  the gradient turns back (sin negated).
-// Bound by memory: one read and one write of every value. A head is cut into items of W values (pairs of W-value chunks in
-// the half layout), and a thread keeps one item position for all the (token, head) units it walks, so the cos / sin of a
-// token are loaded once and serve all its heads from registers. Where a part is no multiple of W its last item starts early
-// and overlaps the one before: both write the same bytes, and every access stays W wide at any even R and any D. The source
-// may have any strides over batch, sequence and heads.
+// Bound by memory: one read and one write of every value. A head is cut into windows of 16 bytes, the last one moved back to
+// end with the head (windows that overlap write the same bytes), so every load and store is whole and all lanes of a wave
+// move data, whatever R and D are: out = x cos + partner (+-sin) needs the partners of a window's values beside them, which
+// are a swap in registers (interleaved) or second loads of a line that is in flight anyway (half layout: one, or
+// a few where the halves do not divide into windows). A thread keeps one window position for all the
+// (token, head) units that it walks, so a token's cos / sin are loaded once and serve all its heads from registers. The
+// source may have any strides over batch, sequence and heads.
 #include <hip/hip_runtime.h>
 #include <torch/extension.h>
 #include <ATen/hip/HIPContext.h>
@@ -19,21 +21,15 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kUnroll = 2;  // units in flight per thread
-constexpr int kMaxHead = 1000;  // a head's items fit kThreads at any width
+constexpr int kPasses = 4;  // units a thread walks in a long call
+constexpr int kMaxHead = 1000;  // a head's windows fit kThreads at any width
 
+// n of N angles (all of them in whole windows); the rest is not looked up
 template <int N>
-__device__ __forceinline__ void load_angles(const float* __restrict__ p, float (&f)[N]) {
-  if constexpr (N >= 4) {
+__device__ __forceinline__ void load_angles(const float* __restrict__ p, float (&f)[N], int n) {
+  const Pack<float, N> v = n == N ? load_any<float, N>(p) : load_part<float, N>(p, n);
 #pragma unroll
-    for (int j = 0; j < N; j += 4) {
-      const Pack<float, 4> v = load_any<float, 4>(p + j);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) f[j + q] = v.v[q];
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < N; ++j) f[j] = p[j];
-  }
+  for (int j = 0; j < N; ++j) f[j] = v.get(j);
 }
 
 struct RopeArgs {
@@ -41,27 +37,40 @@ struct RopeArgs {
   long pb, ps;      // position strides
   long units;       // batch * seq * heads
   int seq, heads, n_rot, D, R, S;
-  int n_pair, n_copy;  // items of the rotated part (pairs of chunks in the half layout), items of the rest
   int units_per_block;
   float sign;
 };
 
-// W: values of a rotated item, M: of a copied one (16 bytes).
-template <typename T, int W, bool INTERLEAVED>
+// The pairs of a window that starts with one, exchanged.
+template <typename T, int M>
+__device__ __forceinline__ Pack<T, M> swap_pairs(const Pack<T, M>& x) {
+  Pack<T, M> p;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int j = 0; j < M; ++j) p.u[j] = x.u[j ^ 1];
+  } else {
+#pragma unroll
+    for (int i = 0; i < M / 2; ++i) p.u[i] = (x.u[i] << 16) | (x.u[i] >> 16);
+  }
+  return p;
+}
+
+// G: a window falls into pieces of G values that turn together, with partners side by side (half layout: the largest power of
+// two that divides the half, the head and 16 bytes; interleaved: the whole window where the head is even, else 1).
+template <typename T, int G, bool INTERLEAVED>
 __global__ __launch_bounds__(kThreads) void rope_any_kernel(const T* __restrict__ src, T* __restrict__ dst,
                                                             const float* __restrict__ cosb, const float* __restrict__ sinb,
                                                             const int64_t* __restrict__ pos, const RopeArgs a) {
-  constexpr int NC = INTERLEAVED ? W / 2 : W, M = 16 / sizeof(T);
-  const int items = a.n_pair + a.n_copy;
-  const int slots = kThreads / items;  // units walked side by side by a block
-  const int slot = threadIdx.x / items, item = threadIdx.x - slot * items;
+  constexpr int M = 16 / sizeof(T);
+  constexpr bool kSwap = INTERLEAVED && G > 1;  // partners within the window
+  const int windows = (a.D + M - 1) / M;
+  const int slots = kThreads / windows;  // units walked side by side by a block
+  const int slot = threadIdx.x / windows, item = threadIdx.x - slot * windows;
   if (slot >= slots) return;
-  const int half = a.R >> 1, rest = a.D - a.R;
-  const bool pair = item < a.n_pair;
-  const int part = !pair && rest < M ? rest : 0;  // a rest too short for one access
-  const int span = INTERLEAVED ? a.R : half;
-  const int d0 = pair ? min(item * W, span - W) : part > 0 ? a.R : min(a.R + (item - a.n_pair) * M, a.D - M);
-  const int angle0 = INTERLEAVED ? d0 >> 1 : d0;
+  const int half = a.R >> 1;
+  const bool short_head = a.D < M;
+  const int d0 = short_head ? 0 : min(item * M, a.D - M);
+  const bool turns = d0 < a.R;
   const long first = (long)blockIdx.x * a.units_per_block;
   const int count = (int)min((long)a.units_per_block, a.units - first);
 
@@ -86,104 +95,104 @@ __global__ __launch_bounds__(kThreads) void rope_any_kernel(const T* __restrict_
 
   long have_b = -1;
   int have_s = -1;
-  float c[NC], s[NC];
+  float c[M], s[M];  // of this window's values; s has the partner's sign
   for (int u0 = slot; u0 < count; u0 += slots * kUnroll) {
-    Pack<T, W> x[kUnroll], z[kUnroll];
-    Pack<T, M> y[kUnroll];
+    Pack<T, M> x[kUnroll], z[kUnroll];
     long ub[kUnroll];
-    int us[kUnroll], uh[kUnroll];
+    int us[kUnroll];
+    bool turn[kUnroll];
 #pragma unroll
     for (int k = 0; k < kUnroll; ++k) {
       if (u0 + k * slots < count) {
+        const T* p = src + bi * a.sb + si * a.ss + head * a.sh + d0;
+        x[k] = short_head ? load_part<T, M>(p, a.D) : load_any<T, M>(p);
+        turn[k] = turns && head < a.n_rot;
+        if constexpr (!kSwap) {
+          z[k] = Pack<T, M>::zero();
+          if (turn[k]) {
+#pragma unroll
+            for (int i = 0; i < M; i += G) {
+              const int d = d0 + i, other = INTERLEAVED ? d ^ 1 : d < half ? d + half : d - half;
+              if (d < a.R) z[k].template put<G>(i, load_any<T, G>(p + (other - d0)));
+            }
+          }
+        }
         ub[k] = bi;
         us[k] = si;
-        uh[k] = head;
-        const T* p = src + bi * a.sb + si * a.ss + head * a.sh + d0;
-        if (pair) {
-          x[k] = load_any<T, W>(p);
-          if (!INTERLEAVED) z[k] = load_any<T, W>(p + half);
-        } else {
-          y[k] = part > 0 ? load_part<T, M>(p, part) : load_any<T, M>(p);
-        }
         advance();
       }
     }
 #pragma unroll
     for (int k = 0; k < kUnroll; ++k) {
       if (u0 + k * slots < count) {
-        T* q = dst + (first + u0 + k * slots) * a.D + d0;
-        if (pair) {
-          if (uh[k] < a.n_rot) {
-            if (have_s != us[k] || have_b != ub[k]) {
-              have_s = us[k];
-              have_b = ub[k];
-              const long at = pos != nullptr ? pos[ub[k] * a.pb + us[k] * a.ps] : us[k];
-              const bool inside = at >= 0 && at < a.S;  // a position outside the tables is never looked up: NaN
-              ACC_CHECK(inside, kChkRopePos);
-              const long row = inside ? at * half + angle0 : 0;
-              if (inside) {
-                load_angles<NC>(cosb + row, c);
-                load_angles<NC>(sinb + row, s);
-              }
+        if (turn[k]) {
+          if (have_s != us[k] || have_b != ub[k]) {
+            have_s = us[k];
+            have_b = ub[k];
+            const long at = pos != nullptr ? pos[ub[k] * a.pb + us[k] * a.ps] : us[k];
+            const bool inside = at >= 0 && at < a.S;  // a position outside the tables is never looked up: NaN
+            ACC_CHECK(inside, kChkRopePos);
+            const long row = inside ? at * half : 0;
+            if constexpr (kSwap) {
+              float cc[M / 2], ss[M / 2];
+              load_angles<M / 2>(cosb + row + d0 / 2, cc, min(M / 2, half - d0 / 2));
+              load_angles<M / 2>(sinb + row + d0 / 2, ss, min(M / 2, half - d0 / 2));
 #pragma unroll
-              for (int j = 0; j < NC; ++j) {
-                c[j] = inside ? c[j] : NAN;
-                s[j] = inside ? s[j] * a.sign : NAN;
-              }
-            }
-            if constexpr (INTERLEAVED) {
-#pragma unroll
-              for (int j = 0; j < NC; ++j) {
-                const float p0 = to_f<T>(x[k].v[2 * j]), p1 = to_f<T>(x[k].v[2 * j + 1]);
-                x[k].v[2 * j] = from_f<T>(p0 * c[j] - p1 * s[j]);
-                x[k].v[2 * j + 1] = from_f<T>(p1 * c[j] + p0 * s[j]);
+              for (int j = 0; j < M; ++j) {
+                c[j] = cc[j / 2];
+                s[j] = j & 1 ? ss[j / 2] : -ss[j / 2];
               }
             } else {
 #pragma unroll
-              for (int j = 0; j < W; ++j) {
-                const float p0 = to_f<T>(x[k].v[j]), p1 = to_f<T>(z[k].v[j]);
-                x[k].v[j] = from_f<T>(p0 * c[j] - p1 * s[j]);
-                z[k].v[j] = from_f<T>(p1 * c[j] + p0 * s[j]);
+              for (int i = 0; i < M; i += G) {
+                const int d = d0 + i, angle = INTERLEAVED ? d / 2 : d < half ? d : d - half;
+                const bool minus = INTERLEAVED ? (d & 1) == 0 : d < half;
+                float cc[G], ss[G];
+                load_angles<G>(cosb + row + angle, cc, d < a.R ? G : 0);
+                load_angles<G>(sinb + row + angle, ss, d < a.R ? G : 0);
+#pragma unroll
+                for (int j = 0; j < G; ++j) {
+                  c[i + j] = cc[j];
+                  s[i + j] = minus ? -ss[j] : ss[j];
+                }
               }
             }
+#pragma unroll
+            for (int j = 0; j < M; ++j) {
+              c[j] = inside ? c[j] : NAN;
+              s[j] *= a.sign;
+            }
           }
-          store_any<T, W>(q, x[k]);
-          if (!INTERLEAVED) store_any<T, W>(q + half, z[k]);
-        } else if (part > 0) {
-          store_part<T, M>(q, y[k], part);
-        } else {
-          store_any<T, M>(q, y[k]);
+          if constexpr (kSwap) z[k] = swap_pairs<T, M>(x[k]);
+          float o[M];
+#pragma unroll
+          for (int j = 0; j < M; ++j) {
+            const float v = x[k].get(j);
+            o[j] = v * c[j] + z[k].get(j) * s[j];
+            if (d0 + j >= a.R) o[j] = v;
+          }
+          x[k] = Pack<T, M>::of(o);
         }
+        T* q = dst + (first + u0 + k * slots) * a.D + d0;
+        if (short_head) store_part<T, M>(q, x[k], a.D);
+        else store_any<T, M>(q, x[k]);
       }
     }
   }
 }
 
-template <typename T, int W>
+template <typename T, int G, bool INTERLEAVED>
 void launch(const torch::Tensor& src, const torch::Tensor& dst, const torch::Tensor& cos, const torch::Tensor& sin,
-            const int64_t* pos, RopeArgs a, bool interleaved, hipStream_t stream) {
+            const int64_t* pos, RopeArgs a, hipStream_t stream) {
   constexpr int M = 16 / sizeof(T);
-  const int span = interleaved ? a.R : a.R / 2;
-  a.n_pair = (span + W - 1) / W;
-  a.n_copy = (a.D - a.R + M - 1) / M;
-  TORCH_CHECK(a.n_pair + a.n_copy <= kThreads, "rope: head size");
-  const int slots = kThreads / (a.n_pair + a.n_copy);
+  const int slots = kThreads / ((a.D + M - 1) / M);
   // Each block walks a few units of every slot: enough to reuse a token's angles, few enough to fill the chip.
-  const long passes = std::min<long>(8, std::max<long>(1, a.units / ((long)slots * 2048)));
+  const long passes = std::min<long>(kPasses, std::max<long>(1, a.units / ((long)slots * 2048)));
   a.units_per_block = (int)(passes * slots);
   const long blocks = (a.units + a.units_per_block - 1) / a.units_per_block;
   TORCH_CHECK(blocks < (1L << 31), "rope: too many heads in one call");
-  const T* sp = reinterpret_cast<const T*>(src.data_ptr());
-  T* dp = reinterpret_cast<T*>(dst.data_ptr());
-  if constexpr (W > 1) {
-    if (interleaved) {
-      hipLaunchKernelGGL((rope_any_kernel<T, W, true>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, sp, dp,
-                         cos.data_ptr<float>(), sin.data_ptr<float>(), pos, a);
-      return;
-    }
-  }
-  hipLaunchKernelGGL((rope_any_kernel<T, W, false>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, sp, dp,
-                     cos.data_ptr<float>(), sin.data_ptr<float>(), pos, a);
+  hipLaunchKernelGGL((rope_any_kernel<T, G, INTERLEAVED>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, reinterpret_cast<const T*>(src.data_ptr()),
+                     reinterpret_cast<T*>(dst.data_ptr()), cos.data_ptr<float>(), sin.data_ptr<float>(), pos, a);
 }
 
 }  // namespace
@@ -223,13 +232,14 @@ torch::Tensor rope_any(torch::Tensor src, torch::Tensor cos, torch::Tensor sin, 
   }
   auto stream = at::hip::getCurrentHIPStream();
   ACC_FOR_FLOAT_TYPES(src.scalar_type(), "rope", {
-    // the widest item that the rotated part holds, up to 16 bytes; the rest of the head follows it
-    constexpr int most = 16 / sizeof(scalar);
-    const long span = interleaved ? R : R / 2;
-    if (most == 8 && span >= 8) launch<scalar, most>(src, out, cos, sin, pp, a, interleaved, stream);
-    else if (span >= 4) launch<scalar, 4>(src, out, cos, sin, pp, a, interleaved, stream);
-    else if (span >= 2) launch<scalar, 2>(src, out, cos, sin, pp, a, interleaved, stream);
-    else launch<scalar, 1>(src, out, cos, sin, pp, a, interleaved, stream);
+    constexpr int M = 16 / sizeof(scalar);
+    const auto fits = [&](long g) { return R / 2 % g == 0 && D % g == 0; };
+    auto go = [&](auto kind) { kind(src, out, cos, sin, pp, a, stream); };
+    if (interleaved) go(D % 2 == 0 ? launch<scalar, M, true> : launch<scalar, 1, true>);
+    else if (fits(M)) go(launch<scalar, M, false>);
+    else if (fits(4)) go(launch<scalar, 4, false>);
+    else if (fits(2)) go(launch<scalar, 2, false>);
+    else go(launch<scalar, 1, false>);
   });
   return out;
 }

@@ -6,14 +6,20 @@
 //   renormalised   softmax: dl_j = h_j (u_j - U)              sigmoid: dl_j = h_j (u_j - U) (1 - s_j)
 //   as they are    softmax: dl_e = s_e (u_e - sum u_j s_j)    sigmoid: dl_j = u_j s_j (1 - s_j)
 // (u_e = 0 for experts that were not chosen; the bias steers the choice alone and has no gradient.)
-// Bound by latency: a token's logits are a few hundred values, held by 8 to 64 lanes of one wave from the load to the last
-// choice. The order must not hang on a rounding of exp, so keys are computed in 64 bits where they are sums of scores and a
-// bias; where they are not (no bias, no groups) the scores' order is the logits' own and is taken from them. Keys become
-// unsigned integers of the same order: choosing is an integer maximum, NaN sorts below every number and cannot be chosen
-// twice.
+// What bounds the kernel is how many instructions a choice takes, not the bytes. A wave chooses for one token, each lane holding
+// 1 to 16 neighbouring experts:
+//   * keys are order-preserving unsigned integers; NaN sorts as -inf, a closed expert is 0;
+//   * a bisection over key values, counting by ballots, finds a bound that a few more than k keys reach (a handful of steps);
+//   * those are compacted in the order of their experts, and each counts the ones before it: that is its rank.
+// 16384 tokens with 256 experts in 8 groups, k = 8: 19.6 us (k rounds of a maximum over the lanes: 28.9 us; keys in 64 bits
+// throughout: 32.7 us), 64 tokens: 4.6 us. The order must not hang on a rounding of exp: where keys are sums of scores and a bias, a wave chooses by
+// keys in 32 bits, and does it again in 64 where two neighbours of the order, or the last open and the first closed group,
+// lie within the rounding errors of 32 (6 tokens in 10000 with distinct logits). Where keys are scores alone (no bias, no
+// closed groups) their order is the logits' own, and exact.
 #include <hip/hip_runtime.h>
 #include <torch/extension.h>
 #include <ATen/hip/HIPContext.h>
+#include <type_traits>
 
 #include "row_ops.h"
 
@@ -31,171 +37,309 @@ struct RouteArgs {
   float scale;
 };
 
-// Order-preserving keys; 0 is below all of them (taken, or not there), 1 a closed expert, 2 NaN.
+// Order-preserving keys above 0.
+__device__ __forceinline__ uint32_t order_key(float f) {
+  if (f != f) f = -INFINITY;
+  const uint32_t u = __float_as_uint(f + 0.f);
+  return u ^ ((u & 0x80000000u) ? 0xffffffffu : 0x80000000u);
+}
 __device__ __forceinline__ uint64_t order_key(double d) {
-  if (d != d) return 2;
-  uint64_t u = __double_as_longlong(d + 0.0);
+  if (d != d) d = -INFINITY;
+  const uint64_t u = __double_as_longlong(d + 0.0);
   return u ^ ((u >> 63) ? ~0ull : 0x8000000000000000ull);
 }
+__device__ __forceinline__ double key_value(uint64_t k) {
+  return __longlong_as_double(k ^ ((k >> 63) ? 0x8000000000000000ull : ~0ull));
+}
+__device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(k ^ ((k & 0x80000000u) ? 0x80000000u : 0xffffffffu)); }
 
-template <int L>
-__device__ __forceinline__ double lanes_sum(double v) {
+__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896340736f); }
+__device__ __forceinline__ double exp_of(double x) { return exp(x); }
+__device__ __forceinline__ float sigmoid_of(float x) { return __builtin_amdgcn_rcpf(1.f + exp_of(-x)); }
+__device__ __forceinline__ double sigmoid_of(double x) { return 1.0 / (1.0 + exp(-x)); }
+
+__device__ __forceinline__ double wave_sum64(double v) {
 #pragma unroll
-  for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
   return v;
 }
-template <int L>
-__device__ __forceinline__ double lanes_max(double v) {
+__device__ __forceinline__ float wave_sum_of(float v) { return wave_reduce<OpSum>(v); }
+__device__ __forceinline__ double wave_sum_of(double v) { return wave_sum64(v); }
+
+// Values at .. at + V - 1 of a row of n (`fill` past its end). `full`: the row has a value for every lane.
+template <typename T, int V>
+__device__ __forceinline__ void load_values(const T* __restrict__ row, int at, int n, bool full, float fill, float (&f)[V]) {
+  constexpr int C = V * sizeof(T) <= 16 ? V : 16 / sizeof(T);
+  if (full) {
 #pragma unroll
-  for (int o = L / 2; o > 0; o >>= 1) v = fmax(v, __shfl_xor(v, o, 64));
-  return v;
+    for (int i = 0; i < V; i += C) {
+      const Pack<T, C> x = load_any<T, C>(row + at + i);
+#pragma unroll
+      for (int v = 0; v < C; ++v) f[i + v] = x.get(v);
+    }
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v) f[v] = to_f<T>(row[min(at + v, n - 1)]);
+#pragma unroll
+    for (int v = 0; v < V; ++v) f[v] = at + v < n ? f[v] : fill;
+  }
 }
 
-// L lanes hold a token, V experts each: expert v * L + lane.
-template <typename T, int L, int V>
+// The scores of f[V], sigmoid, or softmax over the wave; 0 where f is -inf for want of an expert.
+template <int V, typename F>
+__device__ __forceinline__ void scores_of(const float (&f)[V], bool softmax, F (&s)[V]) {
+  if (softmax) {
+    float hi = f[0];  // -inf where there is no expert
+#pragma unroll
+    for (int v = 1; v < V; ++v) hi = fmaxf(hi, f[v]);
+    hi = wave_reduce<OpMax>(hi);
+    F sum = 0;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      s[v] = exp_of((F)f[v] - (F)hi);
+      sum += s[v];
+    }
+    const F inv = (F)1 / wave_sum_of(sum);
+#pragma unroll
+    for (int v = 0; v < V; ++v) s[v] *= inv;
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v) s[v] = sigmoid_of((F)f[v]);
+  }
+}
+
+// What a 32-bit key (a score and a bias) may be off: `noise` for its score, and one rounding of the sum. A sigmoid is within
+// 2^-22 (the exponent's rounding moves s by at most s (1 - s) |x| 2^-23 < 2^-25; exp, sum and reciprocal by a step of s each),
+// a softmax within 2^-19 of itself (exponent and exp, a sum of up to 1024 by lanes of 16, a reciprocal and a product: 30 half
+// steps where it matters: a score e^-d has d 2^-24 e^-d < 2^-25).
+__device__ __forceinline__ float key_margin(float key, float noise) { return noise + fabsf(key) * 0x1p-23f; }
+
+// This wave's writes to its shared memory are there for its other lanes.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// A wave's shared memory.
+template <int V>
+struct Scratch {
+  uint64_t keys[64 * V];  // every expert's, for the ratings; then the candidates'
+  int ids[64 * V];        // the candidates' experts
+  uint64_t sorted[kMaxTop + 1];
+  int chosen[kMaxTop + 1];
+};
+
+// The two best values of a group's lanes, an aligned power of two of them.
+template <typename F>
+__device__ __forceinline__ void merge_two(F& first, F& second, F of, F os) {
+  const F low = of > first ? first : of, high = second > os ? second : os;
+  first = of > first ? of : first;
+  second = low > high ? low : high;
+}
+__device__ __forceinline__ void best_two(float& first, float& second, int lanes) {
+  auto step = [&](auto move) { merge_two(first, second, move(first), move(second)); };
+  if (lanes >= 2) step([](float v) { return __uint_as_float(dpp_move<0xB1>(__float_as_uint(v))); });
+  if (lanes >= 4) step([](float v) { return __uint_as_float(dpp_move<0x4E>(__float_as_uint(v))); });
+  if (lanes >= 8) step([](float v) { return __uint_as_float(dpp_move<0x141>(__float_as_uint(v))); });
+  if (lanes >= 16) step([](float v) { return __uint_as_float(dpp_move<0x140>(__float_as_uint(v))); });
+  if (lanes >= 32) step([](float v) { return __shfl_xor(v, 16, 64); });
+}
+__device__ __forceinline__ void best_two(double& first, double& second, int lanes) {
+  for (int o = 1; o < lanes; o <<= 1) merge_two(first, second, __shfl_xor(first, o, 64), __shfl_xor(second, o, 64));
+}
+
+__device__ __forceinline__ float lane_value(float v, int lane) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane)); }
+__device__ __forceinline__ double lane_value(double v, int lane) {
+  const uint64_t u = __double_as_longlong(v);
+  const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)u, lane), hi = __builtin_amdgcn_readlane((int)(u >> 32), lane);
+  return __longlong_as_double(((uint64_t)hi << 32) | lo);
+}
+__device__ __forceinline__ uint32_t high_of(uint32_t k) { return k; }
+__device__ __forceinline__ uint32_t high_of(uint64_t k) { return (uint32_t)(k >> 32); }
+
+// Lane l holds experts l * V .. l * V + V - 1 of a token. Leaves the k experts that keys of type F choose in `sh.chosen`, in order.
+// False (F = float): two keys are too close to call. `by_logit`: the logits are the keys, and exact.
+template <int V, typename F>
+__device__ __forceinline__ bool choose(const float (&f)[V], const float* __restrict__ bias, Scratch<V>& sh, bool by_logit,
+                                       const RouteArgs& a) {
+  constexpr bool kWide = sizeof(F) == 8;
+  using Key = typename std::conditional<kWide, uint64_t, uint32_t>::type;
+  const int lane = threadIdx.x & 63, e0 = lane * V;
+  Key* const keys = reinterpret_cast<Key*>(sh.keys);
+  Key* const sorted = reinterpret_cast<Key*>(sh.sorted);
+  Key key[V];
+  float noise = 0x1p-22f;
+  {
+    F d[V];
+    if (by_logit) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) d[v] = f[v];
+    } else {
+      scores_of<V, F>(f, a.softmax, d);
+      if (!kWide && a.softmax) {
+        float most = (float)d[0];
+#pragma unroll
+        for (int v = 1; v < V; ++v) most = fmaxf(most, (float)d[v]);
+        noise = wave_reduce<OpMax>(most) * 0x1p-19f;
+      }
+      if (bias != nullptr) {
+        float b[V];
+        load_values<float, V>(bias, e0, a.E, a.E == 64 * V, 0.f, b);
+#pragma unroll
+        for (int v = 0; v < V; ++v) d[v] += (F)b[v];
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) key[v] = e0 + v < a.E ? order_key(d[v]) : (Key)0;
+  }
+  if (a.top_groups < a.groups) {
+    // Ratings: the lanes share out over the groups, a power of two for each.
+    const int size = a.E / a.groups, per = 64 >> (32 - __clz(a.groups - 1)), g = lane / per;
+#pragma unroll
+    for (int v = 0; v < V; ++v) keys[e0 + v] = key[v];
+    wave_sync();
+    F first = (F)-INFINITY, second = (F)-INFINITY;
+    if (g < a.groups)
+      for (int q = lane & (per - 1); q < size; q += per) merge_two(first, second, key_value(keys[g * size + q]), (F)-INFINITY);
+    best_two(first, second, per);
+    const F rating = size > 1 ? first + second : first;
+    int above = 0;
+    for (int i = 0; i < a.groups; ++i) {
+      const F other = lane_value(rating, i * per);
+      above += other > rating || (other == rating && i < g);
+    }
+    const bool in = g < a.groups && above < a.top_groups;
+    if constexpr (!kWide) {
+      const float worst = -wave_reduce<OpMax>(in ? -rating : -INFINITY), best = wave_reduce<OpMax>(g < a.groups && !in ? rating : -INFINITY);
+      if (!(worst - best > 2.f * (key_margin(worst, noise) + key_margin(best, noise)))) return false;
+    }
+    const uint64_t open = __ballot(in);
+    const float inv = 1.f / (float)size;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int eg = (int)(((float)(e0 + v) + 0.5f) * inv);  // exact: E <= 1024
+      if (!((open >> (eg * per & 63)) & 1)) key[v] = 0;
+    }
+    wave_sync();  // the keys are read: the candidates' may take their place
+  }
+
+  // A bound that at least `need` keys reach (one more than k shows how far the first one left out is), and few exceed it.
+  uint32_t hi_key = 0;
+  int open_count = 0;
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    hi_key = high_of(key[v]) > hi_key ? high_of(key[v]) : hi_key;
+    open_count += __popcll(__ballot(key[v] != 0));
+  }
+  const int need = kWide || by_logit || a.k == open_count ? a.k : a.k + 1;
+  // the least of the lanes' best keys is reached by as many keys as there are lanes that have one
+  const uint64_t holders = __ballot(hi_key != 0);
+  uint32_t low = 1;  // reached by all
+  if (__popcll(holders) >= need) low = ~lanes_max_u32<64>(hi_key != 0 ? ~hi_key : 0);
+  uint32_t high = lanes_max_u32<64>(hi_key);  // the bound is at most this
+  low = __builtin_amdgcn_readfirstlane(low);
+  high = __builtin_amdgcn_readfirstlane(high);
+  while (low < high) {
+    const uint32_t mid = low + (high - low + 1) / 2;
+    int reach = 0;
+#pragma unroll
+    for (int v = 0; v < V; ++v) reach += __popcll(__ballot(high_of(key[v]) >= mid));
+    if (reach >= need) {
+      low = mid;
+      if (reach <= need + 8) break;
+    } else {
+      high = mid - 1;
+    }
+  }
+
+  // The candidates, in the order of their experts.
+  int at = 0, n = 0;
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const uint64_t m = __ballot(high_of(key[v]) >= low);
+    n += __popcll(m);
+    at = __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, at));
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v)
+    if (high_of(key[v]) >= low) {
+      keys[at] = key[v];
+      sh.ids[at++] = e0 + v;
+    }
+  wave_sync();
+  for (int i = lane; i < n; i += 64) {
+    const Key mine = keys[i];
+    int rank = 0;
+#pragma unroll 4
+    for (int q = 0; q < n; ++q) {
+      const Key other = keys[q];
+      rank += other > mine || (other == mine && q < i);
+    }
+    if (rank < need) {
+      sorted[rank] = mine;
+      sh.chosen[rank] = sh.ids[i];
+    }
+  }
+  wave_sync();
+  if constexpr (!kWide) {
+    if (!by_logit) {
+      bool close = false;
+      if (lane + 1 < need) {
+        const float one = key_value(sorted[lane]), next = key_value(sorted[lane + 1]);
+        close = !(one - next > key_margin(one, noise) + key_margin(next, noise));
+      }
+      if (__any(close)) return false;
+    }
+  }
+  return true;
+}
+
+template <typename T, int V>
 __global__ __launch_bounds__(kThreads) void route_fwd_kernel(const T* __restrict__ logits, const float* __restrict__ bias,
                                                              float* __restrict__ weights, int64_t* __restrict__ experts,
                                                              const RouteArgs a) {
-  constexpr int PER = kThreads / L;
-  __shared__ double rating_of[kThreads / 64][kMaxGroups];
-  __shared__ double keys_of[kThreads / 64][L == 64 ? V * 64 : 1];
-  const int lane = threadIdx.x % L, wave = threadIdx.x >> 6;
-  const long row = (long)blockIdx.x * PER + threadIdx.x / L;
-  const bool live = row < a.rows;  // lanes of rows past the end walk along: no lane leaves before the last exchange
-  const T* x = logits + (live ? row : 0) * a.stride;
+  __shared__ Scratch<V> scratch[kThreads / 64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const long row = (long)blockIdx.x * (kThreads / 64) + wave;
+  if (row >= a.rows) return;  // the whole wave: nothing below waits for the block
+  const T* x = logits + row * a.stride;
+  Scratch<V>& sh = scratch[wave];
   float f[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) f[v] = v * L + lane < a.E ? to_f<T>(x[v * L + lane]) : -INFINITY;
-
-  uint64_t key[V];
-  float score[V];
+  load_values<T, V>(x, lane * V, a.E, a.E == 64 * V, -INFINITY, f);
   const bool by_logit = bias == nullptr && a.top_groups == a.groups;
-  double hi = -INFINITY, total = 0.0;
-  if (a.softmax) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) hi = (v * L + lane < a.E) ? fmax(hi, (double)f[v]) : hi;
-    hi = lanes_max<L>(hi);
-  }
-  if (by_logit) {
-    float sum = 0.f;
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const bool there = v * L + lane < a.E;
-      score[v] = a.softmax ? expf(f[v] - (float)hi) : 1.f / (1.f + expf(-f[v]));
-      if (there) sum += score[v];
-      key[v] = there ? order_key((double)f[v]) : 0;
-    }
-    if (a.softmax) {
-#pragma unroll
-      for (int o = L / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-#pragma unroll
-      for (int v = 0; v < V; ++v) score[v] /= sum;
-    }
-  } else {
-    double d[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const bool there = v * L + lane < a.E;
-      d[v] = a.softmax ? exp((double)f[v] - hi) : 1.0 / (1.0 + exp(-(double)f[v]));
-      if (there) total += d[v];
-    }
-    if (a.softmax) {
-      total = lanes_sum<L>(total);
-#pragma unroll
-      for (int v = 0; v < V; ++v) d[v] /= total;
-    }
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const int e = v * L + lane;
-      const bool there = e < a.E;
-      score[v] = (float)d[v];
-      if (there && bias != nullptr) d[v] += (double)bias[e];
-      key[v] = there ? order_key(d[v]) : 0;
-      if constexpr (L == 64)
-        if (there && a.top_groups < a.groups) keys_of[wave][e] = d[v];
-    }
-    if constexpr (L == 64) {
-      if (a.top_groups < a.groups) {
-        const int size = a.E / a.groups;
-        __syncthreads();
-        uint64_t mine = 0;
-        if (lane < a.groups) {
-          // two largest by their order, summed in 64 bits
-          double first = 0.0, second = 0.0;
-          uint64_t kf = 0, ks = 0;
-          for (int i = 0; i < size; ++i) {
-            const double q = keys_of[wave][lane * size + i];
-            const uint64_t kq = order_key(q);
-            if (kq > kf) {
-              second = first;
-              ks = kf;
-              first = q;
-              kf = kq;
-            } else if (kq > ks) {
-              second = q;
-              ks = kq;
-            }
-          }
-          const double rating = size > 1 ? first + second : first;
-          rating_of[wave][lane] = rating;
-          mine = order_key(rating);
-        }
-        __syncthreads();
-        int above = 0;
-        if (lane < a.groups)
-          for (int g = 0; g < a.groups; ++g) {
-            const uint64_t other = order_key(rating_of[wave][g]);
-            above += other > mine || (other == mine && g < lane);
-          }
-        const uint64_t open = __ballot(lane < a.groups && above < a.top_groups);
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          const int e = v * L + lane;
-          if (e < a.E && !((open >> (e / size)) & 1)) key[v] = 1;
-        }
-      }
-    }
+  if (!choose<V, float>(f, bias, sh, by_logit, a)) {
+    wave_sync();
+    choose<V, double>(f, bias, sh, false, a);
   }
 
-  // k times the best key of the token's lanes; lane j keeps choice j
-  float my_score = 0.f, sum = 0.f;
-  int my_expert = 0;
-  for (int j = 0; j < a.k; ++j) {
-    uint64_t best = 0;
-    int at = 0;
-    float s = 0.f;
+  // The weights, a choice in each lane. Shares are of the chosen alone: a softmax needs no sum over all experts for them.
+  const int id = lane < a.k ? sh.chosen[lane] : 0;
+  const float v = to_f<T>(x[id]);
+  float w;
+  if (a.softmax) {
+    float hi = f[0];
 #pragma unroll
-    for (int v = 0; v < V; ++v)
-      if (key[v] > best) {
-        best = key[v];
-        at = v * L + lane;
-        s = score[v];
-      }
+    for (int i = 1; i < V; ++i) hi = fmaxf(hi, f[i]);
+    hi = wave_reduce<OpMax>(hi);
+    float all = 0.f;  // also: NaN where a logit is NaN or +inf, or all are -inf
 #pragma unroll
-    for (int o = 1; o < L; o <<= 1) {
-      const uint64_t ob = __shfl_xor((unsigned long long)best, o, 64);
-      const int oa = __shfl_xor(at, o, 64);
-      const float os = __shfl_xor(s, o, 64);
-      if (ob > best || (ob == best && oa < at)) {
-        best = ob;
-        at = oa;
-        s = os;
-      }
-    }
-#pragma unroll
-    for (int v = 0; v < V; ++v)
-      if (v * L + lane == at) key[v] = 0;
-    sum += s;
-    if (lane == j) {
-      my_score = s;
-      my_expert = at;
+    for (int i = 0; i < V; ++i) all += exp_of(f[i] - hi);
+    all = wave_reduce<OpSum>(all);
+    w = lane < a.k ? exp_of(v - hi) : 0.f;
+    const float sum = a.renorm ? wave_reduce<OpSum>(w) : all;
+    w = all == all ? w / fmaxf(sum, 1.17549435e-38f) : NAN;
+  } else {
+    w = lane < a.k ? sigmoid_of(v) : 0.f;
+    if (a.renorm) {
+      const float sum = wave_reduce<OpSum>(w);
+      // scores that are all zero share nothing: 0, not 0 / 0
+      w = sum == sum ? w / fmaxf(sum, 1.17549435e-38f) : NAN;
     }
   }
-  if (live && lane < a.k) {
-    // scores that are all zero share nothing: 0, not 0 / 0
-    const float share = a.renorm ? my_score / fmaxf(sum, 1.17549435e-38f) : my_score;
-    weights[row * a.k + lane] = (sum != sum ? NAN : share) * a.scale;
-    experts[row * a.k + lane] = my_expert;
+  if (lane < a.k) {
+    weights[row * a.k + lane] = w * a.scale;
+    experts[row * a.k + lane] = id;
   }
 }
 
@@ -262,18 +406,15 @@ __global__ __launch_bounds__(kThreads) void route_bwd_kernel(const T* __restrict
     if (v * L + lane < a.E) o[v * L + lane] = from_f<T>(g[v]);
 }
 
-// Calls go(lanes of a token, experts per lane). A token with groups takes a whole wave.
 template <int N> using Const = std::integral_constant<int, N>;
+// Calls go(experts per lane of a wave).
 template <typename F>
-void by_experts(int E, bool whole_wave, F go) {
-  if (E <= 8 && !whole_wave) go(Const<8>{}, Const<1>{});
-  else if (E <= 16 && !whole_wave) go(Const<16>{}, Const<1>{});
-  else if (E <= 32 && !whole_wave) go(Const<32>{}, Const<1>{});
-  else if (E <= 64) go(Const<64>{}, Const<1>{});
-  else if (E <= 128) go(Const<64>{}, Const<2>{});
-  else if (E <= 256) go(Const<64>{}, Const<4>{});
-  else if (E <= 512) go(Const<64>{}, Const<8>{});
-  else go(Const<64>{}, Const<16>{});
+void by_experts(int E, F go) {
+  if (E <= 64) go(Const<1>{});
+  else if (E <= 128) go(Const<2>{});
+  else if (E <= 256) go(Const<4>{});
+  else if (E <= 512) go(Const<8>{});
+  else go(Const<16>{});
 }
 
 RouteArgs args_of(const torch::Tensor& logits, int64_t k, bool softmax, int64_t groups, int64_t top_groups, bool renorm, double scale) {
@@ -305,10 +446,9 @@ std::vector<torch::Tensor> route_experts_fwd(torch::Tensor logits, int64_t k, bo
   if (a.rows == 0) return {w, ids};
   auto stream = at::hip::getCurrentHIPStream();
   ACC_FOR_FLOAT_TYPES(logits.scalar_type(), "route_experts", {
-    by_experts(a.E, a.top_groups < a.groups, [&](auto l, auto v) {
-      constexpr int L = decltype(l)::value, V = decltype(v)::value;
-      constexpr int per = kThreads / L;
-      hipLaunchKernelGGL((route_fwd_kernel<scalar, L, V>), dim3((unsigned)((a.rows + per - 1) / per)), dim3(kThreads), 0, stream,
+    by_experts(a.E, [&](auto v) {
+      constexpr int V = decltype(v)::value, per = kThreads / 64;
+      hipLaunchKernelGGL((route_fwd_kernel<scalar, V>), dim3((unsigned)((a.rows + per - 1) / per)), dim3(kThreads), 0, stream,
                          reinterpret_cast<const scalar*>(logits.data_ptr()), bias.has_value() ? bias->data_ptr<float>() : nullptr,
                          w.data_ptr<float>(), ids.data_ptr<int64_t>(), a);
     });
@@ -328,13 +468,17 @@ torch::Tensor route_experts_bwd(torch::Tensor logits, torch::Tensor weights, tor
   if (a.rows == 0) return out;
   auto stream = at::hip::getCurrentHIPStream();
   ACC_FOR_FLOAT_TYPES(logits.scalar_type(), "route_experts", {
-    by_experts(a.E, false, [&](auto l, auto v) {
-      constexpr int L = decltype(l)::value, V = decltype(v)::value;
-      constexpr int per = kThreads / L;
+    auto go = [&](auto l, auto v) {
+      constexpr int L = decltype(l)::value, V = decltype(v)::value, per = kThreads / L;
       hipLaunchKernelGGL((route_bwd_kernel<scalar, L, V>), dim3((unsigned)((a.rows + per - 1) / per)), dim3(kThreads), 0, stream,
                          reinterpret_cast<const scalar*>(logits.data_ptr()), weights.data_ptr<float>(), experts.data_ptr<int64_t>(),
                          dw.data_ptr<float>(), reinterpret_cast<scalar*>(out.data_ptr()), a);
-    });
+    };
+    // up to 32 experts several tokens share a wave; a token's lanes hold a choice each, so they are as many as the experts
+    if (a.E <= 8) go(Const<8>{}, Const<1>{});
+    else if (a.E <= 16) go(Const<16>{}, Const<1>{});
+    else if (a.E <= 32) go(Const<32>{}, Const<1>{});
+    else by_experts(a.E, [&](auto v) { go(Const<64>{}, v); });
   });
   return out;
 }

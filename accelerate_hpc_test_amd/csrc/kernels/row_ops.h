@@ -4,6 +4,7 @@
 
 #include <hip/hip_runtime.h>
 #include <c10/core/DeviceGuard.h>
+#include <type_traits>
 
 #include "common.h"
 
@@ -13,10 +14,59 @@ using half_t = _Float16;
 template <> __device__ __forceinline__ float to_f<half_t>(half_t x) { return static_cast<float>(x); }
 template <> __device__ __forceinline__ half_t from_f<half_t>(float x) { return static_cast<half_t>(x); }
 
-template <typename T, int N> struct alignas(sizeof(T) * N) Pack { T v[N]; };
+// N elements as they lie in memory, two 16-bit ones to a register: arrays of 16-bit values end up one to a register.
+template <typename T, int N>
+struct Pack {
+  static constexpr int kWords = sizeof(T) * N < 4 ? 1 : sizeof(T) * N / 4;
+  uint32_t u[kWords];
 
-// N elements in one access from an address that is a multiple of the element size only: global memory takes 16-byte
-// accesses at any alignment, so rows of odd width, and views at odd offsets, move as wide as aligned ones.
+  __device__ __forceinline__ float get(int j) const {
+    if constexpr (sizeof(T) == 4) {
+      return __uint_as_float(u[j]);
+    } else {
+      const uint32_t w = u[j / 2];
+      if constexpr (std::is_same<T, half_t>::value) return to_f<T>(__builtin_bit_cast(half_t, (uint16_t)(j & 1 ? w >> 16 : w)));
+      else return __uint_as_float(j & 1 ? w & 0xffff0000u : w << 16);
+    }
+  }
+  static __device__ __forceinline__ Pack of(const float (&f)[N]) {
+    Pack p;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) p.u[j] = __float_as_uint(f[j]);
+    } else if constexpr (N == 1) {
+      p.u[0] = __builtin_bit_cast(uint16_t, from_f<T>(f[0]));
+    } else {
+      using hw = typename std::conditional<std::is_same<T, half_t>::value, half_t, __bf16>::type;
+      typedef hw pair __attribute__((ext_vector_type(2)));
+#pragma unroll
+      for (int j = 0; j < N; j += 2) p.u[j / 2] = __builtin_bit_cast(uint32_t, pair{static_cast<hw>(f[j]), static_cast<hw>(f[j + 1])});
+    }
+    return p;
+  }
+  // elements [i, i + G) from another pack; they were zero
+  template <int G>
+  __device__ __forceinline__ void put(int i, const Pack<T, G>& x) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int j = 0; j < G; ++j) u[i + j] = x.u[j];
+    } else if constexpr (G == 1) {
+      u[i / 2] |= x.u[0] << (16 * (i & 1));
+    } else {
+#pragma unroll
+      for (int j = 0; j < G / 2; ++j) u[i / 2 + j] = x.u[j];
+    }
+  }
+  static __device__ __forceinline__ Pack zero() {
+    Pack p;
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) p.u[i] = 0;
+    return p;
+  }
+};
+
+// N elements from an address that is a multiple of the element size only: global memory takes 16-byte accesses at any
+// alignment, so rows of odd width, and views at odd offsets, move as wide as aligned ones.
 template <int BYTES> struct RawVec;
 template <> struct RawVec<16> { typedef uint32_t type __attribute__((ext_vector_type(4))); };
 template <> struct RawVec<8> { typedef uint32_t type __attribute__((ext_vector_type(2))); };
@@ -25,35 +75,44 @@ template <> struct RawVec<2> { typedef uint16_t type; };
 
 template <typename T, int N>
 __device__ __forceinline__ Pack<T, N> load_any(const T* p) {
-  typedef typename RawVec<sizeof(T) * N>::type raw;
-  typedef raw loose __attribute__((aligned(sizeof(T))));
-  return __builtin_bit_cast(Pack<T, N>, static_cast<raw>(*reinterpret_cast<const loose*>(p)));
+  constexpr int bytes = sizeof(T) * N;
+  if constexpr (bytes > 16) {  // fp32 parameters beside 16-bit rows
+    const Pack<T, N / 2> lo = load_any<T, N / 2>(p), hi = load_any<T, N / 2>(p + N / 2);
+    Pack<T, N> x;
+#pragma unroll
+    for (int i = 0; i < Pack<T, N / 2>::kWords; ++i) {
+      x.u[i] = lo.u[i];
+      x.u[Pack<T, N / 2>::kWords + i] = hi.u[i];
+    }
+    return x;
+  } else {
+    typedef typename RawVec<bytes>::type raw;
+    typedef raw loose __attribute__((aligned(sizeof(T))));
+    const raw r = *reinterpret_cast<const loose*>(p);
+    if constexpr (bytes == 2) return Pack<T, N>{{r}};
+    else return __builtin_bit_cast(Pack<T, N>, r);
+  }
 }
 
 template <typename T, int N>
 __device__ __forceinline__ void store_any(T* p, const Pack<T, N>& x) {
-  typedef typename RawVec<sizeof(T) * N>::type raw;
+  constexpr int bytes = sizeof(T) * N;
+  typedef typename RawVec<bytes>::type raw;
   typedef raw loose __attribute__((aligned(sizeof(T))));
-  *reinterpret_cast<loose*>(p) = __builtin_bit_cast(raw, x);
-}
-
-// The same for chunks wider than 16 bytes (a row operator's fp32 weights beside 16-bit rows).
-template <typename T, int N>
-__device__ __forceinline__ Pack<T, N> load_wide(const T* p) {
-  if constexpr (sizeof(T) * N <= 16) {
-    return load_any<T, N>(p);
-  } else {
-    struct Halves { Pack<T, N / 2> lo, hi; } h{load_wide<T, N / 2>(p), load_wide<T, N / 2>(p + N / 2)};
-    return __builtin_bit_cast(Pack<T, N>, h);
-  }
+  if constexpr (bytes == 2) *reinterpret_cast<loose*>(p) = (uint16_t)x.u[0];
+  else *reinterpret_cast<loose*>(p) = __builtin_bit_cast(raw, x);
 }
 
 // Elements [0, n) of a chunk, n < N: the end of a row whose width is no multiple of N. The rest is zero.
 template <typename T, int N>
 __device__ __forceinline__ Pack<T, N> load_part(const T* p, int n) {
-  Pack<T, N> x;
+  Pack<T, N> x = Pack<T, N>::zero();
 #pragma unroll
-  for (int j = 0; j < N; ++j) x.v[j] = j < n ? p[j] : T(0);
+  for (int j = 0; j < N; ++j)
+    if (j < n) {
+      if constexpr (sizeof(T) == 4) x.u[j] = reinterpret_cast<const uint32_t*>(p)[j];
+      else x.u[j / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[j] << (16 * (j & 1));
+    }
   return x;
 }
 
@@ -61,31 +120,60 @@ template <typename T, int N>
 __device__ __forceinline__ void store_part(T* p, const Pack<T, N>& x, int n) {
 #pragma unroll
   for (int j = 0; j < N; ++j)
-    if (j < n) p[j] = x.v[j];
+    if (j < n) {
+      if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t*>(p)[j] = x.u[j];
+      else reinterpret_cast<uint16_t*>(p)[j] = (uint16_t)(x.u[j / 2] >> (16 * (j & 1)));
+    }
 }
 
-// Reductions over the 64 lanes in registers: two quad permutes, two mirrors within 16 lanes, then exchanges of 16 and 32
-// lanes. Every lane ends with the same bits (each step adds the same two numbers on both sides).
+// Reductions over L lanes (an aligned power of two, 8 to 64) in registers: two quad permutes, mirrors within 8 and 16 lanes, then
+// exchanges of 16 and 32 lanes. Every lane ends with the same bits (each step joins the same two values on both sides).
 template <int CTRL>
-__device__ __forceinline__ float dpp_move(float v) {
-  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+__device__ __forceinline__ uint32_t dpp_move(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
 }
-struct OpSum { static __device__ __forceinline__ float of(float a, float b) { return a + b; } };
-struct OpMax { static __device__ __forceinline__ float of(float a, float b) { return fmaxf(a, b); } };
-
-template <typename Op>
-__device__ __forceinline__ float wave_reduce(float v) {
+template <int L, typename Op>
+__device__ __forceinline__ uint32_t lanes_reduce_u32(uint32_t v) {
+  static_assert(L == 8 || L == 16 || L == 32 || L == 64, "lanes");
   v = Op::of(v, dpp_move<0xB1>(v));   // quad_perm 1,0,3,2
   v = Op::of(v, dpp_move<0x4E>(v));   // quad_perm 2,3,0,1
   v = Op::of(v, dpp_move<0x141>(v));  // row_half_mirror
-  v = Op::of(v, dpp_move<0x140>(v));  // row_mirror
-  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = Op::of(__uint_as_float(a[0]), __uint_as_float(a[1]));
-  auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return Op::of(__uint_as_float(b[0]), __uint_as_float(b[1]));
+  if constexpr (L >= 16) v = Op::of(v, dpp_move<0x140>(v));  // row_mirror
+  if constexpr (L >= 32) {
+    auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = Op::of(a[0], a[1]);
+  }
+  if constexpr (L >= 64) {
+    auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    v = Op::of(b[0], b[1]);
+  }
+  return v;
 }
+struct OpSum {
+  static __device__ __forceinline__ uint32_t of(uint32_t a, uint32_t b) {
+    return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+  }
+  static __device__ __forceinline__ float of(float a, float b) { return a + b; }
+};
+struct OpMax {
+  static __device__ __forceinline__ uint32_t of(uint32_t a, uint32_t b) {
+    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+  }
+  static __device__ __forceinline__ float of(float a, float b) { return fmaxf(a, b); }
+};
+struct OpMaxU32 { static __device__ __forceinline__ uint32_t of(uint32_t a, uint32_t b) { return a > b ? a : b; } };
+struct OpOr { static __device__ __forceinline__ uint32_t of(uint32_t a, uint32_t b) { return a | b; } };
 
-// The same over THREADS threads that form a block (or over one wave). `slots`: 16 floats of shared memory that no other
+template <int L, typename Op>
+__device__ __forceinline__ float lanes_reduce(float v) { return __uint_as_float(lanes_reduce_u32<L, Op>(__float_as_uint(v))); }
+template <typename Op>
+__device__ __forceinline__ float wave_reduce(float v) { return lanes_reduce<64, Op>(v); }
+template <int L>
+__device__ __forceinline__ uint32_t lanes_max_u32(uint32_t v) { return lanes_reduce_u32<L, OpMaxU32>(v); }
+template <int L>
+__device__ __forceinline__ uint32_t lanes_or(uint32_t v) { return lanes_reduce_u32<L, OpOr>(v); }
+
+// wave_reduce over THREADS threads that form a block (or over one wave). `slots`: 16 floats of shared memory that no other
 // reduction uses between two barriers of the block.
 template <typename Op, int THREADS>
 __device__ __forceinline__ float row_reduce(float v, float* slots) {

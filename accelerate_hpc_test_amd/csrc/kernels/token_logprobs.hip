@@ -104,7 +104,7 @@ __global__ __launch_bounds__(NT) void token_logprobs_fwd_kernel(
     for (int u = 0; u < UNROLL; ++u) {
       float f[VEC];
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) f[j] = to_f<T>(p[u].v[j]);
+      for (int j = 0; j < VEC; ++j) f[j] = p[u].get(j);
       take(f, c + u * NT);
     }
   }
@@ -113,11 +113,11 @@ __global__ __launch_bounds__(NT) void token_logprobs_fwd_kernel(
     if (c < nfull) {
       const Pack<T, VEC> p = load_any<T, VEC>(x + (long)c * VEC);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) f[j] = to_f<T>(p.v[j]);
+      for (int j = 0; j < VEC; ++j) f[j] = p.get(j);
     } else {
       const Pack<T, VEC> p = load_part<T, VEC>(x + (long)c * VEC, tail);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) f[j] = j < tail ? to_f<T>(p.v[j]) : -INFINITY;
+      for (int j = 0; j < VEC; ++j) f[j] = j < tail ? p.get(j) : -INFINITY;
     }
     take(f, c);
   }
@@ -192,7 +192,7 @@ __global__ __launch_bounds__(NT) void token_logprobs_fwd_kernel(
         const Pack<T, VEC> p = n == VEC ? load_any<T, VEC>(x + (long)cc * VEC) : load_part<T, VEC>(x + (long)cc * VEC, n);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-          const uint64_t k = key_of(to_f<T>(p.v[j]), cc * VEC + j);
+          const uint64_t k = key_of(p.get(j), cc * VEC + j);
           if (j < n && k >= bound) {
             const int at = atomicAdd(&n_list, 1);
             if (at < kList) list[at] = k;
@@ -255,9 +255,7 @@ __global__ __launch_bounds__(kBwdThreads) void token_logprobs_bwd_kernel(
   const int c0 = span * kBwdThreads * kBwdUnroll;
   T* o = out + row * (long)V;
   if (tok == ignore) {
-    Pack<T, VEC> z;
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) z.v[j] = T(0);
+    const Pack<T, VEC> z = Pack<T, VEC>::zero();
     for (int u = 0; u < kBwdUnroll; ++u) {
       const int c = c0 + u * kBwdThreads + tid;
       if (c < nfull) store_any<T, VEC>(o + (long)c * VEC, z);
@@ -289,9 +287,10 @@ __global__ __launch_bounds__(kBwdThreads) void token_logprobs_bwd_kernel(
   for (int u = 0; u < kBwdUnroll; ++u) {
     const int c = c0 + u * kBwdThreads + tid;
     if (c >= chunks) continue;
-    Pack<T, VEC> q;
+    float f[VEC];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) q.v[j] = from_f<T>(value(to_f<T>(p[u].v[j])) * inv_t);
+    for (int j = 0; j < VEC; ++j) f[j] = value(p[u].get(j)) * inv_t;
+    const Pack<T, VEC> q = Pack<T, VEC>::of(f);
     if (c < nfull) store_any<T, VEC>(o + (long)c * VEC, q);
     else store_part<T, VEC>(o + (long)c * VEC, q, tail);
   }

@@ -159,10 +159,12 @@ struct RouteExperts : public torch::autograd::Function<RouteExperts> {
     ctx->save_for_backward({l2, r[0], r[1]});
     ctx->saved_data["form"] = (int64_t)((softmax ? 1 : 0) | (renorm ? 2 : 0));
     ctx->saved_data["scale"] = scale;
+    ctx->set_materialize_grads(false);
     ctx->mark_non_differentiable({r[1]});
     return {r[0], r[1]};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
+    if (!g[0].defined()) return variable_list(8);
     const auto saved = ctx->get_saved_variables();
     const int64_t form = ctx->saved_data["form"].toInt();
     const Tensor d = route_experts_bwd(saved[0], saved[1], saved[2], g[0].contiguous(), form & 1, form & 2,
