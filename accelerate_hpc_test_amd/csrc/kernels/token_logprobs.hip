@@ -1,10 +1,11 @@
 // Log-probabilities of given tokens, the entropy of their distributions and the k best alternatives, over logits [rows, V]
-// (bf16 / fp16 / fp32, all sums in fp32), and the gradient of all three. With z = logits / temperature and one pass that
-// keeps the running maximum m, S = sum e^(x - m) and U = sum (x - m) e^(x - m) of each row:
-//   log p_i = (x_i - m) / T - log S,   H = log S - U / (S T)
+// (bf16 / fp16 / fp32, all sums in fp32), and the gradient of all three. With b the row's largest logit and
+// t_i = (x_i - b) log2(e) / temperature, one pass keeps the running b, S = sum 2^t and U = sum t 2^t of each row:
+//   log p_i = (x_i - b) / temperature - ln S,   H = ln S - ln 2 U / S
 //   dlogits_i = (1/T) [ -p_i (G + dH (log p_i + H)) + sum of the gradients of the outputs that name i ],
 //   G = the sum of the row's log-probability gradients.
-// Bound by memory: the forward reads the logits once, the backward reads them once and writes the gradient once. An -inf
+// Bound by memory: the forward reads the logits once, the backward reads them once and writes the gradient once. A block takes
+// a row; few rows are cut into slices for several blocks, and a second small kernel joins their sums and best keys. An -inf
 // logit has p = 0 and adds nothing. A row whose token is `ignore` is not read: 0, 0, 0 and -1, and a zero gradient. A row
 // without a distribution (NaN, +inf, all -inf) gives NaN and alternatives -1; a token outside [0, V) gives NaN.
 #include <hip/hip_runtime.h>
@@ -18,9 +19,13 @@ using namespace acc;
 
 namespace {
 
-constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
+constexpr float kFar = -1e30f;  // stands for -inf where it is multiplied with a probability of 0
 constexpr int kMaxTop = 64;
 constexpr int kList = 2048;  // candidates of a row kept in shared memory
+constexpr int kMaxParts = 8;  // slices of a row
+constexpr long kBlocks = 512, kSlice = 32768;
+constexpr int kJoinThreads = kMaxParts * kMaxTop;  // a thread for every key of a row's slices
 constexpr int kBwdThreads = 256, kBwdUnroll = 4;
 
 // Keys ordered as (value, then lower index): the larger key is the better alternative. Equal values, -0 and +0 among them,
@@ -39,64 +44,113 @@ __device__ __forceinline__ int key_index(uint64_t k) { return (int)~(uint32_t)k;
 
 __device__ __forceinline__ uint64_t key_max(uint64_t a, uint64_t b) { return a > b ? a : b; }
 
-// e^((x - m) * scale) for scale2 = scale * log2(e)
-__device__ __forceinline__ float exp_scaled(float d, float scale2) { return __builtin_amdgcn_exp2f(d * scale2); }
+__device__ __forceinline__ float exp2_of(float t) { return __builtin_amdgcn_exp2f(t); }
 
+struct Sums { float b, s, u; };  // of a part of a row: its largest logit, sum 2^t and sum t 2^t against it
+
+// `x` as if its sums were against `b`, at least as large
+__device__ __forceinline__ Sums against(Sums x, float b, float scale) {
+  if (x.b > -INFINITY && b < INFINITY) {
+    const float d = fmaxf((x.b - b) * scale, kFar), f = exp2_of(d);
+    x.u = (x.u + d * x.s) * f;
+    x.s *= f;
+  }
+  return x;
+}
+
+struct RowOut {
+  float *lp, *ent, *top_lp, *stats;
+  int64_t* top_id;
+};
+
+// The row's log-probability, entropy and (for the backward) statistics. Returns ln S, NaN for a row without a distribution.
+template <typename T>
+__device__ __forceinline__ float finish_row(const Sums& r, const T* __restrict__ x, int64_t tok, long row, int V, float inv_t,
+                                            const RowOut& out, bool write) {
+  const bool sound = r.s > 0.f && r.s < INFINITY;  // false for NaN too
+  const float ln_s = sound ? logf(r.s) : NAN;
+  if (write) {
+    const bool named = tok >= 0 && tok < V;
+    ACC_CHECK(named, kChkXentLabel);
+    const float ent = ln_s - kLn2 * (r.u / r.s);
+    out.lp[row] = named ? (to_f<T>(x[named ? tok : 0]) - r.b) * inv_t - ln_s : NAN;
+    out.ent[row] = sound ? ent : NAN;
+    if (out.stats != nullptr) {
+      out.stats[row * 3] = r.b;
+      out.stats[row * 3 + 1] = ln_s;
+      out.stats[row * 3 + 2] = ent;
+    }
+  }
+  return ln_s;
+}
+
+__device__ __forceinline__ void put_alternative(const RowOut& out, long at, uint64_t key, float inv_t, float b, float ln_s) {
+  out.top_lp[at] = (key_value(key) - b) * inv_t - ln_s;
+  out.top_id[at] = key_index(key);
+}
+
+template <int NT>
+__device__ __forceinline__ void put_no_row(const RowOut& out, long row, int K, float value) {
+  for (int j = threadIdx.x; j < K; j += NT) {
+    out.top_lp[row * K + j] = value;
+    out.top_id[row * K + j] = -1;
+  }
+}
+
+// blockIdx.x: row * parts + the slice of it. With one slice the block writes the row's outputs, else its sums and its K best
+// keys (falling, 0 where the slice has fewer elements) for token_logprobs_join_kernel.
 template <typename T, int NT, int UNROLL>
-__global__ __launch_bounds__(NT) void token_logprobs_fwd_kernel(
-    const T* __restrict__ logits, long stride, const int64_t* __restrict__ tokens, float* __restrict__ lp_out,
-    float* __restrict__ ent_out, float* __restrict__ top_lp, int64_t* __restrict__ top_id, float* __restrict__ stats, int V, int K,
-    float inv_t, int64_t ignore) {
+__global__ __launch_bounds__(NT) void token_logprobs_fwd_kernel(const T* __restrict__ logits, long stride,
+                                                                const int64_t* __restrict__ tokens, const RowOut out,
+                                                                Sums* __restrict__ part_sums, uint64_t* __restrict__ part_keys,
+                                                                int parts, int V, int K, float inv_t, int64_t ignore) {
   constexpr int VEC = 16 / sizeof(T), GROUPS = NT / 4;
-  __shared__ float slots[4][16];
+  __shared__ float slots[3][16];
   __shared__ uint64_t group_key[GROUPS];
   __shared__ uint64_t list[kList];
   __shared__ uint64_t threshold, round_key[NT / 64];
   __shared__ int n_list, n_threads, threads_list[NT];
-  const long row = blockIdx.x;
-  const int tid = threadIdx.x;
-  const int64_t tok = tokens[row];
-  if (tok == ignore) {  // uniform over the block
-    if (tid == 0) {
-      lp_out[row] = 0.f;
-      ent_out[row] = 0.f;
+  const long row = parts == 1 ? blockIdx.x : blockIdx.x / parts;
+  const int part = parts == 1 ? 0 : blockIdx.x - (int)row * parts, tid = threadIdx.x;
+  int64_t tok = 0;
+  if (parts == 1) {  // slices do not wait for their row's token: the join writes a row that is ignored
+    tok = tokens[row];
+    if (tok == ignore) {  // uniform over the block
+      if (tid == 0) out.lp[row] = out.ent[row] = 0.f;
+      put_no_row<NT>(out, row, K, 0.f);
+      return;
     }
-    for (int j = tid; j < K; j += NT) {
-      top_lp[row * K + j] = 0.f;
-      top_id[row * K + j] = -1;
-    }
-    return;
   }
   const T* x = logits + row * stride;
+  const float scale = inv_t * kLog2e;
   const int nfull = V / VEC, tail = V % VEC, chunks = nfull + (tail > 0);
-  const float scale2 = inv_t * kLog2e;
+  const int span = (chunks + parts - 1) / parts, c_lo = min(part * span, chunks), c_hi = min(c_lo + span, chunks);
+  const int c_full = min(c_hi, nfull);
 
-  // one pass: running maximum, sum and weighted sum per thread, and the chunk that holds the thread's maximum
-  float m = -INFINITY, sum = 0.f, wsum = 0.f;
-  int best = -1;
-  auto take = [&](const float (&f)[VEC], int c) {
+  // one pass: running sums per thread, and the chunk that holds the thread's maximum
+  Sums r{-INFINITY, 0.f, 0.f};
+  int best = c_lo + tid;  // nothing above -inf: the first chunk stands for the thread
+  Pack<T, VEC> best_chunk;
+  auto take = [&](const float (&f)[VEC], const Pack<T, VEC>& p, int c) {
     float hi = f[0];
 #pragma unroll
     for (int j = 1; j < VEC; ++j) hi = fmaxf(hi, f[j]);
-    if (hi > m) {
-      if (m > -INFINITY) {
-        const float a = exp_scaled(m - hi, scale2);
-        wsum = (wsum + fmaxf(m - hi, -1e30f) * sum) * a;
-        sum *= a;
-      }
-      m = hi;
+    if (hi > r.b) {
+      r = against(r, hi, scale);
+      r.b = hi;
       best = c;
+      best_chunk = p;
     }
-    const float base = m > -INFINITY ? m : 0.f;
+    const float b = r.b > -INFINITY ? r.b : 0.f;
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
-      const float d = f[j] - base, e = exp_scaled(d, scale2);
-      sum += e;
-      wsum = fmaf(fmaxf(d, -1e30f), e, wsum);  // -inf: a finite distance times zero
+      const float t = (f[j] - b) * scale, e = exp2_of(t);
+      r.s += e;
+      r.u = fmaf(fmaxf(t, kFar), e, r.u);
     }
   };
-  int c = tid;
-  for (; c + (UNROLL - 1) * NT < nfull; c += UNROLL * NT) {
+  int c = c_lo + tid;
+  for (; c + (UNROLL - 1) * NT < c_full; c += UNROLL * NT) {
     Pack<T, VEC> p[UNROLL];
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) p[u] = load_any<T, VEC>(x + (long)(c + u * NT) * VEC);
@@ -105,62 +159,57 @@ __global__ __launch_bounds__(NT) void token_logprobs_fwd_kernel(
       float f[VEC];
 #pragma unroll
       for (int j = 0; j < VEC; ++j) f[j] = p[u].get(j);
-      take(f, c + u * NT);
+      take(f, p[u], c + u * NT);
     }
   }
-  for (; c < chunks; c += NT) {
+  for (; c < c_hi; c += NT) {
+    const int n = c < nfull ? VEC : tail;
+    const Pack<T, VEC> p = n == VEC ? load_any<T, VEC>(x + (long)c * VEC) : load_part<T, VEC>(x + (long)c * VEC, n);
     float f[VEC];
-    if (c < nfull) {
-      const Pack<T, VEC> p = load_any<T, VEC>(x + (long)c * VEC);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) f[j] = p.get(j);
-    } else {
-      const Pack<T, VEC> p = load_part<T, VEC>(x + (long)c * VEC, tail);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) f[j] = j < tail ? p.get(j) : -INFINITY;
+    for (int j = 0; j < VEC; ++j) f[j] = j < n ? p.get(j) : -INFINITY;
+    take(f, p, c);
+  }
+  const float m = r.b, b = row_reduce<OpMax, NT>(m, slots[0]);
+  r = against(r, b, scale);
+  r.b = b;
+  r.s = row_reduce<OpSum, NT>(r.s, slots[1]);
+  r.u = row_reduce<OpSum, NT>(r.u, slots[2]);
+  float ln_s = 0.f;
+  uint64_t* keys_out = nullptr;
+  if (parts == 1) {
+    ln_s = finish_row<T>(r, x, tok, row, V, inv_t, out, tid == 0);
+    if (K == 0) return;
+    if (ln_s != ln_s) {
+      put_no_row<NT>(out, row, K, NAN);
+      return;
     }
-    take(f, c);
-  }
-  const float gm = row_reduce<OpMax, NT>(m, slots[0]);
-  if (m > -INFINITY && gm < INFINITY) {
-    const float a = exp_scaled(m - gm, scale2);
-    wsum = (wsum + fmaxf(m - gm, -1e30f) * sum) * a;
-    sum *= a;
-  }
-  const float S = row_reduce<OpSum, NT>(sum, slots[1]), U = row_reduce<OpSum, NT>(wsum, slots[2]);
-  const bool sound = S > 0.f && S < INFINITY;  // false for NaN too
-  const float log_s = sound ? logf(S) : NAN;
-  const float ent = sound ? log_s - inv_t * (U / S) : NAN;
-  if (tid == 0) {
-    const bool named = tok >= 0 && tok < V;
-    ACC_CHECK(named, kChkXentLabel);
-    lp_out[row] = named && sound ? (to_f<T>(x[named ? tok : 0]) - gm) * inv_t - log_s : NAN;
-    ent_out[row] = ent;
-    if (stats != nullptr) {
-      stats[row * 3] = gm;
-      stats[row * 3 + 1] = log_s;
-      stats[row * 3 + 2] = ent;
+  } else {
+    if (tid == 0) part_sums[blockIdx.x] = r;
+    if (K == 0) return;
+    keys_out = part_keys + (long)blockIdx.x * K;
+    if (r.s != r.s || c_lo >= c_hi) {  // the row has no distribution, or this slice no elements
+      for (int j = tid; j < K; j += NT) keys_out[j] = 0;
+      return;
     }
   }
-  if (K == 0) return;
-  if (!sound) {
-    for (int j = tid; j < K; j += NT) {
-      top_lp[row * K + j] = NAN;
-      top_id[row * K + j] = -1;
-    }
-    return;
-  }
+  auto put = [&](int rank, uint64_t key) {
+    if (keys_out != nullptr) keys_out[rank] = key;
+    else put_alternative(out, row * K + rank, key, inv_t, r.b, ln_s);
+  };
 
   // The K best alternatives. Each group of four threads has its best key; the K-th best of those is a bound that K elements
   // at least reach and few exceed. The threads whose own best reaches it read their chunks again (a few of them, from the
   // cache) and list every element that does; the list is ranked by counting.
   uint64_t mine = 0;
-  if (tid < chunks) {
-    if (best < 0) best = tid;  // nothing above -inf: the first element stands for the thread
+  if (c_lo + tid < c_hi) {
     const int n = best < nfull ? VEC : tail;
-    for (int j = n - 1; j >= 0; --j) {
-      const float f = to_f<T>(x[(long)best * VEC + j]);
-      if (f == m) mine = key_of(f, best * VEC + j);
+    if (m == -INFINITY) {
+      mine = key_of(m, best * VEC);  // NaN apart, which no sound row has, the first chunk holds nothing else
+    } else {
+#pragma unroll
+      for (int j = VEC - 1; j >= 0; --j)
+        if (j < n && best_chunk.get(j) == m) mine = key_of(m, best * VEC + j);
     }
   }
   uint64_t g = mine;
@@ -187,7 +236,7 @@ __global__ __launch_bounds__(NT) void token_logprobs_fwd_kernel(
   {
     const int lane = tid & 63, waves = NT / 64, nt = n_threads;
     for (int i = tid >> 6; i < nt; i += waves) {
-      for (int cc = threads_list[i] + lane * NT; cc < chunks; cc += 64 * NT) {
+      for (int cc = c_lo + threads_list[i] + lane * NT; cc < c_hi; cc += 64 * NT) {
         const int n = cc < nfull ? VEC : tail;
         const Pack<T, VEC> p = n == VEC ? load_any<T, VEC>(x + (long)cc * VEC) : load_part<T, VEC>(x + (long)cc * VEC, n);
 #pragma unroll
@@ -207,20 +256,19 @@ __global__ __launch_bounds__(NT) void token_logprobs_fwd_kernel(
     for (int i = tid; i < n; i += NT) {
       const uint64_t k = list[i];
       int rank = 0;
+#pragma unroll 8
       for (int q = 0; q < n; ++q) rank += list[q] > k;
-      if (rank < K) {
-        top_lp[row * K + rank] = (key_value(k) - gm) * inv_t - log_s;
-        top_id[row * K + rank] = key_index(k);
-      }
+      if (rank < K) put(rank, k);
     }
+    for (int j = n + tid; j < K; j += NT) keys_out[j] = 0;  // a slice with fewer elements; a row has K at least
     return;
   }
   // More elements of a few threads than the list holds reach the bound (a row whose largest values all lie one thread's
-  // stride apart): the best one below the last, K times over the row.
+  // stride apart): the best one below the last, K times over the slice.
   uint64_t last = ~0ull;
-  for (int r = 0; r < K; ++r) {
+  for (int rank = 0; rank < K; ++rank) {
     uint64_t k = 0;
-    for (int cc = tid; cc < chunks; cc += NT) {
+    for (int cc = c_lo + tid; cc < c_hi; cc += NT) {
       const int nn = cc < nfull ? VEC : tail;
       for (int j = 0; j < nn; ++j) {
         const uint64_t q = key_of(to_f<T>(x[(long)cc * VEC + j]), cc * VEC + j);
@@ -233,10 +281,48 @@ __global__ __launch_bounds__(NT) void token_logprobs_fwd_kernel(
     __syncthreads();
     for (int i = 0; i < NT / 64; ++i) k = key_max(k, round_key[i]);
     last = k;
-    if (tid == 0) {
-      top_lp[row * K + r] = (key_value(k) - gm) * inv_t - log_s;
-      top_id[row * K + r] = key_index(k);
-    }
+    if (tid == 0) put(rank, k);
+  }
+}
+
+// A block per row: the sums of its slices and the K best of their keys, ranked by counting.
+template <typename T>
+__global__ __launch_bounds__(kJoinThreads) void token_logprobs_join_kernel(const T* __restrict__ logits, long stride,
+                                                                  const int64_t* __restrict__ tokens, const RowOut out,
+                                                                  const Sums* __restrict__ part_sums,
+                                                                  const uint64_t* __restrict__ part_keys, int parts, int V, int K,
+                                                                  float inv_t, int64_t ignore) {
+  __shared__ uint64_t keys[kJoinThreads];
+  const long row = blockIdx.x;
+  const int tid = threadIdx.x, n = parts * K;
+  const float scale = inv_t * kLog2e;
+  const int64_t tok = tokens[row];
+  if (tok == ignore) {
+    if (tid == 0) out.lp[row] = out.ent[row] = 0.f;
+    put_no_row<kJoinThreads>(out, row, K, 0.f);
+    return;
+  }
+  if (tid < n) keys[tid] = part_keys[row * n + tid];
+  // 8 lanes hold the slices' sums, every 8 lanes the same
+  static_assert(kMaxParts == 8, "a slice per lane");
+  Sums r{-INFINITY, 0.f, 0.f};
+  if ((tid & 7) < parts) r = part_sums[row * parts + (tid & 7)];
+  const float b = lanes_reduce<8, OpMax>(r.b);
+  r = against(r, b, scale);
+  r = Sums{b, lanes_reduce<8, OpSum>(r.s), lanes_reduce<8, OpSum>(r.u)};
+  const float ln_s = finish_row<T>(r, logits + row * stride, tok, row, V, inv_t, out, tid == 0);
+  if (K == 0) return;
+  if (ln_s != ln_s) {
+    put_no_row<kJoinThreads>(out, row, K, NAN);
+    return;
+  }
+  __syncthreads();
+  if (tid < n) {
+    const uint64_t k = keys[tid];
+    int rank = 0;
+#pragma unroll 8
+    for (int q = 0; q < n; ++q) rank += keys[q] > k;
+    if (k != 0 && rank < K) put_alternative(out, row * K + rank, k, inv_t, r.b, ln_s);
   }
 }
 
@@ -271,7 +357,7 @@ __global__ __launch_bounds__(kBwdThreads) void token_logprobs_bwd_kernel(
     if (c < nfull) p[u] = load_any<T, VEC>(x + (long)c * VEC);
     else if (c < chunks) p[u] = load_part<T, VEC>(x + (long)c * VEC, tail);
   }
-  const float gm = stats[row * 3], log_s = stats[row * 3 + 1], ent = stats[row * 3 + 2];
+  const float b = stats[row * 3], ln_s = stats[row * 3 + 1], ent = stats[row * 3 + 2];
   const float gl = g_lp != nullptr ? g_lp[row * g_lp_stride] : 0.f, gh = g_ent != nullptr ? g_ent[row * g_ent_stride] : 0.f;
   float total = gl;
   if (g_top != nullptr)
@@ -279,8 +365,7 @@ __global__ __launch_bounds__(kBwdThreads) void token_logprobs_bwd_kernel(
   // a token outside [0, V) had no log-probability: the row's gradient is NaN with it
   if (tok < 0 || tok >= V) total = NAN;
   auto value = [&](float f) {
-    const float lp = fmaxf((f - gm) * inv_t, -1e30f) - log_s;
-    const float prob = exp_scaled(f - gm, inv_t * kLog2e) * __builtin_amdgcn_exp2f(-log_s * kLog2e);
+    const float lp = fmaxf((f - b) * inv_t, kFar) - ln_s, prob = exp2_of(((f - b) * inv_t - ln_s) * kLog2e);
     return -prob * (total + gh * (lp + ent));
   };
 #pragma unroll
@@ -335,20 +420,36 @@ std::vector<torch::Tensor> token_logprobs_fwd(torch::Tensor logits, torch::Tenso
   const c10::DeviceGuard guard(logits.device());
   const auto fopt = logits.options().dtype(torch::kFloat32);
   auto lp = torch::empty({rows}, fopt), ent = torch::empty({rows}, fopt);
-  torch::Tensor top_lp, top_id, stats;
+  torch::Tensor top_lp, top_id, stats, sums, keys;
   if (K > 0) {
     top_lp = torch::empty({rows, K}, fopt);
     top_id = torch::empty({rows, K}, fopt.dtype(torch::kInt64));
   }
   if (want_stats) stats = torch::empty({rows, 3}, fopt);
   if (rows > 0) {
+    // Few rows leave most of the chip idle: slices of at least kSlice bytes, as many as give kBlocks blocks.
+    const long bytes = V * logits.element_size();
+    const int parts = (int)std::max(1L, std::min({(long)kMaxParts, kBlocks / rows, bytes / kSlice}));
+    TORCH_CHECK(rows * parts < (1L << 31), "token_logprobs: too many rows in one call");
+    if (parts > 1) {
+      sums = torch::empty({rows * parts, 3}, fopt);
+      if (K > 0) keys = torch::empty({rows * parts, K}, fopt.dtype(torch::kInt64));
+    }
+    const RowOut out{lp.data_ptr<float>(), ent.data_ptr<float>(), K > 0 ? top_lp.data_ptr<float>() : nullptr,
+                     want_stats ? stats.data_ptr<float>() : nullptr, K > 0 ? top_id.data_ptr<int64_t>() : nullptr};
+    Sums* sp = parts > 1 ? reinterpret_cast<Sums*>(sums.data_ptr<float>()) : nullptr;
+    uint64_t* kp = keys.defined() ? reinterpret_cast<uint64_t*>(keys.data_ptr<int64_t>()) : nullptr;
     auto stream = at::hip::getCurrentHIPStream();
     ACC_FOR_FLOAT_TYPES(logits.scalar_type(), "token_logprobs", {
-      hipLaunchKernelGGL((token_logprobs_fwd_kernel<scalar, 512, 4>), dim3((unsigned)rows), dim3(512), 0, stream,
-                         reinterpret_cast<const scalar*>(logits.data_ptr()), logits.stride(0), tokens.data_ptr<int64_t>(),
-                         lp.data_ptr<float>(), ent.data_ptr<float>(), K > 0 ? top_lp.data_ptr<float>() : nullptr,
-                         K > 0 ? top_id.data_ptr<int64_t>() : nullptr, want_stats ? stats.data_ptr<float>() : nullptr, (int)V,
-                         (int)K, (float)inv_t, ignore);
+      const scalar* x = reinterpret_cast<const scalar*>(logits.data_ptr());
+      // slices: twice the threads for the shortest way through one
+      const int nt = parts > 1 ? 512 : 256;
+      auto kernel = parts > 1 ? token_logprobs_fwd_kernel<scalar, 512, 4> : token_logprobs_fwd_kernel<scalar, 256, 4>;
+      hipLaunchKernelGGL(kernel, dim3((unsigned)(rows * parts)), dim3(nt), 0, stream, x,
+                         logits.stride(0), tokens.data_ptr<int64_t>(), out, sp, kp, parts, (int)V, (int)K, (float)inv_t, ignore);
+      if (parts > 1)
+        hipLaunchKernelGGL((token_logprobs_join_kernel<scalar>), dim3((unsigned)rows), dim3(kJoinThreads), 0, stream, x, logits.stride(0),
+                           tokens.data_ptr<int64_t>(), out, sp, kp, parts, (int)V, (int)K, (float)inv_t, ignore);
     });
   }
   return {lp, ent, top_lp, top_id, stats};
