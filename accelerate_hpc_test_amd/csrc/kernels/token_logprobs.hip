@@ -19,7 +19,7 @@ using namespace acc;
 
 namespace {
 
-constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
+constexpr float kLn2 = 0.693147180559945309417f;
 constexpr float kFar = -1e30f;  // stands for -inf where it is multiplied with a probability of 0
 constexpr int kMaxTop = 64;
 constexpr int kList = 2048;  // candidates of a row kept in shared memory
@@ -58,34 +58,38 @@ __device__ __forceinline__ Sums against(Sums x, float b, float scale) {
   return x;
 }
 
+// 1 / temperature; `scale` is it times log2(e) rounded to 32 bits, `slack` the relative error of that. All exponents of a row
+// are off by the same share, so S is off by slack ln 2 U to first order, and corrected by it.
+struct Temper {
+  double inv_t;
+  float scale, slack;
+};
+
 struct RowOut {
   float *lp, *ent, *top_lp, *stats;
   int64_t* top_id;
 };
 
-// The row's log-probability, entropy and (for the backward) statistics. Returns ln S, NaN for a row without a distribution.
+// The row's log-probability, entropy and, for the backward, b, 1 / S, ln S and the entropy. Returns ln S, NaN for a row without
+// a distribution.
 template <typename T>
-__device__ __forceinline__ float finish_row(const Sums& r, const T* __restrict__ x, int64_t tok, long row, int V, float inv_t,
+__device__ __forceinline__ float finish_row(const Sums& r, const T* __restrict__ x, int64_t tok, long row, int V, const Temper& w,
                                             const RowOut& out, bool write) {
   const bool sound = r.s > 0.f && r.s < INFINITY;  // false for NaN too
-  const float ln_s = sound ? logf(r.s) : NAN;
+  const float sum = sound ? fmaf(w.slack * kLn2, r.u, r.s) : NAN, ln_s = logf(sum);
   if (write) {
     const bool named = tok >= 0 && tok < V;
     ACC_CHECK(named, kChkXentLabel);
-    const float ent = ln_s - kLn2 * (r.u / r.s);
-    out.lp[row] = named ? (to_f<T>(x[named ? tok : 0]) - r.b) * inv_t - ln_s : NAN;
-    out.ent[row] = sound ? ent : NAN;
-    if (out.stats != nullptr) {
-      out.stats[row * 3] = r.b;
-      out.stats[row * 3 + 1] = ln_s;
-      out.stats[row * 3 + 2] = ent;
-    }
+    const float ent = sound ? logf(r.s) - kLn2 * (r.u / r.s) : NAN;
+    out.lp[row] = named ? (float)((double)(to_f<T>(x[named ? tok : 0]) - r.b) * w.inv_t) - ln_s : NAN;
+    out.ent[row] = ent;
+    if (out.stats != nullptr) *reinterpret_cast<float4*>(out.stats + row * 4) = make_float4(r.b, 1.f / sum, ln_s, ent);
   }
   return ln_s;
 }
 
-__device__ __forceinline__ void put_alternative(const RowOut& out, long at, uint64_t key, float inv_t, float b, float ln_s) {
-  out.top_lp[at] = (key_value(key) - b) * inv_t - ln_s;
+__device__ __forceinline__ void put_alternative(const RowOut& out, long at, uint64_t key, const Temper& w, float b, float ln_s) {
+  out.top_lp[at] = (float)((double)(key_value(key) - b) * w.inv_t) - ln_s;
   out.top_id[at] = key_index(key);
 }
 
@@ -103,7 +107,7 @@ template <typename T, int NT, int UNROLL>
 __global__ __launch_bounds__(NT) void token_logprobs_fwd_kernel(const T* __restrict__ logits, long stride,
                                                                 const int64_t* __restrict__ tokens, const RowOut out,
                                                                 Sums* __restrict__ part_sums, uint64_t* __restrict__ part_keys,
-                                                                int parts, int V, int K, float inv_t, int64_t ignore) {
+                                                                int parts, int V, int K, const Temper w, int64_t ignore) {
   constexpr int VEC = 16 / sizeof(T), GROUPS = NT / 4;
   __shared__ float slots[3][16];
   __shared__ uint64_t group_key[GROUPS];
@@ -122,7 +126,7 @@ __global__ __launch_bounds__(NT) void token_logprobs_fwd_kernel(const T* __restr
     }
   }
   const T* x = logits + row * stride;
-  const float scale = inv_t * kLog2e;
+  const float scale = w.scale;
   const int nfull = V / VEC, tail = V % VEC, chunks = nfull + (tail > 0);
   const int span = (chunks + parts - 1) / parts, c_lo = min(part * span, chunks), c_hi = min(c_lo + span, chunks);
   const int c_full = min(c_hi, nfull);
@@ -178,7 +182,7 @@ __global__ __launch_bounds__(NT) void token_logprobs_fwd_kernel(const T* __restr
   float ln_s = 0.f;
   uint64_t* keys_out = nullptr;
   if (parts == 1) {
-    ln_s = finish_row<T>(r, x, tok, row, V, inv_t, out, tid == 0);
+    ln_s = finish_row<T>(r, x, tok, row, V, w, out, tid == 0);
     if (K == 0) return;
     if (ln_s != ln_s) {
       put_no_row<NT>(out, row, K, NAN);
@@ -195,7 +199,7 @@ __global__ __launch_bounds__(NT) void token_logprobs_fwd_kernel(const T* __restr
   }
   auto put = [&](int rank, uint64_t key) {
     if (keys_out != nullptr) keys_out[rank] = key;
-    else put_alternative(out, row * K + rank, key, inv_t, r.b, ln_s);
+    else put_alternative(out, row * K + rank, key, w, r.b, ln_s);
   };
 
   // The K best alternatives. Each group of four threads has its best key; the K-th best of those is a bound that K elements
@@ -291,11 +295,10 @@ __global__ __launch_bounds__(kJoinThreads) void token_logprobs_join_kernel(const
                                                                   const int64_t* __restrict__ tokens, const RowOut out,
                                                                   const Sums* __restrict__ part_sums,
                                                                   const uint64_t* __restrict__ part_keys, int parts, int V, int K,
-                                                                  float inv_t, int64_t ignore) {
+                                                                  const Temper w, int64_t ignore) {
   __shared__ uint64_t keys[kJoinThreads];
   const long row = blockIdx.x;
   const int tid = threadIdx.x, n = parts * K;
-  const float scale = inv_t * kLog2e;
   const int64_t tok = tokens[row];
   if (tok == ignore) {
     if (tid == 0) out.lp[row] = out.ent[row] = 0.f;
@@ -308,9 +311,9 @@ __global__ __launch_bounds__(kJoinThreads) void token_logprobs_join_kernel(const
   Sums r{-INFINITY, 0.f, 0.f};
   if ((tid & 7) < parts) r = part_sums[row * parts + (tid & 7)];
   const float b = lanes_reduce<8, OpMax>(r.b);
-  r = against(r, b, scale);
+  r = against(r, b, w.scale);
   r = Sums{b, lanes_reduce<8, OpSum>(r.s), lanes_reduce<8, OpSum>(r.u)};
-  const float ln_s = finish_row<T>(r, logits + row * stride, tok, row, V, inv_t, out, tid == 0);
+  const float ln_s = finish_row<T>(r, logits + row * stride, tok, row, V, w, out, tid == 0);
   if (K == 0) return;
   if (ln_s != ln_s) {
     put_no_row<kJoinThreads>(out, row, K, NAN);
@@ -322,7 +325,7 @@ __global__ __launch_bounds__(kJoinThreads) void token_logprobs_join_kernel(const
     int rank = 0;
 #pragma unroll 8
     for (int q = 0; q < n; ++q) rank += keys[q] > k;
-    if (k != 0 && rank < K) put_alternative(out, row * K + rank, k, inv_t, r.b, ln_s);
+    if (k != 0 && rank < K) put_alternative(out, row * K + rank, k, w, r.b, ln_s);
   }
 }
 
@@ -331,8 +334,7 @@ template <typename T>
 __global__ __launch_bounds__(kBwdThreads) void token_logprobs_bwd_kernel(
     const T* __restrict__ logits, long stride, const int64_t* __restrict__ tokens, const float* __restrict__ stats,
     const int64_t* __restrict__ top_id, const float* __restrict__ g_lp, long g_lp_stride, const float* __restrict__ g_ent,
-    long g_ent_stride, const float* __restrict__ g_top, T* __restrict__ out, long rows, int V, int K, float inv_t, int64_t ignore,
-    int spans) {
+    long g_ent_stride, const float* __restrict__ g_top, T* __restrict__ out, int V, int K, const Temper w, int64_t ignore, int spans) {
   constexpr int VEC = 16 / sizeof(T);
   const long row = blockIdx.x / spans;
   const int span = (int)(blockIdx.x - row * spans), tid = threadIdx.x;
@@ -357,16 +359,18 @@ __global__ __launch_bounds__(kBwdThreads) void token_logprobs_bwd_kernel(
     if (c < nfull) p[u] = load_any<T, VEC>(x + (long)c * VEC);
     else if (c < chunks) p[u] = load_part<T, VEC>(x + (long)c * VEC, tail);
   }
-  const float b = stats[row * 3], ln_s = stats[row * 3 + 1], ent = stats[row * 3 + 2];
+  const float4 st = *reinterpret_cast<const float4*>(stats + row * 4);  // b, 1 / S, ln S, entropy
   const float gl = g_lp != nullptr ? g_lp[row * g_lp_stride] : 0.f, gh = g_ent != nullptr ? g_ent[row * g_ent_stride] : 0.f;
   float total = gl;
   if (g_top != nullptr)
     for (int j = 0; j < K; ++j) total += g_top[row * K + j];
   // a token outside [0, V) had no log-probability: the row's gradient is NaN with it
   if (tok < 0 || tok >= V) total = NAN;
+  // -p (G + dH (log p + H)) / T = 2^t (c + d t)
+  const float inv_t = (float)w.inv_t, share = -st.y * inv_t, cc = share * (total + gh * (st.w - st.z)), dd = share * gh * kLn2;
   auto value = [&](float f) {
-    const float lp = fmaxf((f - b) * inv_t, kFar) - ln_s, prob = exp2_of(((f - b) * inv_t - ln_s) * kLog2e);
-    return -prob * (total + gh * (lp + ent));
+    const float t = (f - st.x) * w.scale;
+    return exp2_of(t) * fmaf(dd, fmaxf(t, kFar), cc);
   };
 #pragma unroll
   for (int u = 0; u < kBwdUnroll; ++u) {
@@ -374,7 +378,7 @@ __global__ __launch_bounds__(kBwdThreads) void token_logprobs_bwd_kernel(
     if (c >= chunks) continue;
     float f[VEC];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) f[j] = value(p[u].get(j)) * inv_t;
+    for (int j = 0; j < VEC; ++j) f[j] = value(p[u].get(j));
     const Pack<T, VEC> q = Pack<T, VEC>::of(f);
     if (c < nfull) store_any<T, VEC>(o + (long)c * VEC, q);
     else store_part<T, VEC>(o + (long)c * VEC, q, tail);
@@ -394,7 +398,13 @@ __global__ __launch_bounds__(kBwdThreads) void token_logprobs_bwd_kernel(
       if (top_id[row * K + j] == tok) return;  // that alternative's thread writes it
     extra = gl;
   }
-  o[id] = from_f<T>((value(to_f<T>(x[id])) + extra) * inv_t);
+  o[id] = from_f<T>(fmaf(extra, inv_t, value(to_f<T>(x[id]))));
+}
+
+Temper temper_of(double inv_t) {
+  const double scale = inv_t * 1.4426950408889634074;
+  const float rounded = (float)scale;
+  return Temper{inv_t, rounded, (float)((scale - rounded) / rounded)};
 }
 
 void check_logits(const torch::Tensor& logits, const torch::Tensor& tokens) {
@@ -411,7 +421,7 @@ void check_logits(const torch::Tensor& logits, const torch::Tensor& tokens) {
 
 ACC_DEBUG_TAKE_FN(acc_dbg_take_token_logprobs)
 
-// logprobs [rows], entropy [rows], top log-probabilities and tokens [rows, K] (K > 0), stats [rows, 3] (`want_stats`).
+// logprobs [rows], entropy [rows], top log-probabilities and tokens [rows, K] (K > 0), stats [rows, 4] (`want_stats`).
 std::vector<torch::Tensor> token_logprobs_fwd(torch::Tensor logits, torch::Tensor tokens, int64_t K, double inv_t, int64_t ignore,
                                               bool want_stats) {
   check_logits(logits, tokens);
@@ -420,25 +430,22 @@ std::vector<torch::Tensor> token_logprobs_fwd(torch::Tensor logits, torch::Tenso
   const c10::DeviceGuard guard(logits.device());
   const auto fopt = logits.options().dtype(torch::kFloat32);
   auto lp = torch::empty({rows}, fopt), ent = torch::empty({rows}, fopt);
-  torch::Tensor top_lp, top_id, stats, sums, keys;
+  torch::Tensor top_lp, top_id, stats, work;
   if (K > 0) {
     top_lp = torch::empty({rows, K}, fopt);
     top_id = torch::empty({rows, K}, fopt.dtype(torch::kInt64));
   }
-  if (want_stats) stats = torch::empty({rows, 3}, fopt);
+  if (want_stats) stats = torch::empty({rows, 4}, fopt);
   if (rows > 0) {
     // Few rows leave most of the chip idle: slices of at least kSlice bytes, as many as give kBlocks blocks.
     const long bytes = V * logits.element_size();
     const int parts = (int)std::max(1L, std::min({(long)kMaxParts, kBlocks / rows, bytes / kSlice}));
     TORCH_CHECK(rows * parts < (1L << 31), "token_logprobs: too many rows in one call");
-    if (parts > 1) {
-      sums = torch::empty({rows * parts, 3}, fopt);
-      if (K > 0) keys = torch::empty({rows * parts, K}, fopt.dtype(torch::kInt64));
-    }
+    if (parts > 1) work = torch::empty({rows * parts * (K * 8 + (long)sizeof(Sums))}, fopt.dtype(torch::kUInt8));
     const RowOut out{lp.data_ptr<float>(), ent.data_ptr<float>(), K > 0 ? top_lp.data_ptr<float>() : nullptr,
                      want_stats ? stats.data_ptr<float>() : nullptr, K > 0 ? top_id.data_ptr<int64_t>() : nullptr};
-    Sums* sp = parts > 1 ? reinterpret_cast<Sums*>(sums.data_ptr<float>()) : nullptr;
-    uint64_t* kp = keys.defined() ? reinterpret_cast<uint64_t*>(keys.data_ptr<int64_t>()) : nullptr;
+    uint64_t* kp = parts > 1 ? reinterpret_cast<uint64_t*>(work.data_ptr()) : nullptr;
+    Sums* sp = parts > 1 ? reinterpret_cast<Sums*>(kp + rows * parts * K) : nullptr;
     auto stream = at::hip::getCurrentHIPStream();
     ACC_FOR_FLOAT_TYPES(logits.scalar_type(), "token_logprobs", {
       const scalar* x = reinterpret_cast<const scalar*>(logits.data_ptr());
@@ -446,10 +453,10 @@ std::vector<torch::Tensor> token_logprobs_fwd(torch::Tensor logits, torch::Tenso
       const int nt = parts > 1 ? 512 : 256;
       auto kernel = parts > 1 ? token_logprobs_fwd_kernel<scalar, 512, 4> : token_logprobs_fwd_kernel<scalar, 256, 4>;
       hipLaunchKernelGGL(kernel, dim3((unsigned)(rows * parts)), dim3(nt), 0, stream, x,
-                         logits.stride(0), tokens.data_ptr<int64_t>(), out, sp, kp, parts, (int)V, (int)K, (float)inv_t, ignore);
+                         logits.stride(0), tokens.data_ptr<int64_t>(), out, sp, kp, parts, (int)V, (int)K, temper_of(inv_t), ignore);
       if (parts > 1)
         hipLaunchKernelGGL((token_logprobs_join_kernel<scalar>), dim3((unsigned)rows), dim3(kJoinThreads), 0, stream, x, logits.stride(0),
-                           tokens.data_ptr<int64_t>(), out, sp, kp, parts, (int)V, (int)K, (float)inv_t, ignore);
+                           tokens.data_ptr<int64_t>(), out, sp, kp, parts, (int)V, (int)K, temper_of(inv_t), ignore);
     });
   }
   return {lp, ent, top_lp, top_id, stats};
@@ -462,7 +469,7 @@ torch::Tensor token_logprobs_bwd(torch::Tensor logits, torch::Tensor tokens, tor
   check_logits(logits, tokens);
   const long rows = logits.size(0), V = logits.size(1);
   const c10::DeviceGuard guard(logits.device());
-  TORCH_CHECK(stats.scalar_type() == at::kFloat && stats.is_contiguous() && stats.numel() == rows * 3, "token_logprobs: stats");
+  TORCH_CHECK(stats.scalar_type() == at::kFloat && stats.is_contiguous() && stats.numel() == rows * 4, "token_logprobs: stats");
   for (const auto& g : {g_lp, g_ent})
     TORCH_CHECK(!g.has_value() || (g->scalar_type() == at::kFloat && g->dim() == 1 && g->size(0) == rows && g->device() == logits.device()),
                 "token_logprobs: gradients must be fp32 [rows]");
@@ -486,8 +493,8 @@ torch::Tensor token_logprobs_bwd(torch::Tensor logits, torch::Tensor tokens, tor
                        stats.data_ptr<float>(), K > 0 ? top_id->data_ptr<int64_t>() : nullptr,
                        g_lp.has_value() ? g_lp->data_ptr<float>() : nullptr, g_lp.has_value() ? g_lp->stride(0) : 0,
                        g_ent.has_value() ? g_ent->data_ptr<float>() : nullptr, g_ent.has_value() ? g_ent->stride(0) : 0,
-                       K > 0 ? g_top->data_ptr<float>() : nullptr, reinterpret_cast<scalar*>(out.data_ptr()), rows, (int)V, (int)K,
-                       (float)inv_t, ignore, (int)spans);
+                       K > 0 ? g_top->data_ptr<float>() : nullptr, reinterpret_cast<scalar*>(out.data_ptr()), (int)V, (int)K,
+                       temper_of(inv_t), ignore, (int)spans);
   });
   return out;
 }
