@@ -321,9 +321,10 @@ __global__ void rope_kernel(const bf16_t* __restrict__ src, bf16_t* __restrict__
     const vec b = reinterpret_cast<const vec*>(src + off + half)[c];
     vec oa = a, ob = b;
     if (h < n_rot_heads) {
-      const long p = pos != nullptr ? pos[t] : (t % S);
-      ACC_CHECK(p >= 0 && p < S, kChkRopePos);  // debug build: a position past the cos / sin table
-      if (ACC_DEBUG_BUILD && (p < 0 || p >= S)) continue;
+      const long at = pos != nullptr ? pos[t] : (t % S);
+      const bool inside = at >= 0 && at < S;  // a position outside the cos / sin tables is never looked up: NaN
+      ACC_CHECK(inside, kChkRopePos);
+      const long p = inside ? at : 0;
       float cc[W], ss[W];
 #pragma unroll
       for (int q = 0; q < W / 4; ++q) {
@@ -335,8 +336,9 @@ __global__ void rope_kernel(const bf16_t* __restrict__ src, bf16_t* __restrict__
 #pragma unroll
       for (int j = 0; j < W; ++j) {
         const float x1 = bf2f(a.v[j]), x2 = bf2f(b.v[j]);
-        oa.v[j] = f2bf(x1 * cc[j] - x2 * ss[j]);
-        ob.v[j] = f2bf(x2 * cc[j] + x1 * ss[j]);
+        const float r1 = x1 * cc[j] - x2 * ss[j], r2 = x2 * cc[j] + x1 * ss[j];
+        oa.v[j] = f2bf(inside ? r1 : NAN);
+        ob.v[j] = f2bf(inside ? r2 : NAN);
       }
     }
     reinterpret_cast<vec*>(dst + off)[c] = oa;
