@@ -190,7 +190,7 @@ void launch(const torch::Tensor& src, const torch::Tensor& dst, const torch::Ten
   const long passes = std::min<long>(kPasses, std::max<long>(1, a.units / ((long)slots * 2048)));
   a.units_per_block = (int)(passes * slots);
   const long blocks = (a.units + a.units_per_block - 1) / a.units_per_block;
-  TORCH_CHECK(blocks < (1L << 31), "rope: too many heads in one call");
+  TORCH_CHECK(blocks * kThreads < (1L << 32), "rope: too many heads in one call");
   hipLaunchKernelGGL((rope_any_kernel<T, G, INTERLEAVED>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, reinterpret_cast<const T*>(src.data_ptr()),
                      reinterpret_cast<T*>(dst.data_ptr()), cos.data_ptr<float>(), sin.data_ptr<float>(), pos, a);
 }

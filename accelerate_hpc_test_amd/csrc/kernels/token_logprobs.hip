@@ -414,7 +414,6 @@ void check_logits(const torch::Tensor& logits, const torch::Tensor& tokens) {
   TORCH_CHECK(tokens.dim() == 1 && tokens.size(0) == logits.size(0) && tokens.scalar_type() == at::kLong &&
                   tokens.is_contiguous() && tokens.device() == logits.device(),
               "token_logprobs: tokens must be a contiguous int64 [rows] tensor on the logits' device");
-  TORCH_CHECK(logits.size(0) < (1L << 31), "token_logprobs: too many rows");
 }
 
 }  // namespace
@@ -440,7 +439,7 @@ std::vector<torch::Tensor> token_logprobs_fwd(torch::Tensor logits, torch::Tenso
     // Few rows leave most of the chip idle: slices of at least kSlice bytes, as many as give kBlocks blocks.
     const long bytes = V * logits.element_size();
     const int parts = (int)std::max(1L, std::min({(long)kMaxParts, kBlocks / rows, bytes / kSlice}));
-    TORCH_CHECK(rows * parts < (1L << 31), "token_logprobs: too many rows in one call");
+    TORCH_CHECK(rows * parts * 256 < (1L << 32), "token_logprobs: too many rows in one call");
     if (parts > 1) work = torch::empty({rows * parts * (K * 8 + (long)sizeof(Sums))}, fopt.dtype(torch::kUInt8));
     const RowOut out{lp.data_ptr<float>(), ent.data_ptr<float>(), K > 0 ? top_lp.data_ptr<float>() : nullptr,
                      want_stats ? stats.data_ptr<float>() : nullptr, K > 0 ? top_id.data_ptr<int64_t>() : nullptr};
@@ -487,7 +486,7 @@ torch::Tensor token_logprobs_bwd(torch::Tensor logits, torch::Tensor tokens, tor
   ACC_FOR_FLOAT_TYPES(logits.scalar_type(), "token_logprobs", {
     constexpr long per = 16 / sizeof(scalar) * kBwdThreads * kBwdUnroll;
     const long spans = (V + per - 1) / per;
-    TORCH_CHECK(rows * spans < (1L << 31), "token_logprobs: too many rows in one call");
+    TORCH_CHECK(rows * spans * kBwdThreads < (1L << 32), "token_logprobs: too many rows in one call");
     hipLaunchKernelGGL((token_logprobs_bwd_kernel<scalar>), dim3((unsigned)(rows * spans)), dim3(kBwdThreads), 0, stream,
                        reinterpret_cast<const scalar*>(logits.data_ptr()), logits.stride(0), tokens.data_ptr<int64_t>(),
                        stats.data_ptr<float>(), K > 0 ? top_id->data_ptr<int64_t>() : nullptr,

@@ -39,12 +39,12 @@ class LlamaConfig:
     rms_norm_eps: float = 1e-5
     rope_theta: float = 500000.0
     rope_scaling: Optional[dict] = None
-    rope_interleaved: bool = False  # pairs (2i, 2i + 1) instead of (i, i + R/2)
-    partial_rotary_factor: float = 1.0  # the share of each head that is rotated
     max_position_embeddings: int = 8192
     tie_word_embeddings: bool = False
     initializer_range: float = 0.02
     activation_checkpointing: bool = False
+    rope_interleaved: bool = field(default=False, kw_only=True)  # pairs (2i, 2i + 1) instead of (i, i + R/2)
+    partial_rotary_factor: float = field(default=1.0, kw_only=True)  # the share of each head that is rotated
 
     @property
     def rotary_dim(self) -> int:

@@ -600,8 +600,8 @@ class MoELayer(nn.Module):
     def _route(self, logits):
         """Weights (fp32) and experts [T, k] of the router's logits."""
         if self.scoring != "softmax" or self.topk_groups != self.n_groups or self.scale != 1.0:
-            return route_experts(logits, self.top_k, self.scoring, self.router_bias, self.n_groups, self.topk_groups,
-                                 self.norm_topk, self.scale)
+            bias = None if self.router_bias is None else self.router_bias.to(logits.device)
+            return route_experts(logits, self.top_k, self.scoring, bias, self.n_groups, self.topk_groups, self.norm_topk, self.scale)
         probs = torch.softmax(logits.float(), dim=-1)
         if self.router_bias is None:
             w, idx = torch.topk(probs, self.top_k, dim=-1)

@@ -438,7 +438,7 @@ def apply_rope(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, n_rot_he
     if D > 1000:
         raise ValueError(f"HIP rope needs a head size of at most 1000 (got {D})")
     if positions is not None:
-        positions = positions.view(B, S) if positions.numel() == B * S else positions.expand(B, S)
+        positions = positions.reshape(B, S) if positions.numel() == B * S else positions.expand(B, S)
         positions = positions.to(torch.int64)
     return ext().rope(qkv, cos.float().contiguous(), sin.float().contiguous(), positions, n_rot_heads, interleaved)
 

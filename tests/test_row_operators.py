@@ -303,6 +303,20 @@ def test_rope_positions_outside_the_tables(interleaved):
     assert (out[0, :, 0, 8:] == 1).all() and (out[0, :, 1] == 1).all()
 
 
+@gpu
+@pytest.mark.parametrize("D", [128, 24])
+def test_rope_positions_outside_the_tables_whole_heads(D):
+    """bf16 heads rotated whole in halves: their own kernel, forward and backward."""
+    cos, sin = rope_tables(16, D, 10000.0, "cuda")
+    x = torch.ones(1, 5, 3, D, device="cuda", dtype=BF16, requires_grad=True)
+    pos = torch.tensor([[3, 16, -1, -(2**40), 15]], device="cuda")
+    out = apply_rope(x, cos, sin, 2, pos)
+    (d,) = torch.autograd.grad(out, x, torch.ones_like(out))
+    for t in (out, d):
+        assert t[0, [0, 4]].isfinite().all() and t[0, 1:4, :2].isnan().all() and (t[0, :, 2] == 1).all()
+    check(out[0, [0, 4]], rope64(x, cos, sin, 2, torch.tensor([[3, 0, 0, 0, 15]], device="cuda"), False, D)[0, [0, 4]], 6 * U, "inside")
+
+
 @pytest.mark.parametrize("device", ON)
 def test_rope_empty(device):
     cos, sin = rope_tables(8, 4, 10000.0, device)
@@ -492,6 +506,46 @@ def test_token_logprobs_rows_without_a_distribution(device):
     assert r.logprobs[6] == 0 and r.entropy[6] == 0 and r.top_tokens[6].tolist() == [-1, -1] and r.top_logprobs[6].tolist() == [0, 0]
     (d,) = torch.autograd.grad((r.logprobs, r.entropy), leaf, (torch.ones(7, device=device), torch.ones(7, device=device)))
     assert d[:3].isnan().any(-1).all() and not d[3].any() and not d[6].any()
+
+
+@pytest.mark.parametrize("device", ON)
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("V", [50, 70001])
+def test_token_logprobs_masked_rows(device, dtype, V):
+    """Rows that masks leave empty or nearly so, in one block and in slices: the type's lowest value everywhere (a uniform
+    distribution), -inf everywhere, one finite logit at either end, whole stretches of -inf, NaN and +inf far apart."""
+    low = torch.finfo(dtype).min
+    x = torch.full((8, V), -math.inf, device=device, dtype=dtype)
+    x[0] = low
+    x[1, V - 1] = 1.0
+    x[2, 0] = low
+    x[3, V // 2 :] = torch.linspace(-3, 3, V - V // 2, device=device).to(dtype)
+    x[4, V // 3] = math.nan
+    x[5, V // 3] = math.inf
+    x[6] = low
+    x[6, V - 2] = 0.5
+    x = x.requires_grad_()
+    tokens = torch.tensor([V - 1, V - 1, 0, V - 1, 0, 0, V - 2, 3], device=device)
+    r = token_logprobs(x, tokens, top_k=3)
+    (d,) = torch.autograd.grad((r.logprobs[:4].sum() + r.entropy[:4].sum() + r.logprobs[6],), x)
+    tol = 64 * U * math.log(V) + (V * U / 8 if device == "cpu" else 0)
+    assert abs(r.logprobs[0].item() + math.log(V)) < tol and abs(r.entropy[0].item() - math.log(V)) < tol
+    assert r.top_tokens[0].tolist() == [0, 1, 2]
+    for i, t in ((1, V - 1), (2, 0), (6, V - 2)):
+        assert r.logprobs[i] == 0 and r.entropy[i] == 0 and r.top_tokens[i, 0] == t and r.top_logprobs[i, 0] == 0
+        assert not d[i].any()
+    assert r.top_tokens[1].tolist() == [V - 1, 0, 1] and r.top_logprobs[1].tolist() == [0, -math.inf, -math.inf]
+    z = x[3].detach().double()
+    lp = torch.log_softmax(z, -1)
+    assert abs(r.logprobs[3].item() - lp[V - 1].item()) < tol and d[3].isfinite().all()
+    assert r.logprobs[[4, 5, 7]].isnan().all() and r.entropy[[4, 5, 7]].isnan().all() and (r.top_tokens[[4, 5, 7]] == -1).all()
+
+
+@gpu
+def test_token_logprobs_refuses_more_rows_than_a_launch_holds():
+    x = torch.zeros(2**24 + 8, 1, device="cuda", dtype=BF16)
+    with pytest.raises(RuntimeError):
+        token_logprobs(x, torch.zeros(2**24 + 8, dtype=torch.int64, device="cuda"))
 
 
 @pytest.mark.parametrize("device", ON)
@@ -869,6 +923,22 @@ def test_operators_repeat_bit_for_bit_and_on_another_stream():
     torch.cuda.synchronize()
     for a, b, c in zip(first, all_operators(st), there):
         assert torch.equal(a, b) and torch.equal(a, c)
+
+
+@gpu
+def test_backward_is_differentiable_once():
+    """A backward that is itself recorded gives the gradients, and an error where they are differentiated again."""
+    st = all_inputs(5)
+    y, s = layer_norm(st["x"], st["w"], st["b"], 1e-5, st["res"])
+    o = apply_rope(st["qkv"], st["cos"], st["sin"], 3, st["pos"], interleaved=True, rotary_dim=24)
+    r = token_logprobs(st["logits"], st["tokens"])
+    w, _ = route_experts(st["gate"], 4, "sigmoid", st["bias"], 8, 3)
+    for out, leaf, grad in ((y, "x", "dy"), (o, "qkv", "dqkv"), (r.logprobs, "logits", "g1"), (w, "gate", "dw")):
+        (plain,) = torch.autograd.grad(out, st[leaf], st[grad], retain_graph=True)
+        (d,) = torch.autograd.grad(out, st[leaf], st[grad], create_graph=True)
+        assert torch.equal(d, plain) and d.requires_grad
+        with pytest.raises(RuntimeError, match="not differentiable"):
+            d.float().sum().backward()
 
 
 @gpu
