@@ -3,6 +3,7 @@
 // operators is a few microseconds of kernel at small sizes, where Python's autograd.Function cost 77-137 us of host time.
 // Shapes are taken as they come: rows are viewed where strides allow it, copied where not, outputs have the input's shape.
 #include <torch/extension.h>
+#include <c10/core/DeviceGuard.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
 std::vector<torch::Tensor> layer_norm_fwd(torch::Tensor x, c10::optional<torch::Tensor> residual, c10::optional<torch::Tensor> w,
@@ -12,6 +13,8 @@ std::vector<torch::Tensor> layer_norm_bwd(torch::Tensor dy, torch::Tensor s, c10
                                           bool wide_params);
 torch::Tensor rope_any(torch::Tensor src, torch::Tensor cos, torch::Tensor sin, c10::optional<torch::Tensor> pos, int64_t n_rot,
                        bool interleaved, double sign);
+torch::Tensor rope_out(torch::Tensor src, torch::Tensor cos, torch::Tensor sin, c10::optional<torch::Tensor> pos,
+                       int64_t n_rot_heads, int64_t n_heads_total, int64_t head_dim, double sign);
 std::vector<torch::Tensor> token_logprobs_fwd(torch::Tensor logits, torch::Tensor tokens, int64_t K, double inv_t, int64_t ignore,
                                               bool want_stats);
 torch::Tensor token_logprobs_bwd(torch::Tensor logits, torch::Tensor tokens, torch::Tensor stats,
@@ -91,19 +94,29 @@ struct LayerNorm : public torch::autograd::Function<LayerNorm> {
   }
 };
 
+// `whole`: bf16 heads rotated whole in halves, by the kernel for these.
+Tensor rope_by(const Tensor& x, const Tensor& cos, const Tensor& sin, const OptTensor& pos, int64_t n_rot, bool interleaved,
+               bool whole, double sign) {
+  if (x.numel() == 0) return at::empty(x.sizes(), x.options());
+  if (!whole) return rope_any(last_contiguous(x) ? x : x.contiguous(), cos, sin, pos, n_rot, interleaved, sign);
+  const c10::DeviceGuard guard(x.device());
+  return rope_out(x, cos, sin, pos.has_value() ? OptTensor(pos->reshape({-1}).contiguous()) : c10::nullopt, n_rot, x.size(2),
+                  x.size(3), sign);
+}
+
 struct Rope : public torch::autograd::Function<Rope> {
   static Tensor forward(AutogradContext* ctx, const Tensor& qkv, const Tensor& cos, const Tensor& sin, const OptTensor& pos,
-                        int64_t n_rot, bool interleaved) {
+                        int64_t n_rot, bool interleaved, bool whole) {
     ctx->save_for_backward({cos, sin, pos.value_or(Tensor())});
     ctx->saved_data["n_rot"] = n_rot;
-    ctx->saved_data["interleaved"] = interleaved;
-    return rope_any(qkv, cos, sin, pos, n_rot, interleaved, 1.0);
+    ctx->saved_data["form"] = (int64_t)((interleaved ? 1 : 0) | (whole ? 2 : 0));
+    return rope_by(qkv, cos, sin, pos, n_rot, interleaved, whole, 1.0);
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const auto saved = ctx->get_saved_variables();
-    const Tensor d = rope_any(last_contiguous(g[0]) ? g[0] : g[0].contiguous(), saved[0], saved[1], some(saved[2]),
-                              ctx->saved_data["n_rot"].toInt(), ctx->saved_data["interleaved"].toBool(), -1.0);
-    return once({d, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()});
+    const int64_t form = ctx->saved_data["form"].toInt();
+    const Tensor d = rope_by(g[0], saved[0], saved[1], some(saved[2]), ctx->saved_data["n_rot"].toInt(), form & 1, form & 2, -1.0);
+    return once({d, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()});
   }
 };
 
@@ -182,10 +195,10 @@ std::vector<Tensor> layer_norm(const Tensor& x, const OptTensor& w, const OptTen
   return {shaped(out[0], x.sizes()), shaped(out[1], x.sizes())};
 }
 
-Tensor rope(const Tensor& qkv, const Tensor& cos, const Tensor& sin, const OptTensor& pos, int64_t n_rot, bool interleaved) {
-  const Tensor x = last_contiguous(qkv) ? qkv : qkv.contiguous();
-  if (at::GradMode::is_enabled() && x.requires_grad()) return Rope::apply(x, cos, sin, pos, n_rot, interleaved);
-  return rope_any(x, cos, sin, pos, n_rot, interleaved, 1.0);
+Tensor rope(const Tensor& qkv, const Tensor& cos, const Tensor& sin, const OptTensor& pos, int64_t n_rot, bool interleaved,
+            bool whole) {
+  if (at::GradMode::is_enabled() && qkv.requires_grad()) return Rope::apply(qkv, cos, sin, pos, n_rot, interleaved, whole);
+  return rope_by(qkv, cos, sin, pos, n_rot, interleaved, whole, 1.0);
 }
 
 std::vector<Tensor> token_logprobs(const Tensor& logits, const Tensor& tokens, int64_t K, double inv_t, int64_t ignore) {

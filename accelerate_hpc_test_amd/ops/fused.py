@@ -217,6 +217,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     H = x.shape[-1] if x.dim() else 0
     if H < 1:
         raise ValueError(f"layer_norm: x must have a last dimension to normalise, got shape {tuple(x.shape)}")
+    if not x.is_floating_point():
+        raise TypeError(f"layer_norm: x must be of a floating type, got {x.dtype}")
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):
         raise ValueError("layer_norm: residual must have x's shape, type and device")
     for name, p in (("weight", weight), ("bias", bias)):
@@ -388,24 +390,6 @@ def rope_reference(qkv, cos, sin, n_rot_heads, positions=None, interleaved=False
     return torch.cat([out, qkv[..., n_rot_heads:, :]], dim=-2)
 
 
-class _RopeFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, qkv, cos, sin, n_rot_heads, positions):
-        # out of place: one read + one write of qkv (V heads copied through), not a clone followed by an in-place pass
-        B, S, Htot, D = qkv.shape
-        pos = positions.reshape(-1).contiguous() if positions is not None else None
-        out = ext().rope_out(qkv, cos, sin, pos, n_rot_heads, Htot, D, 1.0)
-        ctx.save_for_backward(cos, sin, pos if pos is not None else torch.empty(0))
-        ctx.meta = (n_rot_heads, Htot, D, pos is not None)
-        return out
-
-    @staticmethod
-    def backward(ctx, g):
-        cos, sin, pos = ctx.saved_tensors
-        n_rot, Htot, D, has_pos = ctx.meta
-        return ext().rope_out(g, cos, sin, pos if has_pos else None, n_rot, Htot, D, -1.0), None, None, None, None
-
-
 def apply_rope(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, n_rot_heads: int, positions=None,
                interleaved: bool = False, rotary_dim: Optional[int] = None):
     """qkv: [B, S, Htot, D]; rotates the first `n_rot_heads` heads (Q heads then K heads) by the fp32 tables cos / sin
@@ -429,18 +413,19 @@ def apply_rope(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, n_rot_he
         return rope_reference(qkv, cos, sin, n_rot_heads, positions, interleaved, rotary_dim)
     if qkv.dim() != 4:
         raise ValueError(f"apply_rope: qkv must be [B, S, heads, D], got shape {tuple(qkv.shape)}")
+    # bf16 heads rotated whole in halves have their own kernel (csrc/kernels/norm_act.hip), which copies V heads in the same pass
+    whole = qkv.dtype == torch.bfloat16 and D % 8 == 0 and R == D and not interleaved
+    if D > 1000 and not whole:
+        raise ValueError(f"HIP rope needs a head size of at most 1000 (got {D})")
     B = qkv.shape[0]
     if positions is None:
         cos, sin = cos[:S], sin[:S]  # one row per token of the sequence
-    if (qkv.dtype == torch.bfloat16 and D % 8 == 0 and R == D and not interleaved
-            and (positions is None or (positions.dtype == torch.int64 and positions.numel() == B * S))):
-        return _RopeFn.apply(qkv, cos, sin, n_rot_heads, positions)
-    if D > 1000:
-        raise ValueError(f"HIP rope needs a head size of at most 1000 (got {D})")
-    if positions is not None:
+    if positions is not None and not (positions.dtype == torch.int64 and positions.shape == (B, S)):
         positions = positions.reshape(B, S) if positions.numel() == B * S else positions.expand(B, S)
         positions = positions.to(torch.int64)
-    return ext().rope(qkv, cos.float().contiguous(), sin.float().contiguous(), positions, n_rot_heads, interleaved)
+    if cos.dtype != torch.float32 or sin.dtype != torch.float32:
+        cos, sin = cos.float(), sin.float()
+    return ext().rope(qkv, cos.contiguous(), sin.contiguous(), positions, n_rot_heads, interleaved, whole)
 
 
 # ----------------------------------------------------------------------------------------------------------

@@ -60,6 +60,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0, t
     V = logits.shape[-1]
     if tokens.shape != logits.shape[:-1] or tokens.device != logits.device:
         raise ValueError(f"token_logprobs: tokens must be {tuple(logits.shape[:-1])} on the logits' device, got {tuple(tokens.shape)}")
+    if not logits.is_floating_point():
+        raise TypeError(f"token_logprobs: logits must be of a floating type, got {logits.dtype}")
     if tokens.is_floating_point() or tokens.is_complex() or tokens.dtype == torch.bool:
         raise TypeError(f"token_logprobs: tokens must be integers, got {tokens.dtype}")
     if not 0 <= top_k <= V:

@@ -57,6 +57,8 @@ def route_experts(logits: torch.Tensor, top_k: int, scoring: str = "softmax", bi
     the keys; the weights are differentiable with respect to the logits."""
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise ValueError(f"route_experts: logits must be [tokens, experts], got shape {tuple(logits.shape)}")
+    if not logits.is_floating_point():
+        raise TypeError(f"route_experts: logits must be of a floating type, got {logits.dtype}")
     E = logits.shape[1]
     if scoring not in ("softmax", "sigmoid"):
         raise ValueError(f"route_experts: scoring must be 'softmax' or 'sigmoid', got {scoring!r}")

@@ -202,6 +202,8 @@ def test_layer_norm_refusals(device):
     for bad in (torch.zeros((), device=device), torch.zeros(3, 0, device=device)):
         with pytest.raises(ValueError):
             layer_norm(bad)
+    with pytest.raises(TypeError):
+        layer_norm(torch.zeros(3, 4, dtype=torch.int32, device=device))
     if device == "cuda":
         with pytest.raises(ValueError):
             layer_norm(torch.zeros(1, 32769, device=device, dtype=BF16))
@@ -324,6 +326,10 @@ def test_rope_empty(device):
         x = torch.zeros(shape, device=device, dtype=BF16, requires_grad=True)
         y = apply_rope(x, cos, sin, 0, interleaved=True, rotary_dim=4)
         assert y.shape == shape
+        y.sum().backward()
+        x = torch.zeros(*shape[:3], 8, device=device, dtype=BF16, requires_grad=True)
+        y = apply_rope(x, *rope_tables(8, 8, 10000.0, device), 0)
+        assert y.shape == x.shape
         y.sum().backward()
 
 
@@ -589,6 +595,8 @@ def test_token_logprobs_refusals(device):
     for bad in (t.float(), t.bool()):
         with pytest.raises(TypeError):
             token_logprobs(x, bad)
+    with pytest.raises(TypeError):
+        token_logprobs(x.int(), t)
     if device == "cuda":
         with pytest.raises(ValueError):
             token_logprobs(x, t, top_k=65)
@@ -743,6 +751,8 @@ def test_route_experts_refusals(device):
                      ((x, 2), dict(scale=0.0)), ((x, 2), dict(scale=math.nan)), ((x[0], 2), {}), ((x, 2), dict(n_groups=0))):
         with pytest.raises(ValueError):
             route_experts(*args, **kw)
+    with pytest.raises(TypeError):
+        route_experts(x.int(), 2)
     if device == "cuda":
         with pytest.raises(ValueError):
             route_experts(torch.zeros(1, 1025, device=device), 2)
