@@ -4,7 +4,9 @@
 //   dw = sum over rows of dy * h,  db = sum over rows of dy
 // Both are bound by memory. The row stays in registers between its sums and its output, so x is read once; the variance
 // is the mean of squared distances from the mean, not a difference of two large sums. The threads of a row are chosen by
-// its width alone: one wave (no barrier) up to 256 16-byte chunks, then 256, 512 or 1024 threads.
+// its width and, in the forward, the number of rows: 8 lanes for a 128-byte row (32 rows to a block) up to 1024 threads.
+// 8192 x 4096 bf16 with a residual: 48 us forward and 44 us backward (5.5 and 6.1 TB/s). 200000 x 64 bf16: 12 and 31 us (a wave
+// for each row: 65 and 97), 60000 x 256: 14 and 22 us (23 and 35).
 #include <hip/hip_runtime.h>
 #include <torch/extension.h>
 #include <ATen/hip/HIPContext.h>
@@ -19,26 +21,43 @@ namespace {
 
 constexpr int kMaxChunks = 4096;  // 16-byte chunks in a row: 32768 elements of 16 bits, 16384 of 32
 
-// A chunk of n elements: VEC, the few at the end of a row whose width is no multiple of VEC, or 0 past it.
-template <typename T, int VEC>
-__device__ __forceinline__ Pack<T, VEC> get_chunk(const T* p, int n) {
-  return n == VEC ? load_any<T, VEC>(p) : load_part<T, VEC>(p, n);
+// Chunk c of a row has n = VEC elements, the few at the end of a row whose width is no multiple of VEC, or 0 past it. The few
+// (RAGGED kernels only) are loaded as the last VEC elements of the row, and moved to the front by settle() where they are
+// used: a load that something waits for at once would hold up all the loads behind it. Rows of one chunk or less, shorter
+// than VEC, are loaded element by element.
+template <bool RAGGED, int VEC>
+__device__ __forceinline__ int chunk_size(int c, int nfull, int tail) {
+  return c < nfull ? VEC : RAGGED && c == nfull ? tail : 0;
 }
-template <typename T, int VEC>
+template <bool RAGGED, typename T, int VEC>
+__device__ __forceinline__ Pack<T, VEC> get_chunk(const T* row, int c, int n) {
+  if (n == 0) return Pack<T, VEC>::zero();
+  if constexpr (RAGGED) {
+    if (c == 0 && n < VEC) return load_part<T, VEC>(row, n);
+    return load_any<T, VEC>(row + c * VEC - (VEC - n));
+  }
+  return load_any<T, VEC>(row + c * VEC);
+}
+template <bool RAGGED, typename T, int VEC>
+__device__ __forceinline__ void settle(Pack<T, VEC>& x, int c, int n) {
+  if constexpr (RAGGED)
+    if (n > 0 && n < VEC && c > 0) x = drop_front<T, VEC>(x, VEC - n);
+}
+template <bool RAGGED, typename T, int VEC>
 __device__ __forceinline__ void put_chunk(T* p, const Pack<T, VEC>& x, int n) {
   if (n == VEC) store_any<T, VEC>(p, x);
-  else store_part<T, VEC>(p, x, n);
+  else if constexpr (RAGGED) store_part<T, VEC>(p, x, n);
 }
-template <int VEC>
-__device__ __forceinline__ int chunk_size(int c, int nfull, int tail) { return c < nfull ? VEC : c == nfull ? tail : 0; }
 
-// The row that this thread works on is the same for its whole wave: kept in scalar registers, as are the row's addresses.
+// Where a whole wave works on one row, the row and its addresses are kept in scalar registers.
 template <int TPR, int ROWS>
 __device__ __forceinline__ long first_row() {
-  return (long)blockIdx.x * ROWS + (ROWS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / TPR));
+  if (ROWS == 1) return blockIdx.x;
+  const int slot = threadIdx.x / TPR;
+  return (long)blockIdx.x * ROWS + (TPR < 64 ? slot : __builtin_amdgcn_readfirstlane(slot));
 }
 
-template <typename T, typename W, int TPR, int VPT>
+template <typename T, typename W, int TPR, int VPT, bool RAGGED>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_fwd_kernel(
     const T* __restrict__ x, long x_stride, const T* __restrict__ res, long res_stride, const W* __restrict__ w,
     const W* __restrict__ b, T* __restrict__ y, T* __restrict__ sum_out, float* __restrict__ mean_out,
@@ -52,33 +71,48 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_fwd_kernel(
   constexpr bool kHold = VPT <= 2;
   Pack<W, VEC> wv[VPT], bv[VPT];
   auto load_params = [&](int i) {
-    const int c = li + i * TPR, n = chunk_size<VEC>(c, nfull, tail);
-    if (w != nullptr) wv[i] = get_chunk<W, VEC>(w + c * VEC, n);
-    if (b != nullptr) bv[i] = get_chunk<W, VEC>(b + c * VEC, n);
+    const int c = li + i * TPR, n = chunk_size<RAGGED, VEC>(c, nfull, tail);
+    if (w != nullptr) {
+      wv[i] = get_chunk<RAGGED, W, VEC>(w, c, n);
+      settle<RAGGED, W, VEC>(wv[i], c, n);
+    }
+    if (b != nullptr) {
+      bv[i] = get_chunk<RAGGED, W, VEC>(b, c, n);
+      settle<RAGGED, W, VEC>(bv[i], c, n);
+    }
   };
   if constexpr (kHold) {
 #pragma unroll
     for (int i = 0; i < VPT; ++i) load_params(i);
   }
-  // the trip count is uniform over each row's threads: one wave, or the whole block where barriers are used
+  // the trip count is uniform over each row's threads: lanes of a wave, or the whole block where barriers are used
   for (long row = first_row<TPR, ROWS>(); row < rows; row += (long)gridDim.x * ROWS) {
     const T* xr = x + row * x_stride;
     const T* rr = res == nullptr ? nullptr : res + row * res_stride;
+    Pack<T, VEC> xa[VPT], xb[VPT];
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = li + i * TPR, n = chunk_size<RAGGED, VEC>(c, nfull, tail);
+      xa[i] = get_chunk<RAGGED, T, VEC>(xr, c, n);
+      if (rr != nullptr) xb[i] = get_chunk<RAGGED, T, VEC>(rr, c, n);
+    }
     float v[VPT][VEC];
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int c = li + i * TPR;
-      const int n = chunk_size<VEC>(c, nfull, tail);
-      Pack<T, VEC> a = get_chunk<T, VEC>(xr + c * VEC, n);
+      const int n = chunk_size<RAGGED, VEC>(c, nfull, tail);
+      Pack<T, VEC> a = xa[i];
+      settle<RAGGED, T, VEC>(a, c, n);
       if (rr != nullptr) {
-        const Pack<T, VEC> r = get_chunk<T, VEC>(rr + c * VEC, n);
+        Pack<T, VEC> r = xb[i];
+        settle<RAGGED, T, VEC>(r, c, n);
         float f[VEC];
 #pragma unroll
         for (int j = 0; j < VEC; ++j) f[j] = a.get(j) + r.get(j);
         a = Pack<T, VEC>::of(f);
         // what is normalised is what the residual stream stores
-        put_chunk<T, VEC>(sum_out + row * H + c * VEC, a, n);
+        put_chunk<RAGGED, T, VEC>(sum_out + row * H + c * VEC, a, n);
       }
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
@@ -91,10 +125,10 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_fwd_kernel(
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int c = li + i * TPR;
-      const int n = chunk_size<VEC>(c, nfull, tail);
+      const int n = chunk_size<RAGGED, VEC>(c, nfull, tail);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        v[i][j] = j < n ? v[i][j] - mean : 0.f;
+        v[i][j] = (RAGGED ? j < n : n != 0) ? v[i][j] - mean : 0.f;
         sq = fmaf(v[i][j], v[i][j], sq);
       }
     }
@@ -107,7 +141,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_fwd_kernel(
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int c = li + i * TPR;
-      const int n = chunk_size<VEC>(c, nfull, tail);
+      const int n = chunk_size<RAGGED, VEC>(c, nfull, tail);
       if (n == 0) continue;
       float o[VEC];
       if constexpr (!kHold) load_params(i);
@@ -118,14 +152,14 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_fwd_kernel(
         if (b != nullptr) f += bv[i].get(j);
         o[j] = f;
       }
-      put_chunk<T, VEC>(yr + c * VEC, Pack<T, VEC>::of(o), n);
+      put_chunk<RAGGED, T, VEC>(yr + c * VEC, Pack<T, VEC>::of(o), n);
     }
   }
 }
 
 // One pass over the rows: dx, and each block's share of the column sums of dw and db in registers. The blocks' shares
 // (fp32, [blocks, 2, chunks * VEC]) are added up in a fixed order by layer_norm_colsum_kernel, so results repeat.
-template <typename T, typename W, int TPR, int VPT>
+template <typename T, typename W, int TPR, int VPT, bool RAGGED>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_bwd_kernel(
     const T* __restrict__ dy, long dy_stride, const T* __restrict__ s, long s_stride, const W* __restrict__ w,
     const float* __restrict__ mean, const float* __restrict__ rstd, const T* __restrict__ dres, long dres_stride,
@@ -142,32 +176,59 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_bwd_kernel(
     for (int j = 0; j < VEC; ++j) dw[i][j] = db[i][j] = 0.f;
   // Up to two chunks per thread the weight stays in registers and the next row is loaded while this one is summed: a block
   // walks its rows in sequence, and each would pay the memory's latency after the last one's barrier. Wider rows have no
-  // registers for that.
-  constexpr bool kHold = VPT <= 2;
-  Pack<W, VEC> wv[VPT];
-  auto load_w = [&](int i) {
-    const int c = li + i * TPR;
-    wv[i] = get_chunk<W, VEC>(w + c * VEC, chunk_size<VEC>(c, nfull, tail));
+  // registers for that, and 64 elements per thread none for the row either, beside its columns' sums: the second reading
+  // comes from the cache, in a loop that is not unrolled (2048 rows of 32768 bf16: 314 us, and 424 with the row kept).
+  constexpr bool kHold = VPT <= 2, kKeep = VPT * VEC <= 32;
+  auto load_w = [&](int c) {
+    const int n = chunk_size<RAGGED, VEC>(c, nfull, tail);
+    Pack<W, VEC> p = get_chunk<RAGGED, W, VEC>(w, c, n);
+    settle<RAGGED, W, VEC>(p, c, n);
+    return p;
   };
+  Pack<W, VEC> wv[VPT];
   if (kHold && w != nullptr) {
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) load_w(i);
+    for (int i = 0; i < VPT; ++i) wv[i] = load_w(li + i * TPR);
   }
+  struct Chunk {
+    Pack<T, VEC> s, dy, dres;
+  };
+  auto load_chunk = [&](long row, int c) {
+    Chunk p;
+    const int n = chunk_size<RAGGED, VEC>(c, nfull, tail);
+    p.s = get_chunk<RAGGED, T, VEC>(s + row * s_stride, c, n);
+    p.dy = get_chunk<RAGGED, T, VEC>(dy + row * dy_stride, c, n);  // zero past the row: adds nothing below
+    if (dres != nullptr) p.dres = get_chunk<RAGGED, T, VEC>(dres + row * dres_stride, c, n);
+    return p;
+  };
+  auto settle_chunk = [&](Chunk& p, int c) {
+    const int n = chunk_size<RAGGED, VEC>(c, nfull, tail);
+    settle<RAGGED, T, VEC>(p.s, c, n);
+    settle<RAGGED, T, VEC>(p.dy, c, n);
+    if (dres != nullptr) settle<RAGGED, T, VEC>(p.dres, c, n);
+  };
+  auto put_dx = [&](long row, int c, const Chunk& p, const Pack<W, VEC>& wc, float mu, float r, float s1, float s2) {
+    float o[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      const float dd = p.dy.get(j), h = (p.s.get(j) - mu) * r;
+      const float g = w != nullptr ? dd * wc.get(j) : dd;
+      float f = r * (g - s1 - h * s2);
+      if (dres != nullptr) f += p.dres.get(j);
+      o[j] = f;
+    }
+    put_chunk<RAGGED, T, VEC>(dx + row * H + c * VEC, Pack<T, VEC>::of(o), chunk_size<RAGGED, VEC>(c, nfull, tail));
+  };
   struct Row {
-    Pack<T, VEC> s[VPT], dy[VPT], dres[VPT];
+    Chunk at[VPT];
     float mean, rstd;
   };
   auto load_row = [&](long row, Row& r) {
     r.mean = mean[row];
     r.rstd = rstd[row];
+    if constexpr (kKeep) {
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int c = li + i * TPR;
-      const T *sp = s + row * s_stride + c * VEC, *dp = dy + row * dy_stride + c * VEC, *qp = dres + row * dres_stride + c * VEC;
-      const int n = chunk_size<VEC>(c, nfull, tail);
-      r.s[i] = get_chunk<T, VEC>(sp, n);
-      r.dy[i] = get_chunk<T, VEC>(dp, n);  // zero past the row: adds nothing below
-      if (dres != nullptr) r.dres[i] = get_chunk<T, VEC>(qp, n);
+      for (int i = 0; i < VPT; ++i) r.at[i] = load_chunk(row, li + i * TPR);
     }
   };
   const long step = (long)gridDim.x * ROWS;
@@ -187,10 +248,16 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_bwd_kernel(
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      if (!kHold && w != nullptr) load_w(i);
+      int c = li + i * TPR;
+      // two chunks' loads at a time, the next two behind their sums: the compiler would start all of them and spill
+      if constexpr (!kKeep)
+        if (i % 2 == 0) asm volatile("" : "+v"(c), "+v"(s1));
+      if (!kHold && w != nullptr) wv[i] = load_w(c);
+      if constexpr (!kKeep) cur.at[i] = load_chunk(row, c);
+      settle_chunk(cur.at[i], c);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        const float dd = cur.dy[i].get(j), h = (cur.s[i].get(j) - mu) * r;
+        const float dd = cur.at[i].dy.get(j), h = (cur.at[i].s.get(j) - mu) * r;
         const float g = w != nullptr ? dd * wv[i].get(j) : dd;
         dw[i][j] = fmaf(dd, h, dw[i][j]);
         db[i][j] += dd;
@@ -198,8 +265,8 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_bwd_kernel(
         s2 = fmaf(g, h, s2);
       }
     }
-    s1 = wave_reduce<OpSum>(s1);
-    s2 = wave_reduce<OpSum>(s2);
+    s1 = lanes_reduce<(TPR < 64 ? TPR : 64), OpSum>(s1);
+    s2 = lanes_reduce<(TPR < 64 ? TPR : 64), OpSum>(s2);
     if constexpr (TPR > 64) {  // both sums behind one barrier; the other parity's slots serve the next row
       if ((threadIdx.x & 63) == 0) {
         slots[parity][0][threadIdx.x >> 6] = s1;
@@ -215,27 +282,24 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_bwd_kernel(
     }
     s1 /= width;
     s2 /= width;
+    if constexpr (kKeep) {
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int c = li + i * TPR;
-      const int n = chunk_size<VEC>(c, nfull, tail);
-      if (n == 0) continue;
-      float o[VEC];
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const float dd = cur.dy[i].get(j), h = (cur.s[i].get(j) - mu) * r;
-        const float g = w != nullptr ? dd * wv[i].get(j) : dd;
-        float f = r * (g - s1 - h * s2);
-        if (dres != nullptr) f += cur.dres[i].get(j);
-        o[j] = f;
+      for (int i = 0; i < VPT; ++i) {
+        const int c = li + i * TPR;
+        if (c < chunks) put_dx(row, c, cur.at[i], wv[i], mu, r, s1, s2);
       }
-      put_chunk<T, VEC>(dx + row * H + c * VEC, Pack<T, VEC>::of(o), n);
+    } else {
+      for (int c = li; c < chunks; c += TPR) {
+        Chunk p = load_chunk(row, c);
+        settle_chunk(p, c);
+        put_dx(row, c, p, w != nullptr ? load_w(c) : Pack<W, VEC>::zero(), mu, r, s1, s2);
+      }
     }
   }
   if (part == nullptr) return;
   const long pitch = (long)chunks * VEC;
   float* out = part + (long)blockIdx.x * 2 * pitch;
-  if constexpr (ROWS > 1) {  // the block's waves add into shared memory one after another: a fixed order
+  if constexpr (ROWS > 1) {  // the block's rows add into shared memory one after another: a fixed order
     for (int k = 0; k < ROWS; ++k) {
       if ((int)threadIdx.x / TPR == k) {
 #pragma unroll
@@ -320,6 +384,9 @@ long row_stride(const c10::optional<torch::Tensor>& t) { return t.has_value() ? 
 template <int N> using Const = std::integral_constant<int, N>;
 template <typename F>
 void by_width_fwd(long chunks, long rows, F go) {
+  if (chunks <= 8) return go(Const<8>{}, Const<1>{});
+  if (chunks <= 16) return go(Const<16>{}, Const<1>{});
+  if (chunks <= 32) return go(Const<32>{}, Const<1>{});
   if (chunks <= 64) return go(Const<64>{}, Const<1>{});
   if (rows >= 1024) {  // enough rows to fill the chip: few threads for each, and no barriers up to 256 chunks
     if (chunks <= 128) return go(Const<64>{}, Const<2>{});
@@ -336,13 +403,16 @@ void by_width_fwd(long chunks, long rows, F go) {
 }
 template <typename F>
 void by_width_bwd(long chunks, F go) {
-  if (chunks <= 64) go(Const<64>{}, Const<1>{});
+  if (chunks <= 8) go(Const<8>{}, Const<1>{});
+  else if (chunks <= 16) go(Const<16>{}, Const<1>{});
+  else if (chunks <= 32) go(Const<32>{}, Const<1>{});
+  else if (chunks <= 64) go(Const<64>{}, Const<1>{});
   else if (chunks <= 128) go(Const<64>{}, Const<2>{});
   else if (chunks <= 256) go(Const<256>{}, Const<1>{});
   else if (chunks <= 512) go(Const<256>{}, Const<2>{});
   else if (chunks <= 1024) go(Const<512>{}, Const<2>{});
-  else if (chunks <= 2048) go(Const<1024>{}, Const<2>{});
-  else go(Const<1024>{}, Const<4>{});
+  else if (chunks <= 2048) go(Const<512>{}, Const<4>{});
+  else go(Const<512>{}, Const<8>{});
 }
 
 template <typename T, typename W>
@@ -353,7 +423,8 @@ void launch_fwd(const torch::Tensor& x, const c10::optional<torch::Tensor>& res,
   by_width_fwd((H * (long)sizeof(T) + 15) / 16, rows, [&](auto tpr, auto vpt) {
     constexpr int TPR = decltype(tpr)::value, VPT = decltype(vpt)::value, NT = TPR < 256 ? 256 : TPR, per = NT / TPR;
     const long want = (rows + per - 1) / per, most = 1024L * 256 / NT;
-    hipLaunchKernelGGL((layer_norm_fwd_kernel<T, W, TPR, VPT>), dim3((unsigned)std::min(want, most)), dim3(NT), 0, stream,
+    auto kernel = H % (16 / sizeof(T)) ? layer_norm_fwd_kernel<T, W, TPR, VPT, true> : layer_norm_fwd_kernel<T, W, TPR, VPT, false>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)std::min(want, most)), dim3(NT), 0, stream,
                        reinterpret_cast<const T*>(x.data_ptr()), x.stride(0), ptr<T>(res), row_stride(res), ptr<W>(w), ptr<W>(b),
                        out_ptr<T>(y), out_ptr<T>(sum), out_ptr<float>(mean), out_ptr<float>(rstd), rows, (int)H, eps);
   });
@@ -370,9 +441,11 @@ void launch_bwd(const torch::Tensor& dy, const torch::Tensor& s, const c10::opti
   long blocks = 0;
   by_width_bwd(chunks, [&](auto tpr, auto vpt) {
     constexpr int TPR = decltype(tpr)::value, VPT = decltype(vpt)::value, NT = TPR < 256 ? 256 : TPR, per = NT / TPR;
-    blocks = std::min((rows + per - 1) / per, 512L * 256 / NT);
+    // two blocks for each of the 256 units, or one of 512 and more threads: every block leaves a share to add up
+    blocks = std::min((rows + per - 1) / per, NT == 256 ? 512L : 256L);
     if (sums) part = torch::empty({blocks, 2, pitch}, s.options().dtype(at::kFloat));
-    hipLaunchKernelGGL((layer_norm_bwd_kernel<T, W, TPR, VPT>), dim3((unsigned)blocks), dim3(NT),
+    auto kernel = H % VEC ? layer_norm_bwd_kernel<T, W, TPR, VPT, true> : layer_norm_bwd_kernel<T, W, TPR, VPT, false>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(NT),
                        per > 1 && sums ? 2 * pitch * sizeof(float) : 0, stream, reinterpret_cast<const T*>(dy.data_ptr()),
                        dy.stride(0), reinterpret_cast<const T*>(s.data_ptr()), s.stride(0), ptr<W>(w), mean.data_ptr<float>(),
                        rstd.data_ptr<float>(), ptr<T>(dres), row_stride(dres), out_ptr<T>(dx), out_ptr<float>(part), rows, (int)H);

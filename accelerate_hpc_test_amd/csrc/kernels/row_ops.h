@@ -103,7 +103,7 @@ __device__ __forceinline__ void store_any(T* p, const Pack<T, N>& x) {
   else *reinterpret_cast<loose*>(p) = __builtin_bit_cast(raw, x);
 }
 
-// Elements [0, n) of a chunk, n < N: the end of a row whose width is no multiple of N. The rest is zero.
+// Elements [0, n) of a chunk, n < N, one by one; the rest is zero.
 template <typename T, int N>
 __device__ __forceinline__ Pack<T, N> load_part(const T* p, int n) {
   Pack<T, N> x = Pack<T, N>::zero();
@@ -114,6 +114,36 @@ __device__ __forceinline__ Pack<T, N> load_part(const T* p, int n) {
       else x.u[j / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[j] << (16 * (j & 1));
     }
   return x;
+}
+
+// Elements [s, N) of x moved to its front, zero behind them.
+template <typename T, int N>
+__device__ __forceinline__ Pack<T, N> drop_front(Pack<T, N> x, int s) {
+  constexpr int words = Pack<T, N>::kWords;
+  int by = s;
+  if constexpr (sizeof(T) == 2) {
+    by = s >> 1;
+    if (s & 1) {
+#pragma unroll
+      for (int i = 0; i < words; ++i) x.u[i] = (x.u[i] >> 16) | (i + 1 < words ? x.u[i + 1] << 16 : 0);
+    }
+  }
+#pragma unroll
+  for (int step = 1; step < words; step <<= 1)
+    if (by & step) {
+#pragma unroll
+      for (int i = 0; i < words; ++i) x.u[i] = i + step < words ? x.u[i + step] : 0;
+    }
+  return x;
+}
+
+// load_part at the end of a row, with `before` elements of the row ahead of p: one access that ends with the row and a shift,
+// where the row is that long. (Single loads cost the latency of memory each, all of them at once eight addresses.)
+template <typename T, int N>
+__device__ __forceinline__ Pack<T, N> load_tail(const T* p, int n, int before) {
+  if (n <= 0) return Pack<T, N>::zero();
+  if (before >= N - n) return drop_front<T, N>(load_any<T, N>(p - (N - n)), N - n);
+  return load_part<T, N>(p, n);
 }
 
 template <typename T, int N>
@@ -173,11 +203,11 @@ __device__ __forceinline__ uint32_t lanes_max_u32(uint32_t v) { return lanes_red
 template <int L>
 __device__ __forceinline__ uint32_t lanes_or(uint32_t v) { return lanes_reduce_u32<L, OpOr>(v); }
 
-// wave_reduce over THREADS threads that form a block (or over one wave). `slots`: 16 floats of shared memory that no other
+// The same over THREADS threads: lanes of a wave, or the threads of a block. `slots`: 16 floats of shared memory that no other
 // reduction uses between two barriers of the block.
 template <typename Op, int THREADS>
 __device__ __forceinline__ float row_reduce(float v, float* slots) {
-  v = wave_reduce<Op>(v);
+  v = lanes_reduce<(THREADS < 64 ? THREADS : 64), Op>(v);
   if constexpr (THREADS > 64) {
     if ((threadIdx.x & 63) == 0) slots[threadIdx.x >> 6] = v;
     __syncthreads();

