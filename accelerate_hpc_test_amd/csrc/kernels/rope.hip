@@ -4,11 +4,14 @@
 // Bound by memory: one read and one write of every value. A head is cut into windows of 16 bytes, the last one moved back to
 // end with the head (windows that overlap write the same bytes), so every load and store is whole and all lanes of a wave
 // move data, whatever R and D are: out = x cos + partner (+-sin) needs the partners of a window's values beside them, which
-// are a swap in registers (interleaved) or second loads of a line that is in flight anyway (half layout: one, or
-// a few where the halves do not divide into windows). A thread keeps one window position for all the
+// are a swap in registers (interleaved) or a second load of a line that is in flight anyway (half layout: each half is cut
+// into windows of its own, the last one moved back to end with the half; a few loads where a half is shorter than a window).
+// A thread keeps one window position for all the
 // (token, head) units that it walks, so a token's cos / sin are loaded once and serve all its heads from registers. The
 // source may have any strides over batch, sequence and heads. 8192 tokens with 192 heads of 96 bf16, 24 turned in halves: 109 us,
-// 5.5 TB/s (one unit per thread: 138 us). Halves of an odd length, whose partners are single loads, run at half that rate.
+// 5.5 TB/s (one unit per thread: 138 us). 8192 x 48 heads of 128, 126 turned in halves: 45 us (82 with windows that hold values
+// of both halves and single loads of their partners). Heads with odd halves shorter than a window take such loads still, at
+// half the copy's rate.
 #include <hip/hip_runtime.h>
 #include <torch/extension.h>
 #include <ATen/hip/HIPContext.h>
@@ -38,6 +41,7 @@ struct RopeArgs {
   long pb, ps;      // position strides
   long units;       // batch * seq * heads
   int seq, heads, n_rot, D, R, S;
+  int windows;  // of a head
   int units_per_block;
   float sign;
 };
@@ -56,21 +60,28 @@ __device__ __forceinline__ Pack<T, M> swap_pairs(const Pack<T, M>& x) {
   return p;
 }
 
-// G: a window falls into pieces of G values that turn together, with partners side by side (half layout: the largest power of
-// two that divides the half, the head and 16 bytes; interleaved: the whole window where the head is even, else 1).
+// G: a window falls into pieces of G values that turn together, with partners side by side. Half layout: the whole window where
+// a half has room for one, else the largest power of two that divides the half and the head; interleaved: the whole window
+// where the head is even, else 1.
 template <typename T, int G, bool INTERLEAVED>
 __global__ __launch_bounds__(kThreads) void rope_any_kernel(const T* __restrict__ src, T* __restrict__ dst,
                                                             const float* __restrict__ cosb, const float* __restrict__ sinb,
                                                             const int64_t* __restrict__ pos, const RopeArgs a) {
   constexpr int M = 16 / sizeof(T);
   constexpr bool kSwap = INTERLEAVED && G > 1;  // partners within the window
-  const int windows = (a.D + M - 1) / M;
+  constexpr bool kHalves = !INTERLEAVED && G == M;  // no window holds values of both halves
+  const int windows = a.windows;
   const int slots = kThreads / windows;  // units walked side by side by a block
   const int slot = threadIdx.x / windows, item = threadIdx.x - slot * windows;
   if (slot >= slots) return;
   const int half = a.R >> 1;
   const bool short_head = a.D < M;
-  const int d0 = short_head ? 0 : min(item * M, a.D - M);
+  int d0 = short_head ? 0 : min(item * M, a.D - M);
+  if constexpr (kHalves) {
+    const int per = (half + M - 1) / M;
+    if (item < 2 * per) d0 = item < per ? min(item * M, half - M) : half + min((item - per) * M, half - M);
+    else d0 = min(a.R + (item - 2 * per) * M, a.D - M);  // may begin in the second half, where the rest is shorter than it
+  }
   const bool turns = d0 < a.R;
   const long first = (long)blockIdx.x * a.units_per_block;
   const int count = (int)min((long)a.units_per_block, a.units - first);
@@ -149,8 +160,9 @@ __global__ __launch_bounds__(kThreads) void rope_any_kernel(const T* __restrict_
                 const int d = d0 + i, angle = INTERLEAVED ? d / 2 : d < half ? d : d - half;
                 const bool minus = INTERLEAVED ? (d & 1) == 0 : d < half;
                 float cc[G], ss[G];
-                load_angles<G>(cosb + row + angle, cc, d < a.R ? G : 0);
-                load_angles<G>(sinb + row + angle, ss, d < a.R ? G : 0);
+                const int n = kHalves ? min(G, half - angle) : d < a.R ? G : 0;
+                load_angles<G>(cosb + row + angle, cc, n);
+                load_angles<G>(sinb + row + angle, ss, n);
 #pragma unroll
                 for (int j = 0; j < G; ++j) {
                   c[i + j] = cc[j];
@@ -186,7 +198,10 @@ template <typename T, int G, bool INTERLEAVED>
 void launch(const torch::Tensor& src, const torch::Tensor& dst, const torch::Tensor& cos, const torch::Tensor& sin,
             const int64_t* pos, RopeArgs a, hipStream_t stream) {
   constexpr int M = 16 / sizeof(T);
-  const int slots = kThreads / ((a.D + M - 1) / M);
+  const auto cut = [](int n) { return (n + M - 1) / M; };
+  a.windows = !INTERLEAVED && G == M ? 2 * cut(a.R / 2) + cut(a.D - a.R) : cut(a.D);
+  TORCH_CHECK(a.windows <= kThreads, "rope: head size");
+  const int slots = kThreads / a.windows;
   // Each block walks a few units of every slot: enough to reuse a token's angles, few enough to fill the chip.
   const long passes = std::min<long>(kPasses, std::max<long>(1, a.units / ((long)slots * 2048)));
   a.units_per_block = (int)(passes * slots);
@@ -237,8 +252,8 @@ torch::Tensor rope_any(torch::Tensor src, torch::Tensor cos, torch::Tensor sin, 
     const auto fits = [&](long g) { return R / 2 % g == 0 && D % g == 0; };
     auto go = [&](auto kind) { kind(src, out, cos, sin, pp, a, stream); };
     if (interleaved) go(D % 2 == 0 ? launch<scalar, M, true> : launch<scalar, 1, true>);
-    else if (fits(M)) go(launch<scalar, M, false>);
-    else if (fits(4)) go(launch<scalar, 4, false>);
+    else if (R / 2 >= M) go(launch<scalar, M, false>);
+    else if (M > 4 && fits(4)) go(launch<scalar, (M > 4 ? 4 : 1), false>);
     else if (fits(2)) go(launch<scalar, 2, false>);
     else go(launch<scalar, 1, false>);
   });

@@ -135,6 +135,14 @@ def test_layer_norm_many_rows(rows, hidden, dtype):
     run_norm("cuda", rows, hidden, dtype, True, "both")
 
 
+@gpu
+@pytest.mark.parametrize("rows,hidden,dtype", [(33001, 64, BF16), (33001, 61, BF16), (40003, 32, FP32), (17003, 100, BF16), (9001, 250, FP16),
+                                               (700, 9001, BF16), (600, 20001, BF16), (300, 24576, FP16), (300, 16381, FP32)])
+def test_layer_norm_rows_past_one_round_of_the_blocks(rows, hidden, dtype):
+    # rows that share a wave, and rows of 512 threads: more of each than the blocks of a launch take at once, whole and ragged
+    run_norm("cuda", rows, hidden, dtype, True, "both")
+
+
 @pytest.mark.parametrize("device", ON)
 def test_layer_norm_strides_and_broadcast_gradients(device):
     g = gen(device, 1)
@@ -257,6 +265,15 @@ ROPE_SIZES = [(128, 128), (64, 64), (256, 64), (96, 24), (80, 74), (80, 78), (64
 @pytest.mark.parametrize("D,R", ROPE_SIZES)
 def test_rope(device, D, R, interleaved, dtype):
     run_rope(device, 2, 13, 5, 7, D, R, interleaved, dtype, positions=(D + R) % 3 != 0)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("D,R", [(8, 8), (9, 8), (16, 16), (17, 16), (19, 18), (23, 18), (24, 18), (31, 22), (40, 30), (1000, 994), (1000, 10),
+                                 (999, 998), (1000, 18)])
+def test_rope_windows_of_the_halves(D, R, dtype):
+    # halves of a window, of one value less or more, copied ends shorter and longer than a window, the widest heads
+    run_rope("cuda", 2, 11, 3, 4, D, R, False, dtype, positions=True)
 
 
 @pytest.mark.parametrize("device", ON)
