@@ -177,7 +177,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_bwd_kernel(
   // Up to two chunks per thread the weight stays in registers and the next row is loaded while this one is summed: a block
   // walks its rows in sequence, and each would pay the memory's latency after the last one's barrier. Wider rows have no
   // registers for that, and 64 elements per thread none for the row either, beside its columns' sums: the second reading
-  // comes from the cache, in a loop that is not unrolled (2048 rows of 32768 bf16: 314 us, and 424 with the row kept).
+  // comes from the cache, in a loop that is not unrolled (2048 rows of 32768 bf16: 301 us, and 424 with the row kept).
   constexpr bool kHold = VPT <= 2, kKeep = VPT * VEC <= 32;
   auto load_w = [&](int c) {
     const int n = chunk_size<RAGGED, VEC>(c, nfull, tail);
@@ -245,13 +245,20 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_bwd_kernel(
       load_row(row, cur);
     }
     const float mu = cur.mean, r = cur.rstd;
-    float s1 = 0.f, s2 = 0.f;
+    float s1 = 0.f, s2 = 0.f, s1_before = 0.f, s2_before = 0.f;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       int c = li + i * TPR;
-      // two chunks' loads at a time, the next two behind their sums: the compiler would start all of them and spill
-      if constexpr (!kKeep)
-        if (i % 2 == 0) asm volatile("" : "+v"(c), "+v"(s1));
+      if constexpr (!kKeep) {
+        if (i % 2 == 0) {  // two chunks at a time, which keeps the chains of additions as short as those of narrower rows, and
+          s1_before += s1;  // their loads behind the last two's sums: the compiler would start all of them and spill
+          s2_before += s2;
+          s1 = s2 = 0.f;
+          asm volatile("" : "+v"(c), "+v"(s1_before), "+v"(s2_before));
+        } else {
+          asm volatile("" : "+v"(c));
+        }
+      }
       if (!kHold && w != nullptr) wv[i] = load_w(c);
       if constexpr (!kKeep) cur.at[i] = load_chunk(row, c);
       settle_chunk(cur.at[i], c);
@@ -264,6 +271,10 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_bwd_kernel(
         s1 += g;
         s2 = fmaf(g, h, s2);
       }
+    }
+    if constexpr (!kKeep) {
+      s1 += s1_before;
+      s2 += s2_before;
     }
     s1 = lanes_reduce<(TPR < 64 ? TPR : 64), OpSum>(s1);
     s2 = lanes_reduce<(TPR < 64 ? TPR : 64), OpSum>(s2);
