@@ -542,6 +542,8 @@ static void rope_launch(const torch::Tensor& src, torch::Tensor& dst, const torc
   check_bf16_cuda(dst, "out");
   TORCH_CHECK(src.numel() == dst.numel(), "rope: src / dst size mismatch");
   TORCH_CHECK(cos.scalar_type() == at::kFloat && sin.scalar_type() == at::kFloat, "rope tables must be fp32");
+  TORCH_CHECK(cos.device() == src.device() && sin.device() == src.device() && cos.is_contiguous() && sin.is_contiguous(),
+              "rope: cos and sin must be contiguous, on the input's device");
   TORCH_CHECK(head_dim % 8 == 0, "rope: head_dim must be a multiple of 8");
   TORCH_CHECK(src.numel() % (n_heads_total * head_dim) == 0 && n_rot_heads <= n_heads_total, "rope: bad head counts");
   const long T = src.numel() / (n_heads_total * head_dim);
@@ -549,7 +551,8 @@ static void rope_launch(const torch::Tensor& src, torch::Tensor& dst, const torc
   TORCH_CHECK(cos.numel() >= (long)S * (head_dim / 2) && sin.numel() == cos.numel(), "rope: tables must be [S, D/2]");
   const int64_t* posp = nullptr;
   if (pos.has_value()) {
-    TORCH_CHECK(pos->scalar_type() == at::kLong && pos->numel() == T, "rope: positions must be int64 [T]");
+    TORCH_CHECK(pos->scalar_type() == at::kLong && pos->numel() == T && pos->device() == src.device() && pos->is_contiguous(),
+                "rope: positions must be contiguous int64 [T] on the input's device");
     posp = pos->data_ptr<int64_t>();
   }
   const bool inplace = src.data_ptr() == dst.data_ptr();

@@ -396,8 +396,8 @@ def apply_rope(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, n_rot_he
     [positions, R/2] of `rope_tables`, in half pairs (i, i + R/2) or, `interleaved`, pairs (2i, 2i + 1).
 
     `rotary_dim`: R, the rotated first values of each head, even; None rotates the whole head. `positions`: integers [B, S]
-    (or [1, S], [S] for every batch row), each token's row of the tables; None counts from 0. The result is a new contiguous
-    tensor. On a GPU any strides and even R are taken, in bf16, fp16 and fp32, with D up to 1000; a position outside the
+    (or [1, S], [S] for every batch row), each token's row of the tables; None counts from 0. The tables lie on qkv's device, the
+    positions there or on the host. The result is a new contiguous tensor. On a GPU any strides and even R are taken, in bf16, fp16 and fp32, with D up to 1000; a position outside the
     tables gives NaN in its rotated values."""
     S, Htot, D = qkv.shape[-3:]
     R = D if rotary_dim is None else rotary_dim
@@ -407,6 +407,12 @@ def apply_rope(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, n_rot_he
         raise ValueError(f"apply_rope: cos and sin must be [positions, {R // 2}] tables, got {tuple(cos.shape)}, {tuple(sin.shape)}")
     if not 0 <= n_rot_heads <= Htot:
         raise ValueError(f"apply_rope: {n_rot_heads} of {Htot} heads to rotate")
+    if cos.device != qkv.device or sin.device != qkv.device:
+        raise ValueError(f"apply_rope: cos and sin must be on qkv's device ({qkv.device}), got {cos.device}, {sin.device}")
+    if positions is not None and positions.device != qkv.device:
+        if positions.device.type != "cpu":
+            raise ValueError(f"apply_rope: positions must be on qkv's device ({qkv.device}) or the host, got {positions.device}")
+        positions = positions.to(qkv.device)
     if positions is None and S > cos.shape[0]:
         raise ValueError(f"apply_rope: {S} tokens, but tables for {cos.shape[0]} positions")
     if not (use_native(qkv) and qkv.dtype in ROW_DTYPES):
