@@ -425,7 +425,9 @@ RouteArgs args_of(const torch::Tensor& logits, int64_t k, bool softmax, int64_t 
   TORCH_CHECK(groups >= 1 && groups <= kMaxGroups && E % groups == 0 && top_groups >= 1 && top_groups <= groups,
               "route_experts: groups must divide the experts, at most ", kMaxGroups, " of them");
   TORCH_CHECK(k >= 1 && k <= kMaxTop && k <= E / groups * top_groups, "route_experts: more choices than open experts, or than ", kMaxTop);
-  TORCH_CHECK(logits.size(0) < (1L << 26), "route_experts: too many rows in one call");
+  // a wave for each row, whole blocks: fewer than 2^32 threads to a launch (the backward has at most as many)
+  constexpr long per = kThreads / 64;
+  TORCH_CHECK((logits.size(0) + per - 1) / per * kThreads < (1L << 32), "route_experts: too many rows in one call");
   return RouteArgs{logits.size(0), logits.stride(0), (int)E, (int)k, (int)groups, (int)top_groups, softmax, renorm, (float)scale};
 }
 

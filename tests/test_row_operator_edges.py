@@ -8,7 +8,7 @@ import math
 import pytest
 import torch
 
-from accelerate_hpc_test_amd.ops import apply_rope, rope_tables
+from accelerate_hpc_test_amd.ops import apply_rope, rope_tables, route_experts
 
 U = 2.0 ** -24
 BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
@@ -61,3 +61,20 @@ def test_rope_kernels_refuse_host_memory():
             ext().rope(x, c, s, None if p is None else p.view(1, 3), 1, False, True)
         with pytest.raises(RuntimeError, match="device"):
             ext().rope(x, c, s, None if p is None else p.view(1, 3), 1, True, False)
+
+
+# ---------------------------------------------------------------------------------------------------------- routing to experts
+@gpu
+@pytest.mark.parametrize("rows", [2**26 - 3, 2**26 - 1, 2**26])
+def test_route_experts_refuses_more_rows_than_a_launch_holds(rows):
+    """Four rows to a block of 256 threads: 2^26 - 3 rows are 2^24 blocks, 2^32 threads."""
+    with pytest.raises(RuntimeError, match="too many rows"):
+        route_experts(torch.zeros(1, 2, device="cuda", dtype=BF16).expand(rows, 2), 1)
+
+
+@gpu
+def test_route_experts_most_rows():
+    """The largest launch that is taken writes its last rows (rows at a stride of zero: 2 logits in memory)."""
+    x = torch.tensor([[0.0, 1.0]], device="cuda", dtype=BF16).expand(2**26 - 4, 2)
+    w, ids = route_experts(x, 1)
+    assert bool((ids == 1).all()) and bool((w == 1).all())
