@@ -52,9 +52,9 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0, t
 
     logits [..., V] in bf16, fp16 or fp32; tokens: integers [...]. All outputs are fp32 and differentiable with respect to the
     logits (the alternatives at their chosen tokens). Rows whose token is `ignore_index` give 0, 0, 0 and -1 and no gradient;
-    a token outside [0, V) gives NaN. The backward reads the logits again: beside `cross_entropy` on the same logits, give that
-    `inplace_backward=False`. Logits of -inf are impossible tokens: probability 0, nothing added to the entropy. A row
-    with NaN or +inf, or of -inf alone, has no distribution: NaN, and -1 for the alternatives."""
+    a token outside [0, V) gives a NaN log-probability that carries no gradient. The backward reads the logits again: beside
+    `cross_entropy` on the same logits, give that `inplace_backward=False`. Logits of -inf are impossible tokens: probability 0,
+    nothing added to the entropy. A row with NaN or +inf, or of -inf alone, has no distribution: NaN, and -1 for the alternatives."""
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise ValueError(f"token_logprobs: logits must be [..., vocabulary], got shape {tuple(logits.shape)}")
     V = logits.shape[-1]

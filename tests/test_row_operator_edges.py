@@ -8,7 +8,7 @@ import math
 import pytest
 import torch
 
-from accelerate_hpc_test_amd.ops import apply_rope, rope_tables, route_experts
+from accelerate_hpc_test_amd.ops import apply_rope, rope_tables, route_experts, token_logprobs
 
 U = 2.0 ** -24
 BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
@@ -78,3 +78,27 @@ def test_route_experts_most_rows():
     x = torch.tensor([[0.0, 1.0]], device="cuda", dtype=BF16).expand(2**26 - 4, 2)
     w, ids = route_experts(x, 1)
     assert bool((ids == 1).all()) and bool((w == 1).all())
+
+
+# ------------------------------------------------------------------------------------------------------ token log-probabilities
+@pytest.mark.parametrize("device", ON)
+@pytest.mark.parametrize("V", [50, 70001])  # whole rows, and rows in slices
+def test_token_logprobs_of_tokens_outside_the_vocabulary_carry_no_gradient(device, V):
+    """The log-probability of such a token is a NaN constant; the row's entropy and alternatives are sound, and so are their
+    gradients. Differences of fp32 logits: the row's gradient equals that of a row with no log-probability in the loss."""
+    g = torch.Generator(device=device).manual_seed(3)
+    x = torch.randn(4, V, generator=g, device=device).requires_grad_()
+    inside = torch.tensor([1, 2, 3, 4], device=device)
+    outside = torch.tensor([1, V, 3, -7], device=device)
+    losses = (lambda r: r.entropy.sum(), lambda r: (r.top_logprobs * 0.5).sum(), lambda r: r.entropy.sum() + r.top_logprobs[:, 1].sum())
+    for loss in losses:
+        want, got = (torch.autograd.grad(loss(token_logprobs(x, t, top_k=2)), x)[0] for t in (inside, outside))
+        assert want.isfinite().all() and torch.equal(got, want)
+    # beside log-probabilities: rows 0 and 2 as before, rows 1 and 3 without the term that has no value
+    want, = torch.autograd.grad((lambda r: r.entropy.sum() + r.logprobs[[0, 2]].sum())(token_logprobs(x, inside)), x)
+    r = token_logprobs(x, outside)
+    assert r.logprobs[[1, 3]].isnan().all() and r.logprobs[[0, 2]].isfinite().all()
+    got, = torch.autograd.grad(r.entropy.sum() + r.logprobs.sum(), x)
+    assert torch.equal(got, want)
+    got, = torch.autograd.grad(token_logprobs(x, outside).logprobs.sum(), x)
+    assert not got[[1, 3]].any() and got[[0, 2]].any(-1).all()
