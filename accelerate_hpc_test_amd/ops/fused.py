@@ -369,7 +369,12 @@ def rope_reference(qkv, cos, sin, n_rot_heads, positions=None, interleaved=False
     if positions is None:
         c, s = cos[:T], sin[:T]
     else:
-        c, s = cos[positions.reshape(-1)], sin[positions.reshape(-1)]
+        at = positions.reshape(-1)
+        if at.is_cuda:  # as the kernels: a position outside the tables is never looked up
+            inside = (at >= 0) & (at < cos.shape[0])
+            c, s = (torch.where(inside[:, None], t[torch.where(inside, at, 0)], math.nan) for t in (cos, sin))
+        else:
+            c, s = cos[at], sin[at]
         c = c.view(*positions.shape, R // 2)
         s = s.view(*positions.shape, R // 2)
     x = qkv[..., :n_rot_heads, :R]
@@ -397,8 +402,9 @@ def apply_rope(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, n_rot_he
 
     `rotary_dim`: R, the rotated first values of each head, even; None rotates the whole head. `positions`: integers [B, S]
     (or [1, S], [S] for every batch row), each token's row of the tables; None counts from 0. The tables lie on qkv's device, the
-    positions there or on the host. The result is a new contiguous tensor. On a GPU any strides and even R are taken, in bf16, fp16 and fp32, with D up to 1000; a position outside the
-    tables gives NaN in its rotated values."""
+    positions there or on the host. The result is a new contiguous tensor. On a GPU any strides and even R are taken, in bf16,
+    fp16 and fp32, with D up to 1000; a position outside the tables gives NaN in its rotated values. Tables that require
+    gradients get them, from plain torch operations."""
     S, Htot, D = qkv.shape[-3:]
     R = D if rotary_dim is None else rotary_dim
     if R < 2 or R % 2 or R > D:
@@ -415,7 +421,8 @@ def apply_rope(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, n_rot_he
         positions = positions.to(qkv.device)
     if positions is None and S > cos.shape[0]:
         raise ValueError(f"apply_rope: {S} tokens, but tables for {cos.shape[0]} positions")
-    if not (use_native(qkv) and qkv.dtype in ROW_DTYPES):
+    learned = torch.is_grad_enabled() and (cos.requires_grad or sin.requires_grad)  # the kernels have no gradient for tables
+    if learned or not (use_native(qkv) and qkv.dtype in ROW_DTYPES):
         return rope_reference(qkv, cos, sin, n_rot_heads, positions, interleaved, rotary_dim)
     if qkv.dim() != 4:
         raise ValueError(f"apply_rope: qkv must be [B, S, heads, D], got shape {tuple(qkv.shape)}")

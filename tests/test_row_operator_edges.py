@@ -102,3 +102,40 @@ def test_token_logprobs_of_tokens_outside_the_vocabulary_carry_no_gradient(devic
     assert torch.equal(got, want)
     got, = torch.autograd.grad(token_logprobs(x, outside).logprobs.sum(), x)
     assert not got[[1, 3]].any() and got[[0, 2]].any(-1).all()
+
+
+# ------------------------------------------------------------------------------------------------------------- derivatives
+@pytest.mark.parametrize("device", ON)
+@pytest.mark.parametrize("dtype,D,R,interleaved", ROPE_FORMS + [(FP16, 12, 12, False)])
+def test_rope_gradients_of_the_tables(device, dtype, D, R, interleaved):
+    """Tables that require gradients: d cos = sum a g_a + b g_b, d sin = sum a g_b - b g_a over the pairs of a table row, here B * n_rot
+    of them, and once with an input that requires none. An fp32 sum of 2 n terms is off by 2 n U of their absolute sum."""
+    B, S, n = 2, 3, 3
+    g = torch.Generator(device=device).manual_seed(4)
+    x, dy = (torch.randn(B, S, 4, D, generator=g, device=device).to(dtype) for _ in range(2))
+    pairs = (lambda t: (t[..., 0:R:2], t[..., 1:R:2])) if interleaved else (lambda t: (t[..., : R // 2], t[..., R // 2 : R]))
+    (a, b), (ga, gb) = (pairs(t[:, :, :n].double()) for t in (x, dy))
+    size = (a.abs() + b.abs()) * (ga.abs() + gb.abs())
+    for leaf in (True, False):
+        cos, sin = (t.requires_grad_() for t in rope_tables(S, R, 10000.0, device))
+        x = x.detach().requires_grad_(leaf)
+        y = apply_rope(x, cos, sin, n, interleaved=interleaved, rotary_dim=R)
+        assert y.requires_grad
+        dcos, dsin = torch.autograd.grad(y, (cos, sin), dy)
+        tol = 2 * B * n * U * size.sum((0, 2))
+        assert ((dcos - (a * ga + b * gb).sum((0, 2))).abs() <= tol).all()
+        assert ((dsin - (a * gb - b * ga).sum((0, 2))).abs() <= tol).all()
+        with torch.no_grad():
+            plain = apply_rope(x, cos, sin, n, interleaved=interleaved, rotary_dim=R)
+        assert (plain.double() - y.double()).abs().max() <= 2 * torch.finfo(dtype).eps * y.abs().max()
+
+
+@gpu
+def test_rope_positions_outside_learned_tables():
+    """The torch path of tables that require gradients keeps the kernels' contract: NaN, and nothing read past the tables."""
+    cos, sin = (t.requires_grad_() for t in rope_tables(16, 8, 10000.0, "cuda"))
+    x = torch.ones(1, 4, 2, 12, device="cuda", dtype=FP32)
+    out = apply_rope(x, cos, sin, 1, torch.tensor([[0, 16, -1, 2**40]], device="cuda"), rotary_dim=8)
+    assert out[0, 0].isfinite().all() and out[0, 1:, 0, :8].isnan().all() and (out[0, :, 0, 8:] == 1).all() and (out[0, :, 1] == 1).all()
+    (d,) = torch.autograd.grad(out[0, 0].sum(), cos)
+    assert d.isfinite().all() and d[0].all() and not d[1:].any()
