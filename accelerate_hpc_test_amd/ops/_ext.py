@@ -11,6 +11,7 @@ import importlib
 import os
 
 import torch
+import torch.autograd.forward_ad as _forward_ad
 
 _EXT = None
 _ERR = None
@@ -51,3 +52,13 @@ def native_enabled() -> bool:
 def use_native(t: torch.Tensor) -> bool:
     """True when `t` lives on a GPU and native kernels are enabled (then the extension is mandatory)."""
     return t.is_cuda and native_enabled()
+
+
+def forward_mode(*tensors) -> bool:
+    """True inside a `torch.func` transform, and where one of `tensors` (None skipped) carries a forward-mode tangent: torch operations
+    take these along, a kernel behind an autograd node would drop them."""
+    if torch._C._are_functorch_transforms_active():
+        return True
+    if _forward_ad._current_level < 0:
+        return False
+    return any(t is not None and _forward_ad.unpack_dual(t).tangent is not None for t in tensors)

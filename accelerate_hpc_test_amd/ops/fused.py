@@ -11,7 +11,7 @@ from typing import Optional
 
 import torch
 
-from ._ext import ext, use_native
+from ._ext import ext, forward_mode, use_native
 
 # element types of the row operators (layer norm, RoPE in every layout, ops/logprobs.py, ops/routing.py)
 ROW_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
@@ -224,7 +224,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     for name, p in (("weight", weight), ("bias", bias)):
         if p is not None and (p.shape != (H,) or p.device != x.device):
             raise ValueError(f"layer_norm: {name} must be a [{H}] tensor on x's device")
-    if not (use_native(x) and x.dtype in ROW_DTYPES):
+    if not (use_native(x) and x.dtype in ROW_DTYPES) or forward_mode(x, weight, bias, residual):
         return layer_norm_reference(x, weight, bias, eps, residual)
     if H * x.element_size() > _LAYER_NORM_MAX_BYTES:
         raise ValueError(f"HIP layer norm needs rows of at most {_LAYER_NORM_MAX_BYTES} bytes (got {H} x {x.dtype})")
@@ -422,7 +422,7 @@ def apply_rope(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, n_rot_he
     if positions is None and S > cos.shape[0]:
         raise ValueError(f"apply_rope: {S} tokens, but tables for {cos.shape[0]} positions")
     learned = torch.is_grad_enabled() and (cos.requires_grad or sin.requires_grad)  # the kernels have no gradient for tables
-    if learned or not (use_native(qkv) and qkv.dtype in ROW_DTYPES):
+    if learned or not (use_native(qkv) and qkv.dtype in ROW_DTYPES) or forward_mode(qkv, cos, sin):
         return rope_reference(qkv, cos, sin, n_rot_heads, positions, interleaved, rotary_dim)
     if qkv.dim() != 4:
         raise ValueError(f"apply_rope: qkv must be [B, S, heads, D], got shape {tuple(qkv.shape)}")

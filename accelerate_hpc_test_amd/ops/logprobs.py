@@ -11,7 +11,7 @@ from typing import NamedTuple, Optional
 
 import torch
 
-from ._ext import ext, use_native
+from ._ext import ext, forward_mode, use_native
 from .fused import ROW_DTYPES
 
 MAX_TOP_K = 64  # alternatives per row on a GPU
@@ -69,7 +69,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0, t
     if not (temperature > 0 and math.isfinite(temperature)):
         raise ValueError(f"token_logprobs: temperature must be positive and finite, got {temperature}")
     tokens = tokens.to(torch.int64)
-    if not (use_native(logits) and logits.dtype in ROW_DTYPES):
+    if not (use_native(logits) and logits.dtype in ROW_DTYPES) or forward_mode(logits):
         return token_logprobs_reference(logits, tokens, top_k, temperature, ignore_index)
     if top_k > MAX_TOP_K:
         raise ValueError(f"HIP token_logprobs gives at most {MAX_TOP_K} alternatives (got top_k={top_k})")

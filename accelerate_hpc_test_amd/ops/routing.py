@@ -10,7 +10,7 @@ from typing import Optional
 
 import torch
 
-from ._ext import ext, use_native
+from ._ext import ext, forward_mode, use_native
 from .fused import ROW_DTYPES
 
 MAX_EXPERTS, MAX_TOP_K, MAX_GROUPS = 1024, 64, 64  # of the HIP kernel
@@ -72,7 +72,7 @@ def route_experts(logits: torch.Tensor, top_k: int, scoring: str = "softmax", bi
         if bias.shape != (E,) or bias.device != logits.device:
             raise ValueError(f"route_experts: bias must be a [{E}] tensor on the logits' device")
         bias = bias.detach()
-    if not (use_native(logits) and logits.dtype in ROW_DTYPES):
+    if not (use_native(logits) and logits.dtype in ROW_DTYPES) or forward_mode(logits):
         return route_experts_reference(logits, top_k, scoring, bias, n_groups, topk_groups, renormalize, scale)
     if E > MAX_EXPERTS or top_k > MAX_TOP_K or n_groups > MAX_GROUPS:
         raise ValueError(f"HIP route_experts takes at most {MAX_EXPERTS} experts, {MAX_TOP_K} choices and {MAX_GROUPS} groups "

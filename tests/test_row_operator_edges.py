@@ -7,8 +7,9 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 
-from accelerate_hpc_test_amd.ops import apply_rope, rope_tables, route_experts, token_logprobs
+from accelerate_hpc_test_amd.ops import apply_rope, layer_norm, rope_tables, route_experts, token_logprobs
 
 U = 2.0 ** -24
 BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
@@ -139,3 +140,51 @@ def test_rope_positions_outside_learned_tables():
     assert out[0, 0].isfinite().all() and out[0, 1:, 0, :8].isnan().all() and (out[0, :, 0, 8:] == 1).all() and (out[0, :, 1] == 1).all()
     (d,) = torch.autograd.grad(out[0, 0].sum(), cos)
     assert d.isfinite().all() and d[0].all() and not d[1:].any()
+
+
+def forward_mode_cases(device):
+    """(name, function of the differentiated inputs, those inputs) of each operator; every one in 32 bits, small and smooth."""
+    g = torch.Generator(device=device).manual_seed(6)
+    n = lambda *shape: torch.randn(*shape, generator=g, device=device)  # noqa: E731
+    tables = rope_tables(5, 8, 10000.0, device)
+    tokens = torch.tensor([1, 7, 0], device=device)
+    bias = torch.linspace(-0.1, 0.1, 12, device=device)
+    return [
+        ("layer_norm", lambda x, w, r: layer_norm(x, w, None, 1e-5, r), (n(3, 10), n(10), n(3, 10))),
+        ("rope halves", lambda x: (apply_rope(x, *tables, 2),), (n(1, 5, 3, 8),)),
+        ("rope pairs of a part", lambda x, c, s: (apply_rope(x, c, s, 2, interleaved=True, rotary_dim=8),), (n(1, 5, 3, 12), *tables)),
+        ("token_logprobs", lambda x: token_logprobs(x, tokens, top_k=2, temperature=0.8)[:3], (n(3, 9),)),
+        ("route_experts", lambda x: route_experts(x, 3, "sigmoid", bias, 4, 2)[:1], (n(4, 12),)),
+    ]
+
+
+@pytest.mark.parametrize("device", ON)
+@pytest.mark.parametrize("case", range(5))
+def test_forward_mode_tangents(device, case):
+    """A tangent on any input reaches the outputs, through dual numbers and through torch.func: J v of the forward mode equals u J v of the
+    reverse mode in 64 bits on the host (fp32 chains of at most 20 roundings, values below 100)."""
+    name, fn, inputs = forward_mode_cases(device)[case]
+    tangents = [torch.randn(t.shape, generator=torch.Generator().manual_seed(i)).to(device) for i, t in enumerate(inputs)]
+    fn64 = forward_mode_cases("cpu")[case][1]
+    _, want = torch.autograd.functional.jvp(fn64, tuple(t.double().cpu() for t in inputs), tuple(t.double().cpu() for t in tangents))
+    want = want if isinstance(want, tuple) else (want,)
+    for leaf in (False, True):
+        with fwAD.dual_level():
+            duals = [fwAD.make_dual(t.detach().requires_grad_(leaf), v) for t, v in zip(inputs, tangents)]
+            got = [fwAD.unpack_dual(o).tangent for o in fn(*duals)]
+        for a, b in zip(got, want):
+            assert a is not None and (a.cpu() - b).abs().max() < 20 * 100 * U, name
+    _, got = torch.func.jvp(fn, tuple(inputs), tuple(tangents))
+    for a, b in zip(got, want):
+        assert (a.cpu() - b).abs().max() < 20 * 100 * U, name
+    # torch.func.grad of a sum, against the reverse mode
+    plain = [t.detach().requires_grad_() for t in inputs]
+    rev = torch.autograd.grad(sum(o.sum() for o in fn(*plain)), plain, allow_unused=True)
+    fun = torch.func.grad(lambda *a: sum(o.sum() for o in fn(*a)), argnums=tuple(range(len(inputs))))(*inputs)
+    for a, b in zip(fun, rev):
+        assert (a - b).abs().max() < 20 * 100 * U, name
+    # one input alone has a tangent
+    with fwAD.dual_level():
+        duals = list(inputs)
+        duals[-1] = fwAD.make_dual(inputs[-1], tangents[-1])
+        assert fwAD.unpack_dual(fn(*duals)[0]).tangent is not None, name
