@@ -167,6 +167,21 @@ class LlamaDecoderLayer(nn.Module):
         return hidden, residual
 
 
+def rope_length(model, S: int, position_ids=None) -> Optional[int]:
+    """The length of the sequence that a forward's S tokens belong to, where the tables depend on it ("dynamic" scaling), else None. A shard
+    of a context- or sequence-parallel group counts the whole sequence; given positions count up to the furthest (read on the
+    host, as their frequencies are made there)."""
+    scaling = model.config.rope_scaling
+    if scaling is None or scaling.get("rope_type", scaling.get("type")) != "dynamic":
+        return None
+    if getattr(model, "_cp_seq_len", None):
+        return int(model._cp_seq_len)
+    shards = getattr(model, "_seq_parallel_factor", 1)
+    if shards > 1 or position_ids is None or position_ids.numel() == 0:
+        return S * shards
+    return int(position_ids.max()) + 1
+
+
 @dataclass
 class CausalLMOutput:
     loss: Optional[torch.Tensor] = None
@@ -206,11 +221,11 @@ class LlamaForCausalLM(nn.Module):
             elif isinstance(m, RMSNorm):
                 m.weight.fill_(1.0)
 
-    def _rope(self, S, device):
-        key = (S, str(device))
+    def _rope(self, S, device, length=None):
+        key = (S, str(device), length)
         if key not in self._rope_cache:
             n = max(S, self.config.max_position_embeddings if S > self.config.max_position_embeddings else S)
-            self._rope_cache[key] = rope_tables(n, self.config.rotary_dim, self.config.rope_theta, device, self.config.rope_scaling)
+            self._rope_cache[key] = rope_tables(n, self.config.rotary_dim, self.config.rope_theta, device, self.config.rope_scaling, length)
         return self._rope_cache[key]
 
     def forward(self, input_ids, labels=None, position_ids=None, attention_mask=None, return_logits: bool = True,
@@ -224,7 +239,8 @@ class LlamaForCausalLM(nn.Module):
         if position_ids is not None:
             rope_len = max(int(self.config.max_position_embeddings), getattr(self, "_cp_seq_len", None) or 0,
                            S * getattr(self, "_seq_parallel_factor", 1))
-        cos, sin = self._rope(rope_len, input_ids.device)
+        length = rope_length(self, S, position_ids)
+        cos, sin = self._rope(max(rope_len, length or 0), input_ids.device, length)
         h = self.embed_tokens(input_ids)
         dt = self.layers[0].self_attn.qkv_proj.weight.dtype if len(self.layers) else h.dtype
         if h.device.type in ("cuda", "cpu") and torch.is_autocast_enabled(h.device.type):

@@ -324,10 +324,12 @@ def _yarn_attention_factor(scaling):
     return of(scaling["factor"], m) / of(scaling["factor"], m_all) if m and m_all else of(scaling["factor"], 1.0)
 
 
-def rope_tables(seq_len: int, head_dim: int, theta: float = 500000.0, device=None, scaling: Optional[dict] = None):
+def rope_tables(seq_len: int, head_dim: int, theta: float = 500000.0, device=None, scaling: Optional[dict] = None,
+                length: Optional[int] = None):
     """fp32 cos/sin tables [S, D/2], the angles evaluated in 64 bits; D = `head_dim` is the rotated part of a head. `scaling`
     is a transformers-style `rope_scaling` dict with `rope_type` "llama3", "linear" (positions divided by `factor`),
-    "dynamic" (theta grown for `seq_len` tokens past `original_max_position_embeddings`) or "yarn"."""
+    "dynamic" (theta grown for a sequence of `length` tokens past `original_max_position_embeddings`) or "yarn". `length`: of the
+    sequence that the tables serve, where they have more or fewer rows than that; `seq_len` unless given."""
     inv = 1.0 / (theta ** (torch.arange(0, head_dim, 2, dtype=torch.float64, device="cpu") / head_dim))
     kind = None if scaling is None else scaling.get("rope_type", scaling.get("type"))
     amplitude = 1.0
@@ -346,9 +348,10 @@ def rope_tables(seq_len: int, head_dim: int, theta: float = 500000.0, device=Non
         inv = inv / scaling["factor"]
     elif kind == "dynamic":
         old = scaling["original_max_position_embeddings"]
-        if seq_len > old and head_dim > 2:
+        length = seq_len if length is None else length
+        if length > old and head_dim > 2:
             factor = scaling["factor"]
-            theta = theta * (factor * seq_len / old - (factor - 1)) ** (head_dim / (head_dim - 2))
+            theta = theta * (factor * length / old - (factor - 1)) ** (head_dim / (head_dim - 2))
             inv = 1.0 / (theta ** (torch.arange(0, head_dim, 2, dtype=torch.float64, device="cpu") / head_dim))
     elif kind == "yarn":
         inv = _yarn_inv_freq(inv, head_dim, theta, scaling)

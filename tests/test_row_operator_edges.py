@@ -188,3 +188,66 @@ def test_forward_mode_tangents(device, case):
         duals = list(inputs)
         duals[-1] = fwAD.make_dual(inputs[-1], tangents[-1])
         assert fwAD.unpack_dual(fn(*duals)[0]).tangent is not None, name
+
+
+# ------------------------------------------------------------------------------------------------ tables that follow a model's configuration
+def tiny_model(kind, scaling, device="cpu", **kw):
+    from accelerate_hpc_test_amd.models.llama import LlamaConfig, LlamaForCausalLM
+    from accelerate_hpc_test_amd.models.mixtral import MixtralConfig, MixtralForCausalLM
+
+    size = dict(vocab_size=64, hidden_size=128, intermediate_size=64, num_hidden_layers=1, num_attention_heads=2, num_key_value_heads=1,
+                max_position_embeddings=256, rope_theta=10000.0, rope_scaling=scaling) | kw
+    torch.manual_seed(0)
+    model = LlamaForCausalLM(LlamaConfig(**size)) if kind == "llama" else MixtralForCausalLM(MixtralConfig(num_local_experts=2, **size))
+    model.init_weights()
+    with torch.no_grad():
+        for p in model.parameters():
+            if p.dim() > 1:
+                p.mul_(10)  # attention that looks at positions
+    return model.to(device)
+
+
+@pytest.mark.parametrize("kind", ["llama", "mixtral"])
+@pytest.mark.parametrize("S", [32, 64, 65, 200])
+def test_dynamic_tables_go_by_the_sequence(kind, S):
+    """The same tokens at the same positions give the same logits whether the positions are passed or counted: theta grows with the
+    sequence's length, not with the number of rows of the tables that happen to be made."""
+    model = tiny_model(kind, {"rope_type": "dynamic", "factor": 4.0, "original_max_position_embeddings": 64})
+    ids = torch.randint(0, 64, (2, S), generator=torch.Generator().manual_seed(1))
+    plain = tiny_model(kind, None)
+    with torch.no_grad():
+        want = model(ids).logits
+        assert torch.equal(model(ids, position_ids=torch.arange(S).expand(2, S)).logits, want)
+        assert torch.equal(want, plain(ids).logits) == (S <= 64)
+
+
+@pytest.mark.parametrize("shards", ["context parallel", "sequence parallel"])
+def test_dynamic_tables_of_a_shard_are_those_of_the_whole_sequence(shards):
+    """A rank that holds half of a sequence takes theta from all of it: its queries and keys are those of the single process."""
+    S, half = 200, 100
+    model = tiny_model("llama", {"rope_type": "dynamic", "factor": 4.0, "original_max_position_embeddings": 64})
+    seen = []
+    model.layers[0].self_attn.attention_impl = lambda qkv, n_q, n_kv: (seen.append(qkv), qkv[:, :, :n_q])[1]
+    ids = torch.randint(0, 64, (1, S), generator=torch.Generator().manual_seed(1))
+    with torch.no_grad():
+        model(ids)
+        for lo in (0, half):
+            pos = torch.arange(lo, lo + half)[None]
+            if shards == "context parallel":
+                model._cp_position_ids, model._cp_seq_len = pos, S
+                model(ids[:, lo : lo + half])
+            else:
+                model._seq_parallel_factor = 2
+                model(ids[:, lo : lo + half], position_ids=pos)
+    # products of one shape and another: fp32 sums of 128 terms
+    for got, lo in zip(seen[1:], (0, half)):
+        assert (got - seen[0][:, lo : lo + half]).abs().max() < 2 * 128 * U * seen[0].abs().max()
+
+
+def test_dynamic_tables_take_the_length_apart_from_their_rows():
+    scaling = {"rope_type": "dynamic", "factor": 2.0, "original_max_position_embeddings": 16}
+    for length in (8, 16, 40):
+        long = rope_tables(64, 8, 10000.0, scaling=scaling, length=length)
+        short = rope_tables(length, 8, 10000.0, scaling=scaling)
+        assert all(torch.equal(a[:length], b) for a, b in zip(long, short)) and long[0].shape == (64, 4)
+    assert torch.equal(rope_tables(64, 8, 10000.0, length=3)[0], rope_tables(64, 8, 10000.0)[0])
