@@ -167,6 +167,21 @@ class LlamaDecoderLayer(nn.Module):
         return hidden, residual
 
 
+def rope_scaling(cfg: LlamaConfig) -> Optional[dict]:
+    """`cfg.rope_scaling` with what may be left out of it: the original length is `max_position_embeddings` unless named, and YaRN's
+    factor the ratio of both."""
+    scaling = cfg.rope_scaling
+    kind = None if scaling is None else scaling.get("rope_type", scaling.get("type"))
+    if kind not in ("dynamic", "yarn"):
+        return scaling
+    scaling = dict(scaling)
+    if scaling.get("original_max_position_embeddings") is None:
+        scaling["original_max_position_embeddings"] = cfg.max_position_embeddings
+    if kind == "yarn" and scaling.get("factor") is None:
+        scaling["factor"] = cfg.max_position_embeddings / scaling["original_max_position_embeddings"]
+    return scaling
+
+
 def rope_length(model, S: int, position_ids=None) -> Optional[int]:
     """The length of the sequence that a forward's S tokens belong to, where the tables depend on it ("dynamic" scaling), else None. A shard
     of a context- or sequence-parallel group counts the whole sequence; given positions count up to the furthest (read on the
@@ -225,7 +240,7 @@ class LlamaForCausalLM(nn.Module):
         key = (S, str(device), length)
         if key not in self._rope_cache:
             n = max(S, self.config.max_position_embeddings if S > self.config.max_position_embeddings else S)
-            self._rope_cache[key] = rope_tables(n, self.config.rotary_dim, self.config.rope_theta, device, self.config.rope_scaling, length)
+            self._rope_cache[key] = rope_tables(n, self.config.rotary_dim, self.config.rope_theta, device, rope_scaling(self.config), length)
         return self._rope_cache[key]
 
     def forward(self, input_ids, labels=None, position_ids=None, attention_mask=None, return_logits: bool = True,

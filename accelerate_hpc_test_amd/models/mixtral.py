@@ -16,7 +16,7 @@ import torch
 import torch.nn as nn
 
 from ..ops.fused import cross_entropy, rope_tables
-from .llama import CausalLMOutput, LlamaAttention, LlamaConfig, RMSNorm, rope_length
+from .llama import CausalLMOutput, LlamaAttention, LlamaConfig, RMSNorm, rope_length, rope_scaling
 from .moe import MoEExperts, MoELayer, load_balancing_loss
 
 
@@ -146,7 +146,7 @@ class MixtralForCausalLM(nn.Module):
     def _rope(self, S, device, length=None):
         key = (S, str(device), length)
         if key not in self._rope_cache:
-            self._rope_cache[key] = rope_tables(S, self.config.rotary_dim, self.config.rope_theta, device, self.config.rope_scaling, length)
+            self._rope_cache[key] = rope_tables(S, self.config.rotary_dim, self.config.rope_theta, device, rope_scaling(self.config), length)
         return self._rope_cache[key]
 
     def forward(self, input_ids, labels=None, position_ids=None, attention_mask=None, return_logits: bool = True,

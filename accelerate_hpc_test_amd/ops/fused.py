@@ -332,6 +332,11 @@ def rope_tables(seq_len: int, head_dim: int, theta: float = 500000.0, device=Non
     sequence that the tables serve, where they have more or fewer rows than that; `seq_len` unless given."""
     inv = 1.0 / (theta ** (torch.arange(0, head_dim, 2, dtype=torch.float64, device="cpu") / head_dim))
     kind = None if scaling is None else scaling.get("rope_type", scaling.get("type"))
+    needs = {"linear": ("factor",), "dynamic": ("factor", "original_max_position_embeddings"),
+             "yarn": ("factor", "original_max_position_embeddings")}
+    missing = [k for k in needs.get(kind, ()) if scaling.get(k) is None]
+    if missing:
+        raise ValueError(f"rope_tables: {kind} scaling needs {' and '.join(missing)}")
     amplitude = 1.0
     if kind == "llama3":
         factor = scaling["factor"]

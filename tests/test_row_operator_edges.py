@@ -251,3 +251,32 @@ def test_dynamic_tables_take_the_length_apart_from_their_rows():
         short = rope_tables(length, 8, 10000.0, scaling=scaling)
         assert all(torch.equal(a[:length], b) for a, b in zip(long, short)) and long[0].shape == (64, 4)
     assert torch.equal(rope_tables(64, 8, 10000.0, length=3)[0], rope_tables(64, 8, 10000.0)[0])
+
+
+@pytest.mark.parametrize("kind", ["llama", "mixtral"])
+@pytest.mark.parametrize("name", ["rope_type", "type"])
+@pytest.mark.parametrize("scaling,same_as", [
+    ({"kind": "dynamic", "factor": 2.0}, {"kind": "dynamic", "factor": 2.0, "original_max_position_embeddings": 64}),
+    ({"kind": "yarn", "factor": 4.0}, {"kind": "yarn", "factor": 4.0, "original_max_position_embeddings": 64}),
+    ({"kind": "yarn", "factor": 4.0, "original_max_position_embeddings": None},
+     {"kind": "yarn", "factor": 4.0, "original_max_position_embeddings": 64}),
+    ({"kind": "yarn", "factor": None, "original_max_position_embeddings": 16},
+     {"kind": "yarn", "factor": 4.0, "original_max_position_embeddings": 16}),
+])
+def test_scaling_without_the_original_length(kind, name, scaling, same_as):
+    """Configurations that name no original length mean max_position_embeddings by it; YaRN without a factor means the ratio of both."""
+    ids = torch.randint(0, 64, (1, 100), generator=torch.Generator().manual_seed(1))
+    logits = []
+    for s in (scaling, same_as):
+        s = {name if k == "kind" else k: v for k, v in s.items()}
+        with torch.no_grad():
+            logits.append(tiny_model(kind, s, max_position_embeddings=64)(ids).logits)
+    assert torch.equal(*logits)
+
+
+@pytest.mark.parametrize("scaling,key", [({"rope_type": "linear"}, "factor"), ({"rope_type": "dynamic", "factor": 2.0}, "original"),
+                                         ({"rope_type": "yarn", "factor": 2.0}, "original"), ({"rope_type": "dynamic"}, "factor"),
+                                         ({"type": "yarn", "original_max_position_embeddings": 8}, "factor")])
+def test_rope_tables_name_what_a_scaling_lacks(scaling, key):
+    with pytest.raises(ValueError, match=key):
+        rope_tables(16, 8, 10000.0, scaling=scaling)
