@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import math
 import os
+import warnings
 from typing import Optional
 
 import torch
@@ -337,6 +338,8 @@ def rope_tables(seq_len: int, head_dim: int, theta: float = 500000.0, device=Non
     missing = [k for k in needs.get(kind, ()) if scaling.get(k) is None]
     if missing:
         raise ValueError(f"rope_tables: {kind} scaling needs {' and '.join(missing)}")
+    if kind not in (None, "default", "llama3", *needs):
+        warnings.warn(f"rope_tables: the scaling {kind!r} is not known, the tables are not scaled", stacklevel=2)
     amplitude = 1.0
     if kind == "llama3":
         factor = scaling["factor"]

@@ -4,6 +4,7 @@ tables and routing that follow a configuration. CPU and GPU unless a test says w
 tolerances' terms are those of test_row_operators.py."""
 
 import math
+import warnings
 
 import pytest
 import torch
@@ -280,3 +281,14 @@ def test_scaling_without_the_original_length(kind, name, scaling, same_as):
 def test_rope_tables_name_what_a_scaling_lacks(scaling, key):
     with pytest.raises(ValueError, match=key):
         rope_tables(16, 8, 10000.0, scaling=scaling)
+
+
+def test_rope_tables_warn_about_a_scaling_they_do_not_know():
+    plain = rope_tables(16, 8, 10000.0)
+    with pytest.warns(UserWarning, match="ntk"):
+        got = rope_tables(16, 8, 10000.0, scaling={"type": "ntk", "factor": 2.0})
+    assert all(torch.equal(a, b) for a, b in zip(got, plain))
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        for scaling in ({"rope_type": "default"}, {"rope_type": None, "factor": 2.0}, {"type": "linear", "factor": 2.0}):
+            rope_tables(16, 8, 10000.0, scaling=scaling)
