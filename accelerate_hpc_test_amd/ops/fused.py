@@ -415,7 +415,7 @@ def apply_rope(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, n_rot_he
     (or [1, S], [S] for every batch row), each token's row of the tables; None counts from 0. The tables lie on qkv's device, the
     positions there or on the host. The result is a new contiguous tensor. On a GPU any strides and even R are taken, in bf16,
     fp16 and fp32, with D up to 1000; a position outside the tables gives NaN in its rotated values. Tables that require
-    gradients get them, from plain torch operations."""
+    gradients get them, and 64-bit tables are used as such, in torch operations."""
     S, Htot, D = qkv.shape[-3:]
     R = D if rotary_dim is None else rotary_dim
     if R < 2 or R % 2 or R > D:
@@ -432,8 +432,9 @@ def apply_rope(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, n_rot_he
         positions = positions.to(qkv.device)
     if positions is None and S > cos.shape[0]:
         raise ValueError(f"apply_rope: {S} tokens, but tables for {cos.shape[0]} positions")
-    learned = torch.is_grad_enabled() and (cos.requires_grad or sin.requires_grad)  # the kernels have no gradient for tables
-    if learned or not (use_native(qkv) and qkv.dtype in ROW_DTYPES) or forward_mode(qkv, cos, sin):
+    # the kernels read 32-bit tables, and have no gradient for them
+    torch_tables = torch.float64 in (cos.dtype, sin.dtype) or (torch.is_grad_enabled() and (cos.requires_grad or sin.requires_grad))
+    if torch_tables or not (use_native(qkv) and qkv.dtype in ROW_DTYPES) or forward_mode(qkv, cos, sin):
         return rope_reference(qkv, cos, sin, n_rot_heads, positions, interleaved, rotary_dim)
     if qkv.dim() != 4:
         raise ValueError(f"apply_rope: qkv must be [B, S, heads, D], got shape {tuple(qkv.shape)}")

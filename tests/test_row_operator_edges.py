@@ -292,3 +292,21 @@ def test_rope_tables_warn_about_a_scaling_they_do_not_know():
         warnings.simplefilter("error")
         for scaling in ({"rope_type": "default"}, {"rope_type": None, "factor": 2.0}, {"type": "linear", "factor": 2.0}):
             rope_tables(16, 8, 10000.0, scaling=scaling)
+
+
+@pytest.mark.parametrize("device", ON)
+@pytest.mark.parametrize("dtype,D,R,interleaved", ROPE_FORMS + [(FP16, 12, 12, False)])
+def test_rope_tables_in_64_bits_are_used_in_64_bits(device, dtype, D, R, interleaved):
+    """One rounding, to the input's type: half a step of it and 2 roundings of 64 bits, where 32-bit tables are off by up to 6 U more."""
+    S = 50
+    angle = torch.outer(torch.arange(S, dtype=torch.float64), 10000.0 ** (-torch.arange(0, R, 2, dtype=torch.float64) / R)).to(device)
+    cos, sin = angle.cos(), angle.sin()
+    x = torch.randn(2, S, 4, D, generator=torch.Generator(device=device).manual_seed(7), device=device).to(dtype)
+    out = apply_rope(x, cos, sin, 3, interleaved=interleaved, rotary_dim=R)
+    want = x.double()
+    a, b = (x[:, :, :3, o].double() for o in ((slice(0, R, 2), slice(1, R, 2)) if interleaved else (slice(0, R // 2), slice(R // 2, R))))
+    c, s = cos[:, None], sin[:, None]
+    for o, v in zip((slice(0, R, 2), slice(1, R, 2)) if interleaved else (slice(0, R // 2), slice(R // 2, R)), (a * c - b * s, b * c + a * s)):
+        want[:, :, :3, o] = v
+    tol = torch.finfo(dtype).eps / 2 * want.abs() + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps + 2.0 ** -50
+    assert out.dtype == dtype and ((out.double() - want).abs() <= tol).all()
