@@ -408,13 +408,13 @@ def rope_reference(qkv, cos, sin, n_rot_heads, positions=None, interleaved=False
 
 def apply_rope(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, n_rot_heads: int, positions=None,
                interleaved: bool = False, rotary_dim: Optional[int] = None):
-    """qkv: [B, S, Htot, D]; rotates the first `n_rot_heads` heads (Q heads then K heads) by the fp32 tables cos / sin
+    """qkv: [..., S, Htot, D]; rotates the first `n_rot_heads` heads (Q heads then K heads) by the fp32 tables cos / sin
     [positions, R/2] of `rope_tables`, in half pairs (i, i + R/2) or, `interleaved`, pairs (2i, 2i + 1).
 
-    `rotary_dim`: R, the rotated first values of each head, even; None rotates the whole head. `positions`: integers [B, S]
+    `rotary_dim`: R, the rotated first values of each head, even; None rotates the whole head. `positions`: integers [..., S]
     (or [1, S], [S] for every batch row), each token's row of the tables; None counts from 0. The tables lie on qkv's device, the
     positions there or on the host. The result is a new contiguous tensor. On a GPU any strides and even R are taken, in bf16,
-    fp16 and fp32, with D up to 1000; a position outside the tables gives NaN in its rotated values. Tables that require
+    fp16 and fp32, with D up to 1000 (whole heads in halves: any D); a position outside the tables gives NaN in its rotated values. Tables that require
     gradients get them, and 64-bit tables are used as such, in torch operations."""
     S, Htot, D = qkv.shape[-3:]
     R = D if rotary_dim is None else rotary_dim
@@ -436,21 +436,24 @@ def apply_rope(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, n_rot_he
     torch_tables = torch.float64 in (cos.dtype, sin.dtype) or (torch.is_grad_enabled() and (cos.requires_grad or sin.requires_grad))
     if torch_tables or not (use_native(qkv) and qkv.dtype in ROW_DTYPES) or forward_mode(qkv, cos, sin):
         return rope_reference(qkv, cos, sin, n_rot_heads, positions, interleaved, rotary_dim)
-    if qkv.dim() != 4:
-        raise ValueError(f"apply_rope: qkv must be [B, S, heads, D], got shape {tuple(qkv.shape)}")
     # bf16 heads rotated whole in halves have their own kernel (csrc/kernels/norm_act.hip), which copies V heads in the same pass
     whole = qkv.dtype == torch.bfloat16 and D % 8 == 0 and R == D and not interleaved
-    if D > 1000 and not whole:
+    if D > 1000 and not whole:  # wider than a block of the other kernel
+        if R == D and not interleaved:
+            return rope_reference(qkv, cos, sin, n_rot_heads, positions)
         raise ValueError(f"HIP rope needs a head size of at most 1000 (got {D})")
-    B = qkv.shape[0]
+    lead = qkv.shape[:-3]
+    B = math.prod(lead)
     if positions is None:
         cos, sin = cos[:S], sin[:S]  # one row per token of the sequence
     if positions is not None and not (positions.dtype == torch.int64 and positions.shape == (B, S)):
-        positions = positions.reshape(B, S) if positions.numel() == B * S else positions.expand(B, S)
+        positions = positions.reshape(B, S) if positions.numel() == B * S else positions.expand(*lead, S).reshape(B, S)
         positions = positions.to(torch.int64)
     if cos.dtype != torch.float32 or sin.dtype != torch.float32:
         cos, sin = cos.float(), sin.float()
-    return ext().rope(qkv, cos.contiguous(), sin.contiguous(), positions, n_rot_heads, interleaved, whole)
+    x = qkv if len(lead) == 1 else qkv.reshape(B, S, Htot, D)
+    out = ext().rope(x, cos.contiguous(), sin.contiguous(), positions, n_rot_heads, interleaved, whole)
+    return out if len(lead) == 1 else out.view(qkv.shape)
 
 
 # ----------------------------------------------------------------------------------------------------------

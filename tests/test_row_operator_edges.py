@@ -310,3 +310,46 @@ def test_rope_tables_in_64_bits_are_used_in_64_bits(device, dtype, D, R, interle
         want[:, :, :3, o] = v
     tol = torch.finfo(dtype).eps / 2 * want.abs() + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps + 2.0 ** -50
     assert out.dtype == dtype and ((out.double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("device", ON)
+@pytest.mark.parametrize("dtype,D,R,interleaved", ROPE_FORMS)
+@pytest.mark.parametrize("lead", [(), (2,), (2, 3), (2, 1, 3)])
+def test_rope_of_any_number_of_dimensions(device, dtype, D, R, interleaved, lead):
+    """[..., S, heads, D] is the same rotation for every leading index; positions broadcast against [..., S]."""
+    S = 5
+    g = torch.Generator(device=device).manual_seed(8)
+    cos, sin = rope_tables(9, R, 10000.0, device)
+    x = torch.randn(*lead, S, 4, D, generator=g, device=device).to(dtype)
+    dy = torch.randn(x.shape, generator=g, device=device).to(dtype)
+    kw = dict(interleaved=interleaved, rotary_dim=R)
+    n = math.prod(lead)
+    every = torch.randint(0, 9, (*lead, S), generator=g, device=device)
+    shapes = [None, every, every[..., :1, :] if len(lead) > 1 else every[:1] if lead else every, torch.arange(S, device=device) + 2]
+    for pos in shapes:
+        flat = None if pos is None else pos.expand(*lead, S).reshape(n, S)
+        ref_leaf = x.reshape(n, S, 4, D).detach().requires_grad_()
+        want = apply_rope(ref_leaf, cos, sin, 3, flat, **kw)
+        (dwant,) = torch.autograd.grad(want, ref_leaf, dy.reshape(n, S, 4, D))
+        leaf = x.detach().requires_grad_()
+        got = apply_rope(leaf, cos, sin, 3, pos, **kw)
+        (dgot,) = torch.autograd.grad(got, leaf, dy)
+        assert got.shape == dgot.shape == x.shape and torch.equal(got.reshape(want.shape), want) and torch.equal(dgot.reshape(want.shape), dwant)
+
+
+@pytest.mark.parametrize("device", ON)
+@pytest.mark.parametrize("dtype,D", [(FP32, 1002), (FP32, 1024), (FP16, 2048), (BF16, 1004), (BF16, 1024)])
+def test_rope_of_wide_whole_heads(device, dtype, D):
+    S = 3
+    g = torch.Generator(device=device).manual_seed(9)
+    cos, sin = rope_tables(S, D, 10000.0, device)
+    x = torch.randn(2, S, 2, D, generator=g, device=device).to(dtype).requires_grad_()
+    y = apply_rope(x, cos, sin, 1)
+    a, b = x.detach()[:, :, :1].double().chunk(2, -1)
+    c, s = cos[:, None].double(), sin[:, None].double()
+    want = torch.cat([torch.cat([a * c - b * s, b * c + a * s], -1), x.detach()[:, :, 1:].double()], 2)
+    size = torch.cat([torch.cat([a.abs() + b.abs()] * 2, -1), torch.zeros_like(x.detach()[:, :, 1:])], 2)
+    fi = torch.finfo(dtype)
+    tol = (want.abs() + 3 * U * size) * fi.eps / 2 + 3 * U * size + fi.smallest_normal * fi.eps  # a rounding, and 3 U of the pair in fp32
+    assert ((y.double() - want).abs() <= tol).all()
+    assert torch.autograd.grad(y.sum(), x)[0].isfinite().all()
