@@ -426,34 +426,43 @@ def apply_rope(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, n_rot_he
         raise ValueError(f"apply_rope: {n_rot_heads} of {Htot} heads to rotate")
     if cos.device != qkv.device or sin.device != qkv.device:
         raise ValueError(f"apply_rope: cos and sin must be on qkv's device ({qkv.device}), got {cos.device}, {sin.device}")
-    if positions is not None and positions.device != qkv.device:
-        if positions.device.type != "cpu":
+    lead = qkv.shape[:-3]
+    whole = qkv.dtype == torch.bfloat16 and D % 8 == 0 and R == D and not interleaved
+    if positions is not None:
+        if positions.is_floating_point() or positions.is_complex() or positions.dtype == torch.bool:
+            raise TypeError(f"apply_rope: positions must be integers, got {positions.dtype}")
+        if positions.device != qkv.device and positions.device.type != "cpu":
             raise ValueError(f"apply_rope: positions must be on qkv's device ({qkv.device}) or the host, got {positions.device}")
-        positions = positions.to(qkv.device)
+        positions = positions.to(qkv.device, torch.int64)
+        want = (*lead, S)
+        if positions.shape != want:
+            if positions.dim() <= len(want) and all(p in (1, w) for p, w in zip(positions.shape[::-1], want[::-1])):
+                positions = positions.expand(want)
+            elif positions.numel() == math.prod(want) and (positions.dim() == 1 or (whole and qkv.is_cuda)):
+                positions = positions.reshape(want)  # a token after the other
+            else:
+                raise ValueError(f"apply_rope: positions must be {want}, or broadcast to it, got {tuple(positions.shape)}")
     if positions is None and S > cos.shape[0]:
         raise ValueError(f"apply_rope: {S} tokens, but tables for {cos.shape[0]} positions")
     # the kernels read 32-bit tables, and have no gradient for them
     torch_tables = torch.float64 in (cos.dtype, sin.dtype) or (torch.is_grad_enabled() and (cos.requires_grad or sin.requires_grad))
     if torch_tables or not (use_native(qkv) and qkv.dtype in ROW_DTYPES) or forward_mode(qkv, cos, sin):
         return rope_reference(qkv, cos, sin, n_rot_heads, positions, interleaved, rotary_dim)
-    # bf16 heads rotated whole in halves have their own kernel (csrc/kernels/norm_act.hip), which copies V heads in the same pass
-    whole = qkv.dtype == torch.bfloat16 and D % 8 == 0 and R == D and not interleaved
+    # `whole`: bf16 heads rotated whole in halves have their own kernel (csrc/kernels/norm_act.hip), which copies V heads in the same pass
     if D > 1000 and not whole:  # wider than a block of the other kernel
         if R == D and not interleaved:
             return rope_reference(qkv, cos, sin, n_rot_heads, positions)
         raise ValueError(f"HIP rope needs a head size of at most 1000 (got {D})")
-    lead = qkv.shape[:-3]
-    B = math.prod(lead)
     if positions is None:
         cos, sin = cos[:S], sin[:S]  # one row per token of the sequence
-    if positions is not None and not (positions.dtype == torch.int64 and positions.shape == (B, S)):
-        positions = positions.reshape(B, S) if positions.numel() == B * S else positions.expand(*lead, S).reshape(B, S)
-        positions = positions.to(torch.int64)
     if cos.dtype != torch.float32 or sin.dtype != torch.float32:
         cos, sin = cos.float(), sin.float()
-    x = qkv if len(lead) == 1 else qkv.reshape(B, S, Htot, D)
-    out = ext().rope(x, cos.contiguous(), sin.contiguous(), positions, n_rot_heads, interleaved, whole)
-    return out if len(lead) == 1 else out.view(qkv.shape)
+    cos, sin = cos.contiguous(), sin.contiguous()
+    if len(lead) == 1:
+        return ext().rope(qkv, cos, sin, positions, n_rot_heads, interleaved, whole)
+    B = math.prod(lead)
+    positions = None if positions is None else positions.reshape(B, S)
+    return ext().rope(qkv.reshape(B, S, Htot, D), cos, sin, positions, n_rot_heads, interleaved, whole).view(qkv.shape)
 
 
 # ----------------------------------------------------------------------------------------------------------

@@ -353,3 +353,29 @@ def test_rope_of_wide_whole_heads(device, dtype, D):
     tol = (want.abs() + 3 * U * size) * fi.eps / 2 + 3 * U * size + fi.smallest_normal * fi.eps  # a rounding, and 3 U of the pair in fp32
     assert ((y.double() - want).abs() <= tol).all()
     assert torch.autograd.grad(y.sum(), x)[0].isfinite().all()
+
+
+@pytest.mark.parametrize("device", ON)
+@pytest.mark.parametrize("dtype,D,R,interleaved", ROPE_FORMS)
+def test_rope_positions_are_integers_of_a_fitting_shape(device, dtype, D, R, interleaved):
+    B, S = 2, 3
+    cos, sin = rope_tables(8, R, 10000.0, device)
+    x = torch.randn(B, S, 4, D, generator=torch.Generator(device=device).manual_seed(10), device=device).to(dtype)
+    rope = lambda p: apply_rope(x, cos, sin, 3, p, interleaved=interleaved, rotary_dim=R)  # noqa: E731
+    pos = torch.tensor([[0, 5, 7], [3, 1, 2]], device=device)
+    want = rope(pos)
+    for kind in (torch.int32, torch.int16, torch.int8, torch.uint8):
+        assert torch.equal(rope(pos.to(kind)), want)
+    assert torch.equal(rope(pos.reshape(-1)), want)  # a token after the other
+    assert torch.equal(rope(pos[:, :1]), rope(pos[:, :1].expand(B, S)))
+    for bad in (pos.float(), pos.half(), pos > 2, pos.to(torch.complex64)):
+        with pytest.raises(TypeError, match="integers"):
+            rope(bad)
+    for bad in (pos.new_zeros(B, S + 1), pos.new_zeros(3, S), pos.new_zeros(4), pos.new_zeros(1, B, S), pos.new_zeros(0)):
+        if bad.numel() == B * S:
+            continue  # taken as [B, S]
+        with pytest.raises(ValueError, match="positions"):
+            rope(bad)
+    if (dtype, D, R, interleaved) != (BF16, 16, 16, False) or device == "cpu":  # whole bf16 heads have taken any shape of B * S elements
+        with pytest.raises(ValueError, match="positions"):
+            rope(pos.t())
