@@ -104,19 +104,29 @@ Tensor rope_by(const Tensor& x, const Tensor& cos, const Tensor& sin, const OptT
                   x.size(3), sign);
 }
 
+// The gradient turns back (`sign`). It is a rotation itself, and heads that are rotated whole in halves, which torch operations
+// rotated before there were kernels for them, can be differentiated again as those can; the other forms once.
 struct Rope : public torch::autograd::Function<Rope> {
   static Tensor forward(AutogradContext* ctx, const Tensor& qkv, const Tensor& cos, const Tensor& sin, const OptTensor& pos,
-                        int64_t n_rot, bool interleaved, bool whole) {
+                        int64_t n_rot, bool interleaved, bool whole, double sign) {
     ctx->save_for_backward({cos, sin, pos.value_or(Tensor())});
     ctx->saved_data["n_rot"] = n_rot;
     ctx->saved_data["form"] = (int64_t)((interleaved ? 1 : 0) | (whole ? 2 : 0));
-    return rope_by(qkv, cos, sin, pos, n_rot, interleaved, whole, 1.0);
+    ctx->saved_data["sign"] = sign;
+    return rope_by(qkv, cos, sin, pos, n_rot, interleaved, whole, sign);
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const auto saved = ctx->get_saved_variables();
     const int64_t form = ctx->saved_data["form"].toInt();
-    const Tensor d = rope_by(g[0], saved[0], saved[1], some(saved[2]), ctx->saved_data["n_rot"].toInt(), form & 1, form & 2, -1.0);
-    return once({d, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()});
+    const int64_t n_rot = ctx->saved_data["n_rot"].toInt();
+    const double sign = -ctx->saved_data["sign"].toDouble();
+    const bool again = !(form & 1) && 2 * saved[0].size(1) == g[0].size(-1);
+    if (again && at::GradMode::is_enabled() && g[0].requires_grad())
+      return {Rope::apply(g[0], saved[0], saved[1], some(saved[2]), n_rot, false, (form & 2) != 0, sign), Tensor(), Tensor(), Tensor(),
+              Tensor(), Tensor(), Tensor(), Tensor()};
+    variable_list d = {rope_by(g[0], saved[0], saved[1], some(saved[2]), n_rot, form & 1, form & 2, sign), Tensor(), Tensor(), Tensor(),
+                       Tensor(), Tensor(), Tensor(), Tensor()};
+    return again ? d : once(std::move(d));
   }
 };
 
@@ -197,7 +207,7 @@ std::vector<Tensor> layer_norm(const Tensor& x, const OptTensor& w, const OptTen
 
 Tensor rope(const Tensor& qkv, const Tensor& cos, const Tensor& sin, const OptTensor& pos, int64_t n_rot, bool interleaved,
             bool whole) {
-  if (at::GradMode::is_enabled() && qkv.requires_grad()) return Rope::apply(qkv, cos, sin, pos, n_rot, interleaved, whole);
+  if (at::GradMode::is_enabled() && qkv.requires_grad()) return Rope::apply(qkv, cos, sin, pos, n_rot, interleaved, whole, 1.0);
   return rope_by(qkv, cos, sin, pos, n_rot, interleaved, whole, 1.0);
 }
 

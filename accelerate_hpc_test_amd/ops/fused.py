@@ -415,7 +415,8 @@ def apply_rope(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, n_rot_he
     (or [1, S], [S] for every batch row), each token's row of the tables; None counts from 0. The tables lie on qkv's device, the
     positions there or on the host. The result is a new contiguous tensor. On a GPU any strides and even R are taken, in bf16,
     fp16 and fp32, with D up to 1000 (whole heads in halves: any D); a position outside the tables gives NaN in its rotated values. Tables that require
-    gradients get them, and 64-bit tables are used as such, in torch operations."""
+    gradients get them, and 64-bit tables are used as such, in torch operations. On a GPU heads rotated whole in halves can be
+    differentiated any number of times, the other forms once."""
     S, Htot, D = qkv.shape[-3:]
     R = D if rotary_dim is None else rotary_dim
     if R < 2 or R % 2 or R > D:

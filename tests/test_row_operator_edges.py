@@ -379,3 +379,27 @@ def test_rope_positions_are_integers_of_a_fitting_shape(device, dtype, D, R, int
     if (dtype, D, R, interleaved) != (BF16, 16, 16, False) or device == "cpu":  # whole bf16 heads have taken any shape of B * S elements
         with pytest.raises(ValueError, match="positions"):
             rope(pos.t())
+
+
+@pytest.mark.parametrize("device", ON)
+@pytest.mark.parametrize("dtype,D", [(BF16, 16), (BF16, 12), (FP16, 16), (FP32, 16), (FP32, 6)])
+def test_rope_of_whole_heads_is_differentiable_again(device, dtype, D):
+    """The rotation is linear: its gradient turns back, the gradient of that turns forth, any number of times; and where the incoming gradient
+    is a constant, so is the outgoing one, which a loss may add to others."""
+    g = torch.Generator(device=device).manual_seed(11)
+    x, dy, v = (torch.randn(2, 3, 4, D, generator=g, device=device).to(dtype) for _ in range(3))
+    tables = rope_tables(3, D, 10000.0, device)
+    leaf, dleaf, vleaf = (t.clone().requires_grad_() for t in (x, dy, v))
+    y = apply_rope(leaf, *tables, 3)
+    (plain,) = torch.autograd.grad(y, leaf, dy, retain_graph=True)
+    (d,) = torch.autograd.grad(y, leaf, dleaf, create_graph=True)
+    assert torch.equal(d, plain)
+    (dd,) = torch.autograd.grad(d, dleaf, vleaf, create_graph=True)
+    assert torch.equal(dd, apply_rope(v, *tables, 3))
+    (ddd,) = torch.autograd.grad(dd, vleaf, dy)
+    assert torch.equal(ddd, plain)
+    y = apply_rope(leaf, *tables, 3)
+    (d,) = torch.autograd.grad(y, leaf, dy, create_graph=True)
+    assert not d.requires_grad and torch.equal(d, plain)
+    (d.float().square().sum() + leaf.float().sum()).backward()
+    assert torch.equal(leaf.grad, torch.ones_like(leaf))
