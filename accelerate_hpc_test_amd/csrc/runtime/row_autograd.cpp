@@ -46,7 +46,9 @@ Tensor rows_of(const Tensor& t) {
   Tensor r = t.reshape({rows, width});
   return last_contiguous(r) ? r : r.contiguous();
 }
-Tensor shaped(const Tensor& t, at::IntArrayRef sizes) { return t.sizes() == sizes ? t : t.view(sizes); }
+// `t`, which nothing else holds, in another shape. No view of it: outputs of a node with several must not be changed in place if
+// they are views that were made inside of it.
+Tensor shaped(const Tensor& t, at::IntArrayRef sizes) { return t.sizes() == sizes ? t : at::_unsafe_view(t, sizes); }
 
 // Gradients of a backward that runs to be differentiated again: whoever does that gets an error, not a zero.
 variable_list once(variable_list grads) {

@@ -403,3 +403,42 @@ def test_rope_of_whole_heads_is_differentiable_again(device, dtype, D):
     assert not d.requires_grad and torch.equal(d, plain)
     (d.float().square().sum() + leaf.float().sum()).backward()
     assert torch.equal(leaf.grad, torch.ones_like(leaf))
+
+
+@pytest.mark.parametrize("device", ON)
+@pytest.mark.parametrize("train", [False, True])
+def test_outputs_may_be_changed_in_place(device, train):
+    """Outputs of every shape are tensors of their own, not views of a node's inner ones: in-place changes work and differentiate."""
+    g = torch.Generator(device=device).manual_seed(12)
+    n = lambda *shape: torch.randn(*shape, generator=g, device=device)  # noqa: E731
+    for shape in ((12, 8), (3, 4, 8), (8,), (2, 3, 2, 8)):
+        x, res = n(*shape).requires_grad_(train), n(*shape).requires_grad_(train)
+        mask = torch.rand(shape[:-1], generator=g, device=device)
+        y, s = layer_norm(x, None, None, 1e-5, res)
+        want = y.detach() * 2
+        y.mul_(2)
+        assert torch.equal(y, want) and not y._is_view()
+        tokens = torch.randint(0, 8, shape[:-1], generator=g, device=device)
+        r = token_logprobs(x, tokens, top_k=2)
+        want = [r.logprobs.detach() * mask, r.entropy.detach() * mask, r.top_logprobs.detach() + 1]
+        r.logprobs.mul_(mask)
+        r.entropy.mul_(mask)
+        r.top_logprobs.add_(1)
+        assert all(torch.equal(a, b) for a, b in zip(r, want)) and not any(t._is_view() for t in r)
+        if train:
+            plain = token_logprobs(x, tokens, top_k=2)
+            a = torch.autograd.grad(r.logprobs.sum() + r.entropy.sum() + r.top_logprobs.sum(), x)[0]
+            b = torch.autograd.grad((plain.logprobs * mask).sum() + (plain.entropy * mask).sum() + plain.top_logprobs.sum(), x)[0]
+            assert torch.equal(a, b)
+            ya, yb = y, layer_norm(x, None, None, 1e-5, res)[0] * 2
+            assert torch.equal(*(torch.autograd.grad(t.sum(), res)[0] for t in (ya, yb)))
+    # the residual stream, where its norm is not differentiated
+    x, res = n(2, 3, 8).requires_grad_(train), n(2, 3, 8)
+    _, s = layer_norm(x, None, None, 1e-5, res)
+    want = s.detach() + 1
+    assert torch.equal(s.add_(1), want) and not s._is_view()
+    # choices and weights
+    w, ids = route_experts(n(6, 8).requires_grad_(train), 2)
+    want = w.detach() * 3
+    assert torch.equal(w.mul_(3), want)
+    ids.add_(1)
