@@ -211,8 +211,12 @@ __device__ __forceinline__ bool choose(const float (&f)[V], const float* __restr
     }
     const bool in = g < a.groups && above < a.top_groups;
     if constexpr (!kWide) {
+      // A rating is off by its two keys' errors, each of the key's own size (large keys of opposite signs make a small rating), and by
+      // one rounding. An infinite one is exact.
+      float off = size > 1 ? key_margin(first, noise) + key_margin(second, noise) + fabsf(rating) * 0x1p-23f : key_margin(first, noise);
+      off = wave_reduce<OpMax>(g < a.groups && fabsf(rating) < INFINITY ? off : 0.f);
       const float worst = -wave_reduce<OpMax>(in ? -rating : -INFINITY), best = wave_reduce<OpMax>(g < a.groups && !in ? rating : -INFINITY);
-      if (!(worst - best > 2.f * (key_margin(worst, noise) + key_margin(best, noise)))) return false;
+      if (!(worst - best > 2.f * off)) return false;
     }
     const uint64_t open = __ballot(in);
     const float inv = 1.f / (float)size;

@@ -442,3 +442,30 @@ def test_outputs_may_be_changed_in_place(device, train):
     want = w.detach() * 3
     assert torch.equal(w.mul_(3), want)
     ids.add_(1)
+
+
+@pytest.mark.parametrize("device", ON)
+@pytest.mark.parametrize("B", [0.5, 16.0, 100.0, 1000.0, 20000.0])
+@pytest.mark.parametrize("size", [2, 5])
+def test_route_experts_groups_whose_best_keys_cancel(device, B, size):
+    """Ratings that are small sums of large keys of opposite signs: 32 bits round each key at its own size. The choice of the group, and of the
+    expert in it, is that of 64 bits for ratings a few steps apart."""
+    rows, E = 3000, 2 * size
+    g = torch.Generator().manual_seed(int(B) + size)
+    x = torch.randn(rows, E, generator=g, dtype=torch.float64)
+    x[0, :2], x[0, size : size + 2] = torch.tensor([-0.78342849, 0.03163768]), torch.tensor([0.68000275, -1.67503536])
+    bias = torch.zeros(E)
+    bias[0], bias[1] = B, -B
+    bias[2:size] = bias[size + 2 :] = -4 * B - 4  # never among a group's two best
+    s = torch.sigmoid(x)
+    target = (s[1:, 0] + s[1:, 1] - s[1:, size]).clamp(0.02, 0.98)
+    near = torch.randn(rows - 1, generator=g, dtype=torch.float64) * 2.0**-22 * max(B, 1.0)
+    x[1:, size + 1] = torch.log(target / (1 - target)) + near
+    x = x.float().to(device)
+    bias = bias.to(device)
+    w, ids = route_experts(x, 1, "sigmoid", bias, 2, 1, renormalize=False)
+    key = torch.sigmoid(x.double()) + bias.double()
+    rating = torch.topk(key.view(rows, 2, size), 2, dim=-1)[0].sum(-1)
+    group = (rating[:, 1] > rating[:, 0]).long()
+    want = key.view(rows, 2, size).argmax(-1).gather(1, group[:, None]) + group[:, None] * size
+    assert torch.equal(ids, want) and 0 < group.sum() < rows
