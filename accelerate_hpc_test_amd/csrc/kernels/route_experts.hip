@@ -29,6 +29,7 @@ namespace {
 
 constexpr int kMaxExperts = 1024, kMaxTop = 64, kMaxGroups = 64;
 constexpr int kThreads = 256;
+constexpr float kNoScore = -103.972077f;  // ln 2^-150: the sigmoid of a logit below it is 0 in 32 bits
 
 struct RouteArgs {
   long rows, stride;
@@ -317,9 +318,11 @@ __global__ __launch_bounds__(kThreads) void route_fwd_kernel(const T* __restrict
     choose<V, double>(f, bias, sh, false, a);
   }
 
-  // The weights, a choice in each lane. Shares are of the chosen alone: a softmax needs no sum over all experts for them.
+  // The weights, a choice in each lane. Shares are of the chosen alone, formed against the largest logit among them: that may lie any
+  // distance below the row's, where a bias or closed groups keep others out.
   const int id = lane < a.k ? sh.chosen[lane] : 0;
   const float v = to_f<T>(x[id]);
+  const float top = a.renorm ? wave_reduce<OpMax>(lane < a.k ? v : -INFINITY) : 0.f;
   float w;
   if (a.softmax) {
     float hi = f[0];
@@ -330,16 +333,19 @@ __global__ __launch_bounds__(kThreads) void route_fwd_kernel(const T* __restrict
 #pragma unroll
     for (int i = 0; i < V; ++i) all += exp_of(f[i] - hi);
     all = wave_reduce<OpSum>(all);
-    w = lane < a.k ? exp_of(v - hi) : 0.f;
+    // chosen scores that are all zero share nothing: 0, not 0 / 0
+    const bool none = a.renorm && top == -INFINITY;
+    w = lane < a.k && !none ? exp_of(v - (a.renorm ? top : hi)) : 0.f;
     const float sum = a.renorm ? wave_reduce<OpSum>(w) : all;
-    w = all == all ? w / fmaxf(sum, 1.17549435e-38f) : NAN;
+    w = all == all ? (none ? 0.f : w / sum) : NAN;
+  } else if (a.renorm) {
+    // s_j over the best score, up to a factor that all share: e^(v - min(top, 0)) / (1 + e^v)
+    const bool none = top < kNoScore && !__any(lane < a.k && v != v);
+    w = lane < a.k && !none ? (v > 0.f ? sigmoid_of(v) : exp_of(v - fminf(top, 0.f)) / (1.f + exp_of(v))) : 0.f;
+    const float sum = wave_reduce<OpSum>(w);
+    w = none ? 0.f : w / sum;
   } else {
     w = lane < a.k ? sigmoid_of(v) : 0.f;
-    if (a.renorm) {
-      const float sum = wave_reduce<OpSum>(w);
-      // scores that are all zero share nothing: 0, not 0 / 0
-      w = sum == sum ? w / fmaxf(sum, 1.17549435e-38f) : NAN;
-    }
   }
   if (lane < a.k) {
     weights[row * a.k + lane] = w * a.scale;

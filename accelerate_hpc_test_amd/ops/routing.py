@@ -14,7 +14,8 @@ from ._ext import ext, forward_mode, use_native
 from .fused import ROW_DTYPES
 
 MAX_EXPERTS, MAX_TOP_K, MAX_GROUPS = 1024, 64, 64  # of the HIP kernel
-_TINY = torch.finfo(torch.float32).tiny
+# the sigmoid of a logit below this is 0 in the type: half the smallest number, 2^-150 or 2^-1075
+_NO_SCORE = {torch.float32: -150 * math.log(2), torch.float64: -1075 * math.log(2)}
 
 
 def route_experts_reference(logits, top_k, scoring="softmax", bias=None, n_groups=1, topk_groups=1, renormalize=True, scale=1.0):
@@ -40,9 +41,17 @@ def route_experts_reference(logits, top_k, scoring="softmax", bias=None, n_group
             ids = order.gather(1, torch.sort(shut.to(torch.int8), dim=-1, stable=True)[1])[:, :top_k]
         else:
             ids = torch.sort(key, dim=-1, descending=True, stable=True)[1][:, :top_k]
-    w = score.gather(1, ids)
-    if renormalize:
-        w = w / w.sum(-1, keepdim=True).clamp_min(_TINY)
+    if not renormalize:
+        return score.gather(1, ids) * scale, ids
+    # Shares in logarithms: the chosen scores may lie any distance below the largest. Scores that are all zero share nothing.
+    v = x.gather(1, ids)
+    top = v.detach().amax(-1, keepdim=True)
+    none = top == -math.inf if scoring == "softmax" else top < _NO_SCORE[x.dtype]
+    v = torch.where(none, torch.zeros_like(v), v)
+    w = torch.softmax(v if scoring == "softmax" else torch.nn.functional.logsigmoid(v), -1)
+    w = torch.where(none, torch.zeros_like(w), w)
+    if scoring == "softmax":  # a row without a distribution
+        w = torch.where(score.detach().sum(-1, keepdim=True).isnan(), torch.full_like(w, math.nan), w)
     return w * scale, ids
 
 
@@ -53,7 +62,7 @@ def route_experts(logits: torch.Tensor, top_k: int, scoring: str = "softmax", bi
     Scores are softmax(logits) or sigmoid(logits) (`scoring`). Experts are chosen by score + `bias` ([E], optional: it steers the
     choice alone, balances the load, and gets no gradient), within the `topk_groups` of `n_groups` equal groups whose two best
     keys have the largest sum; equal keys go to the lower index, keys are compared in 64 bits. Weights are the chosen scores,
-    divided by their sum (`renormalize`), times `scale`. Returns (weights fp32 [T, k], experts int64 [T, k]) in falling order of
+    divided by their sum (`renormalize`; scores that are all 0 in 32 bits give 0), times `scale`. Returns (weights fp32 [T, k], experts int64 [T, k]) in falling order of
     the keys; the weights are differentiable with respect to the logits."""
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise ValueError(f"route_experts: logits must be [tokens, experts], got shape {tuple(logits.shape)}")

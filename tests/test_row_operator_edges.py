@@ -469,3 +469,61 @@ def test_route_experts_groups_whose_best_keys_cancel(device, B, size):
     group = (rating[:, 1] > rating[:, 0]).long()
     want = key.view(rows, 2, size).argmax(-1).gather(1, group[:, None]) + group[:, None] * size
     assert torch.equal(ids, want) and 0 < group.sum() < rows
+
+
+@pytest.mark.parametrize("device", ON)
+@pytest.mark.parametrize("dtype", [FP32, BF16, FP16])
+@pytest.mark.parametrize("scoring,depth", [("softmax", 0.0), ("softmax", 90.0), ("softmax", 200.0), ("softmax", 30000.0), ("sigmoid", 0.0),
+                                           ("sigmoid", 40.0), ("sigmoid", 85.0), ("sigmoid", 92.0), ("sigmoid", 98.0)])
+@pytest.mark.parametrize("by", ["bias", "groups"])
+def test_route_experts_shares_of_experts_far_below_the_largest_logit(device, dtype, scoring, depth, by):
+    """Where a bias, or closed groups, keep the largest logits out, the chosen scores may lie far below 32 bits' range; their shares do not. By
+    the definition in 64 bits, in logarithms: share = exp(ln s_j) / sum exp(ln s). Errors: exponents of up to 8 below the best
+    chosen one, rounded (8 * 1.5 U), and the sums and quotient counted as for other shares."""
+    E, k, rows = 12, 3, 40
+    g = torch.Generator().manual_seed(int(depth))
+    x = 2 * torch.randn(rows, E, generator=g).clamp(-2, 2)
+    x[:, 4:] -= depth
+    x = x.to(dtype).to(device)
+    bias = torch.zeros(E, device=device)
+    if by == "bias":
+        bias[:4] = -4.0
+        args = (bias,)
+    else:
+        bias[:8] = -4.0  # the last group's rating is the best
+        args = (bias, 3, 1)
+    leaf = x.detach().requires_grad_()
+    w, ids = route_experts(leaf, k, scoring, *args, scale=1.5)
+    assert (ids >= (8 if by == "groups" else 4)).all()
+    u = torch.randn(rows, k, generator=g).to(device)
+    (dx,) = torch.autograd.grad(w, leaf, u)
+    v = x.double().gather(1, ids).requires_grad_()
+    share = torch.softmax(v if scoring == "softmax" else torch.nn.functional.logsigmoid(v), -1)
+    n = (40 + k + 12) * U
+    assert ((w - 1.5 * share.detach()).abs() <= n * 1.5 * share.detach()).all()
+    (dv,) = torch.autograd.grad(1.5 * share, v, u.double())
+    want = torch.zeros_like(dx, dtype=torch.float64).scatter_(1, ids, dv)
+    size = 1.5 * share.detach() * (u.abs().double() + (u.abs() * share.detach()).sum(-1, keepdim=True))
+    tol = torch.zeros_like(want).scatter_(1, ids, 2 * n * size) + torch.finfo(dtype).eps / 2 * want.abs() * (1 + 2**-7) + torch.finfo(dtype).tiny
+    assert ((dx.double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("device", ON)
+def test_route_experts_shares_of_scores_that_are_zero(device):
+    """Chosen experts without any score share nothing: 0, no NaN, and no gradient; a row without a distribution stays NaN."""
+    bias = torch.tensor([-9.0, 0.0, 0.0, 0.0], device=device)
+    x = torch.full((3, 4), -math.inf, device=device)
+    x[0, 0] = 1.0
+    x[1] = torch.tensor([1.0, -math.inf, 0.5, -math.inf], device=device)
+    leaf = x.requires_grad_()
+    w, ids = route_experts(leaf, 2, "softmax", bias)
+    assert not w[0].any() and w[1].tolist() == [1.0, 0.0] and ids[1, 0] == 2 and w[2].isnan().all()
+    d = torch.autograd.grad(w[:2].sum(), leaf)[0]
+    assert not d[:2].any()
+    leaf = torch.tensor([[0.0, -105.0, -104.5, -120.0], [0.0, -103.5, -103.5, -math.inf], [0.0, -3e38, -math.inf, -3e38],
+                         [0.0, math.nan, -200.0, math.nan]], device=device).requires_grad_()
+    w, ids = route_experts(leaf, 2, "sigmoid", bias)
+    assert not w[0].any() and w[1].tolist() == [0.5, 0.5] and not w[2].any()
+    assert route_experts(leaf[3:], 3, "sigmoid", bias[:4])[0].isnan().all()  # a poisoned choice
+    d = torch.autograd.grad((w[:3] * w[:3]).sum(), leaf)[0]
+    assert not d[0].any() and not d[2].any() and d.isfinite().all()
