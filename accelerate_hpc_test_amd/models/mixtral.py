@@ -174,11 +174,13 @@ class MixtralForCausalLM(nn.Module):
             loss = cross_entropy(logits, shift_labels, ignore_index=-100, inplace_backward=not return_logits)
             want_aux = self.config.output_router_logits if output_router_logits is None else output_router_logits
             if want_aux and self.config.router_aux_loss_coef > 0:
-                aux = load_balancing_loss([l.block_sparse_moe.last_router_logits for l in self.layers],
-                                          self.config.num_local_experts, self.config.num_experts_per_tok)
+                routers = [l.block_sparse_moe for l in self.layers]
+                choices = None if all(r.plain_routing for r in routers) else [r.last_router_choice for r in routers]
+                aux = load_balancing_loss([r.last_router_logits for r in routers], self.config.num_local_experts,
+                                          self.config.num_experts_per_tok, choices, self.config.router_scoring)
                 loss = loss + self.config.router_aux_loss_coef * aux.to(loss.dtype)
         for l in self.layers:
-            l.block_sparse_moe.last_router_logits = None
+            l.block_sparse_moe.last_router_logits = l.block_sparse_moe.last_router_choice = None
         return CausalLMOutput(loss=loss, logits=logits if return_logits else None)
 
     @torch.no_grad()

@@ -525,6 +525,7 @@ class MoELayer(nn.Module):
         self.experts = MoEExperts(num_experts, hidden, intermediate)
         self.ep_group = None
         self.last_router_logits = None
+        self.last_router_choice = None  # the experts [T, k], where they are not the plain top-k of the logits' softmax
         # optional per-expert selection bias (DeepSeek-V3-style aux-loss-free balancing): shifts which experts are
         # chosen, not the combine weights; None = plain top-k of the router softmax (Mixtral)
         self.router_bias: Optional[torch.Tensor] = None
@@ -562,6 +563,7 @@ class MoELayer(nn.Module):
         logits = self.gate(t)
         self.last_router_logits = logits
         w, idx = self._route(logits)
+        self.last_router_choice = None if self.plain_routing else idx
         w = w.to(t.dtype)
         flat_e = idx.reshape(-1)
         if self.ep_group is None or comm.group_size(self.ep_group) == 1:
@@ -597,9 +599,14 @@ class MoELayer(nn.Module):
         out = torch.zeros_like(t).index_add_(0, src_tok, y_sorted * w_sorted.unsqueeze(-1))
         return out.view(shape)
 
+    @property
+    def plain_routing(self) -> bool:
+        """Mixtral's form: the top-k of the softmax, with or without a bias."""
+        return self.scoring == "softmax" and self.topk_groups == self.n_groups and self.scale == 1.0
+
     def _route(self, logits):
         """Weights (fp32) and experts [T, k] of the router's logits."""
-        if self.scoring != "softmax" or self.topk_groups != self.n_groups or self.scale != 1.0:
+        if not self.plain_routing:
             bias = None if self.router_bias is None else self.router_bias.to(logits.device)
             return route_experts(logits, self.top_k, self.scoring, bias, self.n_groups, self.topk_groups, self.norm_topk, self.scale)
         probs = torch.softmax(logits.float(), dim=-1)
@@ -664,11 +671,16 @@ def _attach_bounds(seg):
     return seg
 
 
-def load_balancing_loss(router_logits: list, num_experts: int, top_k: int) -> torch.Tensor:
-    """Switch-style auxiliary loss (HF `load_balancing_loss_func`): E · Σ_e f_e · P_e over all layers' tokens."""
+def load_balancing_loss(router_logits: list, num_experts: int, top_k: int, choices: Optional[list] = None,
+                        scoring: str = "softmax") -> torch.Tensor:
+    """Switch-style auxiliary loss (HF `load_balancing_loss_func`): E · Σ_e f_e · P_e over all layers' tokens. `choices`: the experts
+    [T, k] that each layer's router chose, where that is not the plain top-k of its softmax; P is of its scores, summed to 1."""
     logits = torch.cat([l.float() for l in router_logits], 0)
-    probs = torch.softmax(logits, -1)
-    _, sel = torch.topk(probs, top_k, -1)
+    if scoring == "softmax":
+        probs = torch.softmax(logits, -1)
+    else:
+        probs = torch.softmax(F.logsigmoid(logits), -1)  # sigmoid scores over their sum
+    sel = torch.topk(probs, top_k, -1)[1] if choices is None else torch.cat(choices, 0)
     mask = F.one_hot(sel, num_experts).float()  # [T, k, E]
     tokens_per_expert = mask.mean(0)  # [k, E]
     prob_per_expert = probs.mean(0)  # [E]

@@ -527,3 +527,69 @@ def test_route_experts_shares_of_scores_that_are_zero(device):
     assert route_experts(leaf[3:], 3, "sigmoid", bias[:4])[0].isnan().all()  # a poisoned choice
     d = torch.autograd.grad((w[:3] * w[:3]).sum(), leaf)[0]
     assert not d[0].any() and not d[2].any() and d.isfinite().all()
+
+
+# -------------------------------------------------------------------------------------------------------------- the experts' layer
+ROUTERS = [dict(router_scoring="sigmoid"), dict(router_scoring="sigmoid", router_n_groups=4, router_topk_groups=2, routed_scaling_factor=2.5),
+           dict(router_n_groups=4, router_topk_groups=1), dict(routed_scaling_factor=2.0)]
+
+
+@pytest.mark.parametrize("device", ON)
+@pytest.mark.parametrize("router", ROUTERS)
+@pytest.mark.parametrize("bias", [False, True])
+def test_auxiliary_loss_counts_the_experts_that_were_chosen(device, router, bias):
+    """E sum_e f_e P_e with f of the choices that the layers made (closed groups and the bias left out) and P of the router's own scores, summed
+    to 1, against the definition in 64 bits."""
+    from accelerate_hpc_test_amd.models.mixtral import MixtralConfig, MixtralForCausalLM
+
+    E, k, coef = 8, 2, 0.5
+    cfg = MixtralConfig(vocab_size=64, hidden_size=256, intermediate_size=256, num_hidden_layers=2, num_attention_heads=2,
+                        num_key_value_heads=1, max_position_embeddings=128, num_local_experts=E, num_experts_per_tok=k,
+                        output_router_logits=True, router_aux_loss_coef=coef, **router)
+    torch.manual_seed(0)
+    model = MixtralForCausalLM(cfg)
+    model.init_weights()
+    model = model.to(device, BF16 if device == "cuda" else FP32)
+    taken = []
+    for layer in model.layers:
+        moe = layer.block_sparse_moe
+        with torch.no_grad():
+            moe.gate.weight.mul_(20)
+        if bias:
+            moe.router_bias = torch.tensor([-9.0, 0, 0, 0, 0, 0, 0, 0.1], device=device)
+        moe._route = lambda logits, route=moe._route: (taken.append((logits, route(logits))), taken[-1][1])[1]
+    ids = torch.randint(0, 64, (1, 128), generator=torch.Generator().manual_seed(2)).to(device)
+    with_aux = model(ids, labels=ids).loss
+    choices = torch.cat([t[1][1] for t in taken])
+    logits = torch.cat([t[0] for t in taken]).detach().double()
+    score = torch.sigmoid(logits) if cfg.router_scoring == "sigmoid" else torch.softmax(logits, -1)
+    P = (score / score.sum(-1, keepdim=True)).mean(0)
+    f = torch.zeros(E, dtype=torch.float64, device=device).scatter_add_(0, choices.reshape(-1), torch.ones_like(choices.reshape(-1), dtype=torch.float64))
+    want = E * (f / choices.shape[0] * P).sum()
+    if bias:
+        assert not (choices == 0).any()
+    if cfg.router_topk_groups < cfg.router_n_groups:
+        assert max(len(set((row // 2).tolist())) for row in choices) <= cfg.router_topk_groups
+    got_aux = (with_aux - model(ids, labels=ids, output_router_logits=False).loss) / coef
+    # 256 tokens' scores in fp32, and a difference of two losses near 5
+    assert abs(got_aux.item() - want.item()) < 64 * U * want.item() + 8 * U * abs(with_aux.item()) / coef
+    for layer in model.layers:
+        assert layer.block_sparse_moe.last_router_logits is None and layer.block_sparse_moe.last_router_choice is None
+
+
+@pytest.mark.parametrize("device", ON)
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_auxiliary_loss_gradient(device, scoring):
+    from accelerate_hpc_test_amd.models.moe import load_balancing_loss
+
+    T, E, k = 30, 8, 2
+    g = torch.Generator(device=device).manual_seed(13)
+    x = [torch.randn(T, E, generator=g, device=device).requires_grad_() for _ in range(2)]
+    ids = [torch.randint(0, E, (T, k), generator=g, device=device) for _ in range(2)]
+    got = torch.autograd.grad(load_balancing_loss(x, E, k, ids, scoring), x)
+    wide = [t.detach().double().requires_grad_() for t in x]
+    s = torch.cat(wide).softmax(-1) if scoring == "softmax" else torch.cat(wide).sigmoid()
+    f = torch.nn.functional.one_hot(torch.cat(ids), E).double().sum(1).mean(0)
+    want = torch.autograd.grad(E * (f * (s / s.sum(-1, keepdim=True)).mean(0)).sum(), wide)
+    for a, b in zip(got, want):  # some 20 roundings, of values up to E * k / (2 T) before they cancel
+        assert (a - b).abs().max() < 20 * U * E * k / (2 * T) * 4
