@@ -25,8 +25,9 @@ class TokenLogprobs(NamedTuple):
 
 
 def token_logprobs_reference(logits, tokens, top_k=0, temperature=1.0, ignore_index=-100):
-    acc = logits if logits.dtype == torch.float64 else logits.float()
     counts = tokens != ignore_index
+    acc = logits if logits.dtype == torch.float64 else logits.float()
+    acc = torch.where(counts.unsqueeze(-1), acc, torch.zeros_like(acc))  # ignored rows are not read: they may hold anything
     named = (tokens >= 0) & (tokens < logits.shape[-1])
     z = acc / temperature
     logp = torch.log_softmax(z, dim=-1)

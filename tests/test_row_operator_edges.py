@@ -593,3 +593,22 @@ def test_auxiliary_loss_gradient(device, scoring):
     want = torch.autograd.grad(E * (f * (s / s.sum(-1, keepdim=True)).mean(0)).sum(), wide)
     for a, b in zip(got, want):  # some 20 roundings, of values up to E * k / (2 T) before they cancel
         assert (a - b).abs().max() < 20 * U * E * k / (2 * T) * 4
+
+
+@pytest.mark.parametrize("device", ON)
+@pytest.mark.parametrize("V", [50, 70001])
+@pytest.mark.parametrize("poison", [-math.inf, math.inf, math.nan])
+def test_token_logprobs_ignored_rows_carry_no_gradient_whatever_they_hold(device, V, poison):
+    """Padding may hold anything: zero outputs and a zero gradient, to the other rows' exact results."""
+    x = torch.randn(3, V, generator=torch.Generator(device=device).manual_seed(14), device=device)
+    x[1] = poison
+    tokens = torch.tensor([1, -100, 2], device=device)
+    leaf = x.requires_grad_()
+    r = token_logprobs(leaf, tokens, top_k=3)
+    assert r.logprobs[1] == 0 and r.entropy[1] == 0 and not r.top_logprobs[1].any() and (r.top_tokens[1] == -1).all()
+    (d,) = torch.autograd.grad(r.logprobs.sum() + r.entropy.sum() + r.top_logprobs.sum(), leaf)
+    assert not d[1].any()
+    rest = x.detach()[[0, 2]].requires_grad_()
+    s = token_logprobs(rest, tokens[[0, 2]], top_k=3)
+    (want,) = torch.autograd.grad(s.logprobs.sum() + s.entropy.sum() + s.top_logprobs.sum(), rest)
+    assert torch.equal(d[[0, 2]], want) and torch.equal(r.logprobs[[0, 2]], s.logprobs) and torch.equal(r.entropy[[0, 2]], s.entropy)
