@@ -23,7 +23,8 @@ using namespace acc;
 namespace {
 
 constexpr float kLn2 = 0.693147180559945309417f;
-constexpr float kFar = -1e30f;  // stands for -inf where it is multiplied with a probability of 0
+constexpr float kFar = -256.f;  // stands for all exponents below it where they are multiplied with 2^t, which is 0 there: finite, and
+                                // small enough for a product with any gradient
 constexpr int kMaxTop = 64;
 constexpr int kList = 2048;  // candidates of a row kept in shared memory
 constexpr int kMaxParts = 8;  // slices of a row

@@ -612,3 +612,28 @@ def test_token_logprobs_ignored_rows_carry_no_gradient_whatever_they_hold(device
     s = token_logprobs(rest, tokens[[0, 2]], top_k=3)
     (want,) = torch.autograd.grad(s.logprobs.sum() + s.entropy.sum() + s.top_logprobs.sum(), rest)
     assert torch.equal(d[[0, 2]], want) and torch.equal(r.logprobs[[0, 2]], s.logprobs) and torch.equal(r.entropy[[0, 2]], s.entropy)
+
+
+@pytest.mark.parametrize("device", ON)
+@pytest.mark.parametrize("g_ent", [1.0, 1e9, 1e12, 1e30])
+@pytest.mark.parametrize("T", [1.0, 1e-3])
+def test_token_logprobs_large_entropy_gradients_beside_impossible_tokens(device, g_ent, T):
+    """dlogits = -p dH (ln p + H) / T is 0 where p is, however large dH is: a scaled loss over rows with -inf and far logits. Bounds as for
+    other gradients: sums of 90 terms, exponents d = |x - b| / T rounded (d U relative, at most 20 where p counts)."""
+    g = torch.Generator(device=device).manual_seed(15)
+    x = torch.randn(5, 90, generator=g, device=device) * (1.0 if T == 1.0 else T)
+    x[:, 3::4] = -math.inf
+    x[1, 5] = -1e4
+    x[2, 6] = torch.finfo(FP32).min
+    x[3, 1:] = -math.inf
+    leaf = x.requires_grad_()
+    tokens = torch.zeros(5, dtype=torch.int64, device=device)
+    (d,) = torch.autograd.grad(token_logprobs(leaf, tokens, temperature=T).entropy, leaf, torch.full((5,), g_ent, device=device))
+    z = x.detach().double() / T
+    lp = torch.log_softmax(z, -1)
+    p = lp.exp()
+    fin = torch.where(p > 0, lp, torch.zeros_like(lp))
+    H = -(p * fin).sum(-1, keepdim=True)
+    want = -p * g_ent * (fin + H) / T
+    tol = U * (90 + 40) * p * g_ent * (fin.abs() + H + 1) / T
+    assert ((d - want).abs() <= tol).all() and not d[x == -math.inf].any()
