@@ -51,7 +51,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0, t
                    ignore_index: int = -100) -> TokenLogprobs:
     """log softmax(logits / temperature) at `tokens`, the entropy of that distribution, and its `top_k` best alternatives.
 
-    logits [..., V] in bf16, fp16 or fp32; tokens: integers [...]. All outputs are fp32 and differentiable with respect to the
+    logits [..., V] in bf16, fp16 or fp32; tokens: integers [...]; temperature: 2^-100 to 2^100. All outputs are fp32 and differentiable with respect to the
     logits (the alternatives at their chosen tokens). Rows whose token is `ignore_index` give 0, 0, 0 and -1 and no gradient;
     a token outside [0, V) gives a NaN log-probability that carries no gradient. The backward reads the logits again: beside
     `cross_entropy` on the same logits, give that `inplace_backward=False`. Logits of -inf are impossible tokens: probability 0,
@@ -67,8 +67,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0, t
         raise TypeError(f"token_logprobs: tokens must be integers, got {tokens.dtype}")
     if not 0 <= top_k <= V:
         raise ValueError(f"token_logprobs: top_k must be within the vocabulary ({top_k} of {V})")
-    if not (temperature > 0 and math.isfinite(temperature)):
-        raise ValueError(f"token_logprobs: temperature must be positive and finite, got {temperature}")
+    if not 2.0**-100 <= temperature <= 2.0**100:  # its quotient with any logit difference that counts is held in 32 bits
+        raise ValueError(f"token_logprobs: temperature must be within 2^-100 and 2^100, got {temperature}")
     tokens = tokens.to(torch.int64)
     if not (use_native(logits) and logits.dtype in ROW_DTYPES) or forward_mode(logits):
         return token_logprobs_reference(logits, tokens, top_k, temperature, ignore_index)

@@ -75,8 +75,8 @@ def route_experts(logits: torch.Tensor, top_k: int, scoring: str = "softmax", bi
         raise ValueError(f"route_experts: {topk_groups} of {n_groups} groups over {E} experts")
     if not 1 <= top_k <= E // n_groups * topk_groups:
         raise ValueError(f"route_experts: top_k={top_k} of {E // n_groups * topk_groups} experts within reach")
-    if not (math.isfinite(scale) and scale != 0):
-        raise ValueError(f"route_experts: scale must be finite and not zero, got {scale}")
+    if not 2.0**-60 <= abs(scale) <= 2.0**60:  # shares down to 2^-60 and gradients up to 2^60 stay within 32 bits
+        raise ValueError(f"route_experts: scale must be between 2^-60 and 2^60 in size, got {scale}")
     if bias is not None:
         if bias.shape != (E,) or bias.device != logits.device:
             raise ValueError(f"route_experts: bias must be a [{E}] tensor on the logits' device")

@@ -637,3 +637,33 @@ def test_token_logprobs_large_entropy_gradients_beside_impossible_tokens(device,
     want = -p * g_ent * (fin + H) / T
     tol = U * (90 + 40) * p * g_ent * (fin.abs() + H + 1) / T
     assert ((d - want).abs() <= tol).all() and not d[x == -math.inf].any()
+
+
+@pytest.mark.parametrize("device", ON)
+def test_temperatures_and_scales_that_32_bits_hold(device):
+    """The whole documented range of temperatures gives the distribution's limits; what lies outside of it is refused, and so are scales of
+    routing weights that 32 bits cannot carry."""
+    x = torch.tensor([[0.0, 1.0, 3.0, -math.inf], [5.0, 5.0, 4.0, 1.0]], device=device).requires_grad_()
+    tokens = torch.tensor([2, 0], device=device)
+    r = token_logprobs(x, tokens, top_k=2, temperature=2.0**100)
+    n = torch.tensor([3.0, 4.0], dtype=torch.float64)
+    assert (r.logprobs.cpu() + n.log()).abs().max() < 8 * U and (r.entropy.cpu() - n.log()).abs().max() < 8 * U
+    assert torch.autograd.grad(r.logprobs.sum() + r.entropy.sum(), x)[0].abs().max() < 2.0**-99
+    r = token_logprobs(x, tokens, top_k=2, temperature=2.0**-100)
+    assert r.logprobs[0] == 0 and abs(r.logprobs[1].item() + math.log(2)) < 4 * U and r.entropy[0] == 0
+    assert abs(r.entropy[1].item() - math.log(2)) < 4 * U and r.top_tokens.tolist() == [[2, 1], [0, 1]]
+    assert torch.autograd.grad(r.logprobs.sum() + r.entropy.sum(), x)[0].isfinite().all()
+    for bad in (2.0**-101, 2.0**101, 1e-39, 1e39, 1e300, 5e-324):
+        with pytest.raises(ValueError, match="temperature"):
+            token_logprobs(x, tokens, temperature=bad)
+    logits = torch.tensor([[0.0, 1.0, 3.0]], device=device).requires_grad_()
+    plain, ids = route_experts(logits, 2)
+    for scale in (2.0**-60, 2.0**60, -2.0):
+        w, _ = route_experts(logits, 2, scale=scale)
+        assert torch.equal(w, plain * scale)
+        (d,) = torch.autograd.grad(w[0, 0] / scale, logits, retain_graph=True)
+        (want,) = torch.autograd.grad(plain[0, 0], logits, retain_graph=True)
+        assert (d - want).abs().max() < 16 * U
+    for bad in (2.0**-61, 2.0**61, 1e-50, 1e300, math.inf, math.nan, 0.0):
+        with pytest.raises(ValueError, match="scale"):
+            route_experts(logits, 2, scale=bad)
