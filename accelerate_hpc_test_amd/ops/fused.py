@@ -214,7 +214,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     Returns (y, residual_out) where residual_out = s in x's type, as `rms_norm` does (s is what is normalised), or x itself.
 
     x and residual: one shape and one type (bf16, fp16 or fp32), any strides; weight / bias: [hidden], each optional, in x's
-    type or fp32. Statistics and the weight's gradient sums are fp32. On a GPU the row takes at most 64 KiB."""
+    type or fp32 (another type enters in fp32). Statistics and the weight's gradient sums are fp32. On a GPU the row takes at most 64 KiB."""
     H = x.shape[-1] if x.dim() else 0
     if H < 1:
         raise ValueError(f"layer_norm: x must have a last dimension to normalise, got shape {tuple(x.shape)}")
@@ -229,9 +229,9 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
         return layer_norm_reference(x, weight, bias, eps, residual)
     if H * x.element_size() > _LAYER_NORM_MAX_BYTES:
         raise ValueError(f"HIP layer norm needs rows of at most {_LAYER_NORM_MAX_BYTES} bytes (got {H} x {x.dtype})")
-    # the kernel takes both parameters in one type: x's, or fp32
+    # the kernel takes both parameters in one type: x's, or fp32, which holds those of any other 16-bit type
     dtype = x.dtype
-    if any(p is not None and p.dtype == torch.float32 for p in (weight, bias)):
+    if any(p is not None and p.dtype != dtype for p in (weight, bias)):
         dtype = torch.float32
     if weight is not None and not (weight.dtype == dtype and weight.is_contiguous()):
         weight = weight.to(dtype).contiguous()

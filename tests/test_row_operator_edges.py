@@ -667,3 +667,28 @@ def test_temperatures_and_scales_that_32_bits_hold(device):
     for bad in (2.0**-61, 2.0**61, 1e-50, 1e300, math.inf, math.nan, 0.0):
         with pytest.raises(ValueError, match="scale"):
             route_experts(logits, 2, scale=bad)
+
+
+# ------------------------------------------------------------------------------------------------------------------- layer norm
+@pytest.mark.parametrize("device", ON)
+@pytest.mark.parametrize("dtype,weight,bias", [(BF16, FP16, FP16), (BF16, FP16, None), (BF16, None, FP16), (FP16, BF16, FP16),
+                                               (FP16, BF16, FP32), (FP32, BF16, FP16), (BF16, torch.float64, None)])
+def test_layer_norm_parameters_of_other_types_keep_their_bits(device, dtype, weight, bias):
+    """Parameters in a type that is not the input's enter as they are, in 32 bits; their gradients come back in their own type. Sums of 40
+    values in fp32 and half a step of each output's type."""
+    rows, H = 7, 40
+    g = torch.Generator(device=device).manual_seed(16)
+    n = lambda *s: torch.randn(*s, generator=g, device=device)  # noqa: E731
+    x, dy = n(rows, H).to(dtype).requires_grad_(), n(rows, H).to(dtype)
+    w = None if weight is None else (1 + 2.0**-9 * n(H)).to(weight).requires_grad_()  # bits that bf16 does not have
+    b = None if bias is None else (1 + 2.0**-9 * n(H)).to(bias).requires_grad_()
+    y, _ = layer_norm(x, w, b)
+    wide = [None if t is None else t.detach().double().requires_grad_() for t in (x, w, b)]
+    want = torch.nn.functional.layer_norm(wide[0], (H,), wide[1], wide[2], 1e-5)
+    leaves = [(a, r) for a, r in zip((x, w, b), wide) if a is not None]
+    grads = torch.autograd.grad(y, [a for a, _ in leaves], dy)
+    wants = torch.autograd.grad(want, [r for _, r in leaves], dy.double())
+    for got, ref, size in [(y, want, 4.0)] + [(a, r, 4.0 * rows) for a, r in zip(grads, wants)]:
+        tol = torch.finfo(got.dtype).eps / 2 * ref.abs() * (1 + 2**-7) + 64 * U * size
+        assert ((got.double() - ref).abs() <= tol).all()
+    assert all(d.dtype == a.dtype for d, (a, _) in zip(grads, leaves))
