@@ -692,3 +692,64 @@ def test_layer_norm_parameters_of_other_types_keep_their_bits(device, dtype, wei
         tol = torch.finfo(got.dtype).eps / 2 * ref.abs() * (1 + 2**-7) + 64 * U * size
         assert ((got.double() - ref).abs() <= tol).all()
     assert all(d.dtype == a.dtype for d, (a, _) in zip(grads, leaves))
+
+
+# ------------------------------------------------------------------------- alternatives beyond the list of a row (token_logprobs.hip)
+LIST = 2048  # candidates of a row, or of a slice of one, that its block keeps
+
+
+def most_listed(x, rows, k):
+    """Of `rows` rows like those of x: how many elements the fullest block lists: the block's threads take 16-byte chunks in turn, four threads are a group, and what reaches the
+    best key of the k-th best group is listed. Rows are cut into up to 8 slices of at least 32 KiB for 512 blocks in all."""
+    V = x.shape[1]
+    per = 16 // x.element_size()
+    parts = max(1, min(8, 512 // rows, V * x.element_size() // 32768))
+    threads = 512 if parts > 1 else 256
+    chunks = -(-V // per)
+    span = -(-chunks // parts) * per
+    most = 0
+    for row in x.float().cpu():
+        for lo in range(0, V, span):
+            part = row[lo : lo + span]
+            rank = torch.empty(len(part), dtype=torch.int64)
+            rank[torch.sort(part, descending=True, stable=True)[1]] = torch.arange(len(part))
+            group = torch.arange(len(part)) // per % threads // 4
+            best = torch.full((threads // 4,), len(part)).scatter_reduce_(0, group, rank, "amin")
+            most = max(most, best.sort()[0][k - 1].item() + 1)
+    return most
+
+
+def crowded(dtype, rows, device, distinct):
+    """Rows whose best values all lie in the chunks of some neighbouring threads, in every turn of them: 64 threads of fp32, 32 of 16 bits."""
+    per = 4 if dtype == FP32 else 8
+    threads, turns = (512, 80) if rows < 200 else (256, 12)
+    g = torch.Generator(device=device).manual_seed(rows)
+    x = torch.randn(rows, turns, threads, per, generator=g, device=device)
+    few = x[:: max(1, rows // 3), :, 100 : 100 + 256 // per]
+    few[:] = 8.0
+    if distinct:
+        few += torch.rand(*few.shape, generator=g, device=device)
+    return x.reshape(rows, -1)[:, : threads * turns * per - (3 if rows % 2 else 0)].to(dtype)
+
+
+@pytest.mark.parametrize("device", ON)
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("rows,k", [(2, 40), (3, 64), (258, 40), (259, 64)])
+@pytest.mark.parametrize("distinct", [False, True])
+def test_token_logprobs_alternatives_beyond_the_list(device, dtype, rows, k, distinct):
+    x = crowded(dtype, rows, device, distinct)
+    assert most_listed(x[:1], rows, k) > LIST
+    x = x.requires_grad_()
+    tokens = torch.zeros(rows, dtype=torch.int64, device=device)
+    r = token_logprobs(x, tokens, top_k=k)
+    want = torch.sort(x.detach().float(), dim=-1, descending=True, stable=True)[1][:, :k]
+    assert torch.equal(r.top_tokens, want)
+    lp = torch.log_softmax(x.detach().double(), -1)
+    # a thread adds V / 512 or V / 256 values (V / 8 on the host) and 9 levels follow; exponents of up to 14 are rounded
+    n = 80 + x.shape[1] / (256 if device == "cuda" else 8)
+    assert (r.top_logprobs - lp.gather(1, want)).abs().max() < n * U * 4
+    (d,) = torch.autograd.grad(r.top_logprobs.sum(), x)
+    ref = -lp.exp() * k
+    ref.scatter_add_(1, want, torch.ones(rows, k, dtype=torch.float64, device=device))
+    assert ((d.double() - ref).abs() <= torch.finfo(dtype).eps / 2 * ref.abs() * (1 + 2**-7) + U * (n * 4 * lp.exp() * k + 4 * ref.abs())
+            + torch.finfo(dtype).smallest_normal).all()
