@@ -370,9 +370,13 @@ __global__ __launch_bounds__(kBwdThreads) void token_logprobs_bwd_kernel(
     for (int j = 0; j < K; ++j) total += g_top[row * K + j];
   // -p (G + dH (log p + H)) / T = 2^t (c + d t)
   const float inv_t = (float)w.inv_t, share = -st.y * inv_t, cc = share * (total + gh * (st.w - st.z)), dd = share * gh * kLn2;
+  // The exponent's product and its scale are rounded: p is off by up to 1.5 |ln p| 2^-24 of itself. 16-bit gradients do not show it;
+  // in fp32 what the rounding left out multiplies p (777 rows of 50257: 46 to 47 us with and without).
   auto value = [&](float f) {
-    const float t = (f - st.x) * w.scale;
-    return exp2_of(t) * fmaf(dd, fmaxf(t, kFar), cc);
+    const float far = kFar / w.scale, d = sizeof(T) == 4 ? fmaxf(f - st.x, far) : f - st.x, t = d * w.scale;
+    float p = exp2_of(t);
+    if constexpr (sizeof(T) == 4) p = fmaf(p, kLn2 * fmaf(t, w.slack, fmaf(d, w.scale, -t)), p);
+    return p * fmaf(dd, fmaxf(t, kFar), cc);
   };
 #pragma unroll
   for (int u = 0; u < kBwdUnroll; ++u) {

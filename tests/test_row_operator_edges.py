@@ -753,3 +753,22 @@ def test_token_logprobs_alternatives_beyond_the_list(device, dtype, rows, k, dis
     ref.scatter_add_(1, want, torch.ones(rows, k, dtype=torch.float64, device=device))
     assert ((d.double() - ref).abs() <= torch.finfo(dtype).eps / 2 * ref.abs() * (1 + 2**-7) + U * (n * 4 * lp.exp() * k + 4 * ref.abs())
             + torch.finfo(dtype).smallest_normal).all()
+
+
+@gpu
+@pytest.mark.parametrize("T", [1.0, 0.7, 1.3])
+@pytest.mark.parametrize("top", [0.0, 3.3])
+def test_token_logprobs_small_probabilities_are_as_exact_as_large_ones(T, top):
+    """dlogits_i = -p_i / T in fp32: exp2's step, the sum's and the quotients' make 24 U of p_i, and the difference to the largest logit |z| U,
+    which is exact where that is 0. The exponent's product and scale are not rounded besides."""
+    rows, V = 64, 256
+    g = torch.Generator(device="cuda").manual_seed(17)
+    x = -75 * T * torch.rand(rows, V, generator=g, device="cuda")
+    x[:, 0] = 0
+    x = (x + top).requires_grad_()
+    tokens = torch.zeros(rows, dtype=torch.int64, device="cuda")
+    (d,) = torch.autograd.grad(token_logprobs(x, tokens, temperature=T).logprobs.sum(), x)
+    z = x.detach().double() / T
+    want = -torch.softmax(z, -1) / T
+    tol = U * (24 + (z - z.amax(-1, keepdim=True)).abs() * (top != 0)) * want.abs()
+    assert ((d - want).abs() <= tol)[:, 1:].all(), ((d - want).abs() / (U * want.abs()))[:, 1:].max()
