@@ -318,17 +318,21 @@ __global__ __launch_bounds__(kThreads) void route_fwd_kernel(const T* __restrict
     choose<V, double>(f, bias, sh, false, a);
   }
 
-  // The weights, a choice in each lane. Shares are of the chosen alone, formed against the largest logit among them: that may lie any
-  // distance below the row's, where a bias or closed groups keep others out.
+  // The weights, a choice in each lane. Shares are of the chosen alone, formed against the largest logit among them (`top`): that may
+  // lie any distance below the row's (`hi`), where a bias or closed groups keep others out. Else the first choice has both.
   const int id = lane < a.k ? sh.chosen[lane] : 0;
   const float v = to_f<T>(x[id]);
-  const float top = a.renorm ? wave_reduce<OpMax>(lane < a.k ? v : -INFINITY) : 0.f;
+  float top = lane_value(v, 0);
+  if (a.renorm && !by_logit) top = wave_reduce<OpMax>(lane < a.k ? v : -INFINITY);
   float w;
   if (a.softmax) {
-    float hi = f[0];
+    float hi = top;
+    if (!by_logit) {
+      hi = f[0];
 #pragma unroll
-    for (int i = 1; i < V; ++i) hi = fmaxf(hi, f[i]);
-    hi = wave_reduce<OpMax>(hi);
+      for (int i = 1; i < V; ++i) hi = fmaxf(hi, f[i]);
+      hi = wave_reduce<OpMax>(hi);
+    }
     float all = 0.f;  // also: NaN where a logit is NaN or +inf, or all are -inf
 #pragma unroll
     for (int i = 0; i < V; ++i) all += exp_of(f[i] - hi);
@@ -341,7 +345,7 @@ __global__ __launch_bounds__(kThreads) void route_fwd_kernel(const T* __restrict
   } else if (a.renorm) {
     // s_j over the best score, up to a factor that all share: e^(v - min(top, 0)) / (1 + e^v)
     const bool none = top < kNoScore && !__any(lane < a.k && v != v);
-    w = lane < a.k && !none ? (v > 0.f ? sigmoid_of(v) : exp_of(v - fminf(top, 0.f)) / (1.f + exp_of(v))) : 0.f;
+    w = lane < a.k && !none ? (v > 0.f ? 1.f : exp_of(v - fminf(top, 0.f))) * __builtin_amdgcn_rcpf(1.f + exp_of(-fabsf(v))) : 0.f;
     const float sum = wave_reduce<OpSum>(w);
     w = none ? 0.f : w / sum;
   } else {
