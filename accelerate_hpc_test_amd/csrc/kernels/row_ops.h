@@ -192,7 +192,6 @@ struct OpMax {
   static __device__ __forceinline__ float of(float a, float b) { return fmaxf(a, b); }
 };
 struct OpMaxU32 { static __device__ __forceinline__ uint32_t of(uint32_t a, uint32_t b) { return a > b ? a : b; } };
-struct OpOr { static __device__ __forceinline__ uint32_t of(uint32_t a, uint32_t b) { return a | b; } };
 
 template <int L, typename Op>
 __device__ __forceinline__ float lanes_reduce(float v) { return __uint_as_float(lanes_reduce_u32<L, Op>(__float_as_uint(v))); }
@@ -200,8 +199,6 @@ template <typename Op>
 __device__ __forceinline__ float wave_reduce(float v) { return lanes_reduce<64, Op>(v); }
 template <int L>
 __device__ __forceinline__ uint32_t lanes_max_u32(uint32_t v) { return lanes_reduce_u32<L, OpMaxU32>(v); }
-template <int L>
-__device__ __forceinline__ uint32_t lanes_or(uint32_t v) { return lanes_reduce_u32<L, OpOr>(v); }
 
 // The same over THREADS threads: lanes of a wave, or the threads of a block. `slots`: 16 floats of shared memory that no other
 // reduction uses between two barriers of the block.
