@@ -59,11 +59,12 @@ def route_experts(logits: torch.Tensor, top_k: int, scoring: str = "softmax", bi
                   n_groups: int = 1, topk_groups: int = 1, renormalize: bool = True, scale: float = 1.0):
     """The `top_k` experts of each token and their weights from router logits [T, E] (bf16, fp16 or fp32).
 
-    Scores are softmax(logits) or sigmoid(logits) (`scoring`). Experts are chosen by score + `bias` ([E], optional: it steers the
-    choice alone, balances the load, and gets no gradient), within the `topk_groups` of `n_groups` equal groups whose two best
-    keys have the largest sum; equal keys go to the lower index, keys are compared in 64 bits. Weights are the chosen scores,
-    divided by their sum (`renormalize`; scores that are all 0 in 32 bits give 0), times `scale`. Returns (weights fp32 [T, k], experts int64 [T, k]) in falling order of
-    the keys; the weights are differentiable with respect to the logits."""
+    Scores are softmax(logits) or sigmoid(logits) (`scoring`). Experts are chosen by score + `bias` ([E], optional, in 32 bits: it
+    steers the choice alone, balances the load, and gets no gradient), within the `topk_groups` of `n_groups` equal groups whose two
+    best keys have the largest sum; equal keys go to the lower index, keys are compared in 64 bits. Weights are the chosen scores,
+    divided by their sum (`renormalize`; scores that are all 0 in 32 bits give 0), times `scale` (2^-60 to 2^60 in size). Returns
+    (weights fp32 [T, k], experts int64 [T, k]) in falling order of the keys; the weights are differentiable with respect to the
+    logits, on a GPU once."""
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise ValueError(f"route_experts: logits must be [tokens, experts], got shape {tuple(logits.shape)}")
     if not logits.is_floating_point():
@@ -80,13 +81,13 @@ def route_experts(logits: torch.Tensor, top_k: int, scoring: str = "softmax", bi
     if bias is not None:
         if bias.shape != (E,) or bias.device != logits.device:
             raise ValueError(f"route_experts: bias must be a [{E}] tensor on the logits' device")
-        bias = bias.detach()
+        bias = bias.detach() if logits.dtype == torch.float64 else bias.detach().float()
     if not (use_native(logits) and logits.dtype in ROW_DTYPES) or forward_mode(logits):
         return route_experts_reference(logits, top_k, scoring, bias, n_groups, topk_groups, renormalize, scale)
     if E > MAX_EXPERTS or top_k > MAX_TOP_K or n_groups > MAX_GROUPS:
         raise ValueError(f"HIP route_experts takes at most {MAX_EXPERTS} experts, {MAX_TOP_K} choices and {MAX_GROUPS} groups "
                          f"(got {E}, {top_k}, {n_groups})")
     if bias is not None:
-        bias = bias.float().contiguous()
+        bias = bias.contiguous()
     w, ids = ext().route_experts(logits, top_k, scoring == "softmax", bias, n_groups, topk_groups, renormalize, scale)
     return w, ids

@@ -772,3 +772,16 @@ def test_token_logprobs_small_probabilities_are_as_exact_as_large_ones(T, top):
     want = -torch.softmax(z, -1) / T
     tol = U * (24 + (z - z.amax(-1, keepdim=True)).abs() * (top != 0)) * want.abs()
     assert ((d - want).abs() <= tol)[:, 1:].all(), ((d - want).abs() / (U * want.abs()))[:, 1:].max()
+
+
+@pytest.mark.parametrize("device", ON)
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+def test_route_experts_bias_enters_in_32_bits_on_every_device(device, dtype):
+    """A bias in 64 bits whose entries 32 bits do not tell apart: a tie, which goes to the lower index."""
+    x = torch.zeros(3, 16, device=device, dtype=dtype)
+    bias = torch.ones(16, dtype=torch.float64, device=device)
+    bias[9] += 2.0**-40
+    assert route_experts(x, 2, "sigmoid", bias)[1].tolist() == [[0, 1]] * 3
+    assert route_experts(x, 2, "softmax", bias, 4, 1)[1].tolist() == [[0, 1]] * 3
+    bias[9] += 2.0**-20
+    assert route_experts(x, 2, "sigmoid", bias)[1].tolist() == [[9, 0]] * 3
