@@ -785,3 +785,91 @@ def test_route_experts_bias_enters_in_32_bits_on_every_device(device, dtype):
     assert route_experts(x, 2, "softmax", bias, 4, 1)[1].tolist() == [[0, 1]] * 3
     bias[9] += 2.0**-20
     assert route_experts(x, 2, "sigmoid", bias)[1].tolist() == [[9, 0]] * 3
+
+
+# ------------------------------------------------------------------------------------------------------- offsets past 32 bits
+def ends(rows, count=3):
+    """The first and last rows, and those about element 2^31 and 2^32 of rows of the given width."""
+    return lambda width: sorted({r for at in (0, 2**31 // width, 2**32 // width, rows - 1) for r in range(at - count, at + count) if 0 <= r < rows})
+
+
+@gpu
+def test_layer_norm_past_32_bit_offsets():
+    rows, H = 2**32 // 4096 + 70, 4096  # 4.3e9 elements a tensor, 8.6 GB
+    g = torch.Generator(device="cuda").manual_seed(18)
+    some = torch.randn(64, H, generator=g, device="cuda").to(BF16)
+    x = torch.empty(rows, H, dtype=BF16, device="cuda")
+    x.view(-1, 2, H)[:] = some[:2]  # every row one of two
+    at = ends(rows)(H)
+    for i, r in enumerate(at):
+        x[r] = some[i + 2]
+    x.requires_grad_()
+    w = (1 + 0.2 * torch.randn(H, generator=g, device="cuda")).to(BF16)
+    y, _ = layer_norm(x, w)
+    (d,) = torch.autograd.grad(y, x, x.detach())
+    # as many rows as take the same forward: below 1024 the statistics are summed by more threads, in another order
+    small = x.detach()[at + list(range(1100))].clone().requires_grad_()
+    ys, _ = layer_norm(small, w)
+    (ds,) = torch.autograd.grad(ys, small, small.detach())
+    assert torch.equal(y[at], ys[: len(at)]) and torch.equal(d[at], ds[: len(at)])
+
+
+@gpu
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rope_past_32_bit_offsets(interleaved):
+    B, S, H, D = 2, 2**32 // (2 * 48 * 128) + 40, 48, 128
+    cos, sin = rope_tables(64, D, 10000.0, "cuda")
+    x = torch.empty(B, S, H, D, dtype=BF16, device="cuda")
+    x[:] = torch.randn(H, D, generator=torch.Generator(device="cuda").manual_seed(19), device="cuda").to(BF16)
+    pos = (torch.arange(B * S, device="cuda") % 64).view(B, S)
+    out = apply_rope(x, cos, sin, 40, pos, interleaved=interleaved).view(B * S, H, D)
+    want = apply_rope(x[:1, :64].contiguous(), cos, sin, 40, interleaved=interleaved)[0]
+    at = torch.tensor(ends(B * S)(H * D), device="cuda")
+    assert torch.equal(out[at], want[at % 64])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_token_logprobs_past_32_bit_offsets(dtype):
+    V = 128256 if dtype == BF16 else 50257
+    rows = (2**32 if dtype == BF16 else 2**31) // V + 30
+    g = torch.Generator(device="cuda").manual_seed(20)
+    some = torch.randn(300, V, generator=g, device="cuda").to(dtype)
+    x = torch.empty(rows, V, dtype=dtype, device="cuda")
+    x[:] = some[0]
+    at = ends(rows)(V)
+    for i, r in enumerate(at):
+        x[r] = some[i + 1]
+    tokens = (torch.arange(rows, device="cuda") * 7919) % V
+    x.requires_grad_()
+    r = token_logprobs(x, tokens, top_k=3)
+    (d,) = torch.autograd.grad(r.logprobs.sum() + r.entropy.sum(), x)
+    small = some.clone()  # as many rows as are not cut into slices
+    small[: len(at)] = x.detach()[at]
+    small_tokens = torch.zeros(300, dtype=torch.int64, device="cuda")
+    small_tokens[: len(at)] = tokens[at]
+    small.requires_grad_()
+    s = token_logprobs(small, small_tokens, top_k=3)
+    (ds,) = torch.autograd.grad(s.logprobs.sum() + s.entropy.sum(), small)
+    for a, b in zip(r, s):
+        assert torch.equal(a[at], b[: len(at)])
+    assert torch.equal(d[at], ds[: len(at)])
+
+
+@gpu
+def test_route_experts_past_32_bit_offsets():
+    rows, E = 2**32 // 1024 + 40, 1024
+    g = torch.Generator(device="cuda").manual_seed(21)
+    some = torch.randn(64, E, generator=g, device="cuda").to(BF16)
+    x = torch.empty(rows, E, dtype=BF16, device="cuda")
+    x[:] = some[0]
+    at = ends(rows)(E)
+    for i, r in enumerate(at):
+        x[r] = some[i + 1]
+    x.requires_grad_()
+    w, ids = route_experts(x, 4)
+    (d,) = torch.autograd.grad(w[:, 0].sum(), x)
+    small = x.detach()[at].clone().requires_grad_()
+    ws, idss = route_experts(small, 4)
+    (ds,) = torch.autograd.grad(ws[:, 0].sum(), small)
+    assert torch.equal(w[at], ws) and torch.equal(ids[at], idss) and torch.equal(d[at], ds)
