@@ -873,3 +873,25 @@ def test_route_experts_past_32_bit_offsets():
     ws, idss = route_experts(small, 4)
     (ds,) = torch.autograd.grad(ws[:, 0].sum(), small)
     assert torch.equal(w[at], ws) and torch.equal(ids[at], idss) and torch.equal(d[at], ds)
+
+
+@pytest.mark.parametrize("device", ON)
+@pytest.mark.parametrize("dtype", [FP32, FP16, BF16])
+@pytest.mark.parametrize("rows", [3, 300])  # in slices, and whole
+@pytest.mark.parametrize("at", [0, 70001, -1])
+def test_token_logprobs_many_small_probabilities_beside_a_large_one(device, dtype, rows, at):
+    """One likely token and 160000 others of less than half an fp32 step of it each: a thread that adds them one by one to its sum loses all of its
+    own. In turns of 32 values, V / (256 * 16) turns, 9 levels and 20 roundings of the rest: 100 U of S, and of U, whose terms are 18
+    times as large."""
+    V = 160001
+    x = torch.full((rows, V), -17.5, device=device, dtype=dtype)  # e^-17.5 = 0.84 * 2^-25, and a number of every type
+    x[:, at] = 0.0
+    tokens = torch.full((rows,), at % V, dtype=torch.int64, device=device)
+    r = token_logprobs(x, tokens, top_k=2)
+    e = math.exp(-17.5)
+    S = 1 + (V - 1) * e
+    H = math.log(S) + 17.5 * (V - 1) * e / S
+    tol = (100 if device == "cuda" else 100 + V / 8) * U
+    assert (r.logprobs.double() + math.log(S)).abs().max() <= tol
+    assert (r.top_logprobs[:, 1].double() + 17.5 + math.log(S)).abs().max() <= tol + 18 * U
+    assert (r.entropy.double() - H).abs().max() <= 20 * tol * (S - 1 if device == "cuda" else 1) + tol
