@@ -406,6 +406,20 @@ def rope_reference(qkv, cos, sin, n_rot_heads, positions=None, interleaved=False
     return torch.cat([out, qkv[..., n_rot_heads:, :]], dim=-2)
 
 
+def _fit_positions(positions, want, device, flat):
+    """`positions` as int64 of shape `want` on `device`: broadcast, or (`flat`: of any shape) a token after the other."""
+    if positions.is_floating_point() or positions.is_complex() or positions.dtype == torch.bool:
+        raise TypeError(f"apply_rope: positions must be integers, got {positions.dtype}")
+    if positions.device != device and positions.device.type != "cpu":
+        raise ValueError(f"apply_rope: positions must be on qkv's device ({device}) or the host, got {positions.device}")
+    positions = positions.to(device, torch.int64)
+    if positions.dim() <= len(want) and all(p in (1, w) for p, w in zip(positions.shape[::-1], want[::-1])):
+        return positions.expand(want)
+    if positions.numel() == math.prod(want) and (positions.dim() == 1 or flat):
+        return positions.reshape(want)
+    raise ValueError(f"apply_rope: positions must be {want}, or broadcast to it, got {tuple(positions.shape)}")
+
+
 def apply_rope(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, n_rot_heads: int, positions=None,
                interleaved: bool = False, rotary_dim: Optional[int] = None):
     """qkv: [..., S, Htot, D]; rotates the first `n_rot_heads` heads (Q heads then K heads) by the fp32 tables cos / sin
@@ -414,56 +428,49 @@ def apply_rope(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, n_rot_he
     `rotary_dim`: R, the rotated first values of each head, even; None rotates the whole head. `positions`: integers [..., S]
     (or [1, S], [S] for every batch row), each token's row of the tables; None counts from 0. The tables lie on qkv's device, the
     positions there or on the host. The result is a new contiguous tensor. On a GPU any strides and even R are taken, in bf16,
-    fp16 and fp32, with D up to 1000 (whole heads in halves: any D); a position outside the tables gives NaN in its rotated values. Tables that require
-    gradients get them, and 64-bit tables are used as such, in torch operations. On a GPU heads rotated whole in halves can be
-    differentiated any number of times, the other forms once."""
-    S, Htot, D = qkv.shape[-3:]
+    fp16 and fp32, with D up to 1000 (whole heads in halves: any D); a position outside the tables gives NaN in its rotated
+    values. Tables that require gradients get them, and 64-bit tables are used as such, in torch operations. On a GPU heads
+    rotated whole in halves can be differentiated any number of times, the other forms once."""
+    *lead, S, Htot, D = shape = qkv.shape
+    table = cos.shape
+    device, dtype = qkv.device, qkv.dtype
     R = D if rotary_dim is None else rotary_dim
     if R < 2 or R % 2 or R > D:
         raise ValueError(f"apply_rope: the rotated part must be even and within the head ({R} of {D})")
-    if cos.dim() != 2 or cos.shape != sin.shape or cos.shape[1] != R // 2:
-        raise ValueError(f"apply_rope: cos and sin must be [positions, {R // 2}] tables, got {tuple(cos.shape)}, {tuple(sin.shape)}")
+    if len(table) != 2 or sin.shape != table or table[1] != R // 2:
+        raise ValueError(f"apply_rope: cos and sin must be [positions, {R // 2}] tables, got {tuple(table)}, {tuple(sin.shape)}")
     if not 0 <= n_rot_heads <= Htot:
         raise ValueError(f"apply_rope: {n_rot_heads} of {Htot} heads to rotate")
-    if cos.device != qkv.device or sin.device != qkv.device:
-        raise ValueError(f"apply_rope: cos and sin must be on qkv's device ({qkv.device}), got {cos.device}, {sin.device}")
-    lead = qkv.shape[:-3]
-    whole = qkv.dtype == torch.bfloat16 and D % 8 == 0 and R == D and not interleaved
-    if positions is not None:
-        if positions.is_floating_point() or positions.is_complex() or positions.dtype == torch.bool:
-            raise TypeError(f"apply_rope: positions must be integers, got {positions.dtype}")
-        if positions.device != qkv.device and positions.device.type != "cpu":
-            raise ValueError(f"apply_rope: positions must be on qkv's device ({qkv.device}) or the host, got {positions.device}")
-        positions = positions.to(qkv.device, torch.int64)
-        want = (*lead, S)
-        if positions.shape != want:
-            if positions.dim() <= len(want) and all(p in (1, w) for p, w in zip(positions.shape[::-1], want[::-1])):
-                positions = positions.expand(want)
-            elif positions.numel() == math.prod(want) and (positions.dim() == 1 or (whole and qkv.is_cuda)):
-                positions = positions.reshape(want)  # a token after the other
-            else:
-                raise ValueError(f"apply_rope: positions must be {want}, or broadcast to it, got {tuple(positions.shape)}")
-    if positions is None and S > cos.shape[0]:
-        raise ValueError(f"apply_rope: {S} tokens, but tables for {cos.shape[0]} positions")
-    # the kernels read 32-bit tables, and have no gradient for them
-    torch_tables = torch.float64 in (cos.dtype, sin.dtype) or (torch.is_grad_enabled() and (cos.requires_grad or sin.requires_grad))
-    if torch_tables or not (use_native(qkv) and qkv.dtype in ROW_DTYPES) or forward_mode(qkv, cos, sin):
-        return rope_reference(qkv, cos, sin, n_rot_heads, positions, interleaved, rotary_dim)
-    # `whole`: bf16 heads rotated whole in halves have their own kernel (csrc/kernels/norm_act.hip), which copies V heads in the same pass
-    if D > 1000 and not whole:  # wider than a block of the other kernel
-        if R == D and not interleaved:
-            return rope_reference(qkv, cos, sin, n_rot_heads, positions)
-        raise ValueError(f"HIP rope needs a head size of at most 1000 (got {D})")
+    if cos.device != device or sin.device != device:
+        raise ValueError(f"apply_rope: cos and sin must be on qkv's device ({device}), got {cos.device}, {sin.device}")
+    # bf16 heads rotated whole in halves have their own kernel (csrc/kernels/norm_act.hip), which copies V heads in the same pass
+    whole = R == D and not interleaved and dtype is torch.bfloat16 and D % 8 == 0
     if positions is None:
+        if S > table[0]:
+            raise ValueError(f"apply_rope: {S} tokens, but tables for {table[0]} positions")
+    elif positions.dtype is not torch.int64 or positions.shape != (*lead, S) or positions.device != device:
+        positions = _fit_positions(positions, (*lead, S), device, flat=whole and qkv.is_cuda)
+    # the kernels read 32-bit tables, and have no gradient for them
+    wide = cos.dtype is torch.float64 or sin.dtype is torch.float64
+    learned = (cos.requires_grad or sin.requires_grad) and torch.is_grad_enabled()
+    # wider than a block of the kernel for every layout
+    too_wide = D > 1000 and not whole
+    if wide or learned or not (use_native(qkv) and dtype in ROW_DTYPES) or forward_mode(qkv, cos, sin) or (
+        too_wide and R == D and not interleaved
+    ):
+        return rope_reference(qkv, cos, sin, n_rot_heads, positions, interleaved, rotary_dim)
+    if too_wide:
+        raise ValueError(f"HIP rope needs a head size of at most 1000 (got {D})")
+    if positions is None and table[0] != S:
         cos, sin = cos[:S], sin[:S]  # one row per token of the sequence
-    if cos.dtype != torch.float32 or sin.dtype != torch.float32:
+    if cos.dtype is not torch.float32 or sin.dtype is not torch.float32:
         cos, sin = cos.float(), sin.float()
     cos, sin = cos.contiguous(), sin.contiguous()
     if len(lead) == 1:
         return ext().rope(qkv, cos, sin, positions, n_rot_heads, interleaved, whole)
     B = math.prod(lead)
     positions = None if positions is None else positions.reshape(B, S)
-    return ext().rope(qkv.reshape(B, S, Htot, D), cos, sin, positions, n_rot_heads, interleaved, whole).view(qkv.shape)
+    return ext().rope(qkv.reshape(B, S, Htot, D), cos, sin, positions, n_rot_heads, interleaved, whole).view(shape)
 
 
 # ----------------------------------------------------------------------------------------------------------
