@@ -182,19 +182,27 @@ def rope_scaling(cfg: LlamaConfig) -> Optional[dict]:
     return scaling
 
 
-def rope_length(model, S: int, position_ids=None) -> Optional[int]:
-    """The length of the sequence that a forward's S tokens belong to, where the tables depend on it ("dynamic" scaling), else None. A shard
-    of a context- or sequence-parallel group counts the whole sequence; given positions count up to the furthest (read on the
-    host, as their frequencies are made there)."""
-    scaling = model.config.rope_scaling
-    if scaling is None or scaling.get("rope_type", scaling.get("type")) != "dynamic":
-        return None
-    if getattr(model, "_cp_seq_len", None):
-        return int(model._cp_seq_len)
-    shards = getattr(model, "_seq_parallel_factor", 1)
-    if shards > 1 or position_ids is None or position_ids.numel() == 0:
-        return S * shards
-    return int(position_ids.max()) + 1
+def model_rope(model, S: int, rows: int, position_ids, device):
+    """The cos / sin tables of a forward with S tokens, of at least `rows` positions, kept in the model's `_rope_cache`. "dynamic" scaling
+    goes by the length of the sequence that the tokens belong to: all of it for a shard of a context- or sequence-parallel
+    group, else up to the furthest of given positions (read on the host, where the tables are made)."""
+    cfg, cache = model.config, model._rope_cache
+    scaling = rope_scaling(cfg)
+    length, given = None, False
+    if scaling is not None and scaling.get("rope_type", scaling.get("type")) == "dynamic":
+        shards = getattr(model, "_seq_parallel_factor", 1)
+        whole = getattr(model, "_cp_seq_len", None)
+        given = position_ids is not None and position_ids.numel() > 0 and shards == 1 and not whole
+        length = int(position_ids.max()) + 1 if given else whole or S * shards
+        length = max(length, scaling["original_max_position_embeddings"])  # the frequencies change past it only
+        rows = length if given else max(rows, S * shards)
+    key = (rows, str(device), length, given)
+    if key not in cache:
+        if given:  # such lengths vary without end, their tables are not all kept (a captured graph holds none of them)
+            for old in [k for k in cache if k[3]][:-8]:
+                del cache[old]
+        cache[key] = rope_tables(rows, cfg.rotary_dim, cfg.rope_theta, device, scaling, length)
+    return cache[key]
 
 
 @dataclass
@@ -236,13 +244,6 @@ class LlamaForCausalLM(nn.Module):
             elif isinstance(m, RMSNorm):
                 m.weight.fill_(1.0)
 
-    def _rope(self, S, device, length=None):
-        key = (S, str(device), length)
-        if key not in self._rope_cache:
-            n = max(S, self.config.max_position_embeddings if S > self.config.max_position_embeddings else S)
-            self._rope_cache[key] = rope_tables(n, self.config.rotary_dim, self.config.rope_theta, device, rope_scaling(self.config), length)
-        return self._rope_cache[key]
-
     def forward(self, input_ids, labels=None, position_ids=None, attention_mask=None, return_logits: bool = True,
                 shift_labels=None):
         """`labels` are shifted inside (HF convention). Under context/sequence parallelism pass `shift_labels`
@@ -254,8 +255,7 @@ class LlamaForCausalLM(nn.Module):
         if position_ids is not None:
             rope_len = max(int(self.config.max_position_embeddings), getattr(self, "_cp_seq_len", None) or 0,
                            S * getattr(self, "_seq_parallel_factor", 1))
-        length = rope_length(self, S, position_ids)
-        cos, sin = self._rope(max(rope_len, length or 0), input_ids.device, length)
+        cos, sin = model_rope(self, S, rope_len, position_ids, input_ids.device)
         h = self.embed_tokens(input_ids)
         dt = self.layers[0].self_attn.qkv_proj.weight.dtype if len(self.layers) else h.dtype
         if h.device.type in ("cuda", "cpu") and torch.is_autocast_enabled(h.device.type):

@@ -15,8 +15,8 @@ from typing import Optional
 import torch
 import torch.nn as nn
 
-from ..ops.fused import cross_entropy, rope_tables
-from .llama import CausalLMOutput, LlamaAttention, LlamaConfig, RMSNorm, rope_length, rope_scaling
+from ..ops.fused import cross_entropy
+from .llama import CausalLMOutput, LlamaAttention, LlamaConfig, RMSNorm, model_rope
 from .moe import MoEExperts, MoELayer, load_balancing_loss
 
 
@@ -143,18 +143,11 @@ class MixtralForCausalLM(nn.Module):
         self._ep_group = group
         return mods
 
-    def _rope(self, S, device, length=None):
-        key = (S, str(device), length)
-        if key not in self._rope_cache:
-            self._rope_cache[key] = rope_tables(S, self.config.rotary_dim, self.config.rope_theta, device, rope_scaling(self.config), length)
-        return self._rope_cache[key]
-
     def forward(self, input_ids, labels=None, position_ids=None, attention_mask=None, return_logits: bool = True,
                 shift_labels=None, output_router_logits: Optional[bool] = None):
         B, S = input_ids.shape
         rope_len = S if position_ids is None else max(S, int(self.config.max_position_embeddings))
-        length = rope_length(self, S, position_ids)
-        cos, sin = self._rope(max(rope_len, length or 0), input_ids.device, length)
+        cos, sin = model_rope(self, S, rope_len, position_ids, input_ids.device)
         h = self.embed_tokens(input_ids)
         dt = self.layers[0].self_attn.qkv_proj.weight.dtype if len(self.layers) else h.dtype
         if h.device.type in ("cuda", "cpu") and torch.is_autocast_enabled(h.device.type):

@@ -895,3 +895,18 @@ def test_token_logprobs_many_small_probabilities_beside_a_large_one(device, dtyp
     assert (r.logprobs.double() + math.log(S)).abs().max() <= tol
     assert (r.top_logprobs[:, 1].double() + 17.5 + math.log(S)).abs().max() <= tol + 18 * U
     assert (r.entropy.double() - H).abs().max() <= 20 * tol * (S - 1 if device == "cuda" else 1) + tol
+
+
+@pytest.mark.parametrize("kind", ["llama", "mixtral"])
+def test_dynamic_tables_of_many_lengths_are_not_all_kept(kind):
+    """Batches whose furthest position varies: sequences within the original length share one table, longer ones keep a few, each with the rows
+    that it needs."""
+    model = tiny_model(kind, {"rope_type": "dynamic", "factor": 2.0, "original_max_position_embeddings": 64}, max_position_embeddings=4096)
+    ids = torch.randint(0, 64, (1, 8), generator=torch.Generator().manual_seed(1))
+    with torch.no_grad():
+        for last in list(range(8, 60, 5)) + [63]:
+            model(ids, position_ids=torch.arange(last - 7, last + 1)[None])
+        assert len(model._rope_cache) == 1
+        for last in range(64, 160, 3):
+            model(ids, position_ids=torch.arange(last - 7, last + 1)[None])
+    assert len(model._rope_cache) <= 10 and sum(c.shape[0] for c, _ in model._rope_cache.values()) <= 10 * 160
