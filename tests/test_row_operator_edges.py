@@ -910,3 +910,11 @@ def test_dynamic_tables_of_many_lengths_are_not_all_kept(kind):
         for last in range(64, 160, 3):
             model(ids, position_ids=torch.arange(last - 7, last + 1)[None])
     assert len(model._rope_cache) <= 10 and sum(c.shape[0] for c, _ in model._rope_cache.values()) <= 10 * 160
+
+
+@gpu
+@pytest.mark.parametrize("rows,hidden,dtype", [(1200, 32768, BF16), (1100, 20001, FP16), (1300, 16384, FP32), (1027, 16383, FP32)])
+def test_layer_norm_many_of_the_widest_rows(rows, hidden, dtype):
+    from test_row_operators import run_norm
+
+    run_norm("cuda", rows, hidden, dtype, True, "both")
