@@ -11,11 +11,11 @@
 //   * keys are order-preserving unsigned integers; NaN sorts as -inf, a closed expert is 0;
 //   * a bisection over key values, counting by ballots, finds a bound that a few more than k keys reach (a handful of steps);
 //   * those are compacted in the order of their experts, and each counts the ones before it: that is its rank.
-// 16384 tokens with 256 experts in 8 groups, k = 8: 19.6 us (k rounds of a maximum over the lanes: 28.9 us; keys in 64 bits
-// throughout: 32.7 us), 64 tokens: 4.6 us. The order must not hang on a rounding of exp: where keys are sums of scores and a bias, a wave chooses by
-// keys in 32 bits, and does it again in 64 where two neighbours of the order, or the last open and the first closed group,
-// lie within the rounding errors of 32 (6 tokens in 10000 with distinct logits). Where keys are scores alone (no bias, no
-// closed groups) their order is the logits' own, and exact.
+// 16384 tokens with 256 experts in 8 groups, k = 8: 20.3 us (k rounds of a maximum over the lanes: 28.9 us; keys in 64 bits
+// throughout: 32.7 us), 64 tokens: 5.1 us. The order must not hang on a rounding of exp: where keys are sums of scores and a bias,
+// a wave chooses by keys in 32 bits, and does it again in 64 where two neighbours of the order, or the last open and the first
+// closed group, lie within the rounding errors of 32 (6 tokens in 10000 with distinct logits). Where keys are scores alone (no
+// bias, no closed groups) their order is the logits' own, and exact.
 #include <hip/hip_runtime.h>
 #include <torch/extension.h>
 #include <ATen/hip/HIPContext.h>
