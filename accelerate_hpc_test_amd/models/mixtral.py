@@ -168,9 +168,9 @@ class MixtralForCausalLM(nn.Module):
             want_aux = self.config.output_router_logits if output_router_logits is None else output_router_logits
             if want_aux and self.config.router_aux_loss_coef > 0:
                 routers = [l.block_sparse_moe for l in self.layers]
-                choices = None if all(r.plain_routing for r in routers) else [r.last_router_choice for r in routers]
                 aux = load_balancing_loss([r.last_router_logits for r in routers], self.config.num_local_experts,
-                                          self.config.num_experts_per_tok, choices, self.config.router_scoring)
+                                          self.config.num_experts_per_tok, [r.last_router_choice for r in routers],
+                                          self.config.router_scoring)
                 loss = loss + self.config.router_aux_loss_coef * aux.to(loss.dtype)
         for l in self.layers:
             l.block_sparse_moe.last_router_logits = l.block_sparse_moe.last_router_choice = None

@@ -563,7 +563,7 @@ class MoELayer(nn.Module):
         logits = self.gate(t)
         self.last_router_logits = logits
         w, idx = self._route(logits)
-        self.last_router_choice = None if self.plain_routing else idx
+        self.last_router_choice = None if self.plain_routing and self.router_bias is None else idx
         w = w.to(t.dtype)
         flat_e = idx.reshape(-1)
         if self.ep_group is None or comm.group_size(self.ep_group) == 1:
@@ -674,13 +674,16 @@ def _attach_bounds(seg):
 def load_balancing_loss(router_logits: list, num_experts: int, top_k: int, choices: Optional[list] = None,
                         scoring: str = "softmax") -> torch.Tensor:
     """Switch-style auxiliary loss (HF `load_balancing_loss_func`): E · Σ_e f_e · P_e over all layers' tokens. `choices`: the experts
-    [T, k] that each layer's router chose, where that is not the plain top-k of its softmax; P is of its scores, summed to 1."""
+    [T, k] that each layer's router chose, None for one that took the plain top-k; P is of its scores, summed to 1."""
     logits = torch.cat([l.float() for l in router_logits], 0)
     if scoring == "softmax":
         probs = torch.softmax(logits, -1)
     else:
         probs = torch.softmax(F.logsigmoid(logits), -1)  # sigmoid scores over their sum
-    sel = torch.topk(probs, top_k, -1)[1] if choices is None else torch.cat(choices, 0)
+    sel = torch.topk(probs, top_k, -1)[1]
+    if choices is not None:
+        plain = sel.split([l.shape[0] for l in router_logits])
+        sel = torch.cat([p if c is None else c for p, c in zip(plain, choices)], 0)
     mask = F.one_hot(sel, num_experts).float()  # [T, k, E]
     tokens_per_expert = mask.mean(0)  # [k, E]
     prob_per_expert = probs.mean(0)  # [E]
